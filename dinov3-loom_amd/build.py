@@ -1,7 +1,7 @@
 """Build recipe for libdinov3_hrx.so: every HIP kernel and host source of the
 forward pass is compiled with hipcc for gfx950 (wave64) and linked into one
 shared library that exports the C ABI of include/dinov3.h and
-include/dinov3_engine.h; the command-line front end lib/dinov3-hrx
+include/dinov3_engine.h and include/dinov3_packed.h; the command-line front end lib/dinov3-hrx
 (csrc/cli.cpp) links against it. The machine-ceiling probes
 (csrc/kernels/probe.hip, include/dinov3_probe.h) go into a library of their
 own, lib/libdinov3_probe.so, which only bench.py and the tests load.
@@ -29,8 +29,12 @@ SOURCES = [
     "kernels/gemm.hip",
     "kernels/attention.hip",
     "kernels/norm.hip",
+    "kernels/packed_attention.hip",
+    "kernels/packed_linear.hip",
+    "kernels/packed_rotate.hip",
     "engine.cpp",
     "model.cpp",
+    "packed.cpp",
     "host_copy.cpp",
     "weights.cpp",
     "safetensors.cpp",

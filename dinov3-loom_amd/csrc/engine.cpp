@@ -426,6 +426,8 @@ void engine_check(dhx_engine* e, hipError_t err, const char* what) { hip_check(e
 
 void engine_ensure_usable(const dhx_engine* e) { ensure_usable(e); }
 
+void engine_set_error(dhx_engine* e, const char* message) { e->error = message; }
+
 }  // namespace dhx
 
 extern "C" {
@@ -480,6 +482,17 @@ void dhx_engine_free(dhx_engine* e) {
 }
 
 const char* dhx_last_error(const dhx_engine* e) { return e ? e->error.c_str() : dhx::global_error(); }
+
+void* dhx_stream(const dhx_engine* e) { return e ? e->stream : nullptr; }
+
+int dhx_address(dhx_engine* e, dhx_region r, void** out) {
+    return guarded(e, [&] {
+        if (!out) throw dhx::Error("null argument");
+        ensure_usable(e);
+        check_region(e, r);
+        *out = region_ptr(e, r);
+    });
+}
 
 int dhx_allocate(dhx_engine* e, uint64_t bytes, dhx_region* out) {
     return guarded(e, [&] {

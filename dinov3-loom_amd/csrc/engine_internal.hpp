@@ -1,5 +1,6 @@
 // Engine functions used by the model's allocation-free forward
-// (dinov3_forward_noalloc); not part of the C ABI.
+// (dinov3_forward_noalloc) and the operators on packed batches (packed.cpp);
+// not part of the C ABI.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -48,5 +49,7 @@ int engine_device(const dhx_engine* e);
 // hip_check for callers outside the engine: poisons it on failure.
 void engine_check(dhx_engine* e, hipError_t err, const char* what);
 void engine_ensure_usable(const dhx_engine* e);
+// Keeps a message for dhx_last_error (entry points outside engine.cpp).
+void engine_set_error(dhx_engine* e, const char* message);
 
 }  // namespace dhx

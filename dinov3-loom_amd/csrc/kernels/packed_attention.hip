@@ -1,0 +1,338 @@
+// Softmax attention on packed batches (include/dinov3_packed.h): every
+// sequence of its own length, grouped heads, causal or not, any number of
+// queries against any number of keys.
+//
+// The queries of the heads that share a key head are the rows of one matrix:
+// row r of a sequence is its token r / group, head r % group of the group. A
+// tile of rows walks the keys once, with the running maximum and sum of the
+// softmax, and everything is computed transposed so that a lane owns one row:
+//   S^T = K . Q^T      (MFMA a = K rows from LDS, b = Q^T held in registers)
+//   O^T += V^T . P^T   (MFMA a = V^T rows, LDS transpose reads of the V block;
+//                       b = P^T straight from the S^T accumulators)
+// Lane l holds row l % 32 and 16 of every 32 keys, lane l ^ 32 the other 16.
+// exp(scale (s - m)) is one FMA and v_exp_f32 per score, with m the running
+// maximum of the raw scores, moved only when a block's weights against it sum
+// past e^8 (its maximum is then needed, and O is rescaled); the sum keeps the
+// float32 weights, P is rounded to the type of V for its product.
+//
+// K and V blocks come by DMA straight into LDS, 128- or 256-byte rows whose
+// 16-byte chunks are XOR-swizzled by the row, so that the row reads of K and
+// the transpose reads of V spread over all banks.
+#include "packed.hpp"
+
+namespace dhx {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLazySum = 2980.957987f;  // e^8, the slack of the running maximum
+constexpr float kNoMax = -1e30f;          // running maximum of a row that has seen no key
+
+// D: head channels as the kernel multiplies them (a multiple of 32; channels
+// from head_dim on are zero in Q and K and dropped from O).
+template <int D>
+struct Geo {
+    static constexpr int PITCH = D <= 64 ? 64 : 128;  // elements of a K or V row in LDS
+    static constexpr int CH = PITCH / 8;              // 16-byte chunks of it
+    static constexpr int ROWS = 64 / CH;              // rows that one DMA load moves
+    static constexpr int KK = D / 16;                 // MFMA steps of S
+    static constexpr int CT = D / 32;                 // 32-channel blocks of O
+};
+
+template <class T>
+__device__ __forceinline__ typename Num<T>::v4 read_tr(const T* p) {
+    const short4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p);
+    return __builtin_bit_cast(typename Num<T>::v4, v);
+}
+
+#define DHX_PACKED_ATTENTION_PARAMS Addr q_starts_, Addr k_starts_, Addr q_, Addr k_, Addr v_, int sequences, int group, int kv_heads, int head_dim, int q_rows, int k_rows, int causal, int slots, int splits, float c, Addr out_, Addr lse_, Addr part_, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride, uint64_t out_stride, uint64_t q_head, uint64_t k_head, uint64_t v_head, uint64_t out_head
+
+// Tile and key head of a workgroup. Workgroups go round the 8 XCDs, each with
+// its own L2, so the key heads are dealt to the XCDs (an XCD walks one head's
+// keys and values at a time) and, where there are fewer than 8, a head's tiles
+// in turn to the XCDs that share it. From the last tile on: the longest ones
+// of a causal prompt begin first.
+struct Place {
+    int head, slot;
+};
+__host__ __device__ inline int xcd_share(int kv_heads) { return kv_heads % 8 == 0 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1; }
+__device__ __forceinline__ Place place_of(int g, int slots, int kv_heads) {
+    const int share = xcd_share(kv_heads), m = 8 / share, per = (slots + m - 1) / m;
+    const int x = g & 7, i = g >> 3, h = i / per;
+    return Place{x % share + share * h, slots - 1 - ((i - h * per) * m + x / share)};
+}
+
+// A workgroup's rows and its sequence.
+struct Tile {
+    int q0, lq, k0, lk;  // the sequence's first query row and key row and their numbers
+    int row0;            // first row of the tile within the sequence, in rows of the group
+};
+
+// Finds the sequence of tile slot `slot`: sequence s has the slots from
+// starts[s] * group / BQ + s on, at least as many as it has tiles of BQ rows.
+// False if the slot has no rows.
+template <int BQ>
+__device__ __forceinline__ bool find_tile(Tile& t, int slot, const int32_t* q_starts, const int32_t* k_starts,
+                                          int sequences, int group, int q_rows, int k_rows) {
+    auto base = [&](int s) { return (int64_t)((uint32_t)start_at(q_starts, s, q_rows) * (uint32_t)group / BQ) + s; };
+    const int s = wave_last(sequences, slot, base);
+    if (s < 0) return false;
+    t.q0 = __builtin_amdgcn_readfirstlane(start_at(q_starts, s, q_rows));
+    t.lq = __builtin_amdgcn_readfirstlane(max(0, start_at(q_starts, s + 1, q_rows) - t.q0));
+    t.k0 = __builtin_amdgcn_readfirstlane(start_at(k_starts, s, k_rows));
+    t.lk = __builtin_amdgcn_readfirstlane(max(0, start_at(k_starts, s + 1, k_rows) - t.k0));
+    const int64_t row0 = ((int64_t)slot - (int64_t)((uint32_t)t.q0 * (uint32_t)group / BQ) - s) * BQ;
+    if (row0 < 0 || row0 >= (int64_t)t.lq * group) return false;
+    t.row0 = (int)row0;
+    return true;
+}
+
+// The running state of one lane's row.
+template <class T, int D>
+struct Row {
+    typename Num<T>::v8 qf[Geo<D>::KK];
+    float16_t o[Geo<D>::CT];
+    float m = kNoMax, l = 0.f;
+    int limit;  // keys 0 .. limit-1 of the sequence are seen
+};
+
+// Loads of a 32-key block for one wave's lane: which LDS elements it reads.
+struct LaneAt {
+    int k, v;
+};
+template <int PITCH>
+__device__ __forceinline__ LaneAt lane_at(int lane) {
+    const int l32 = lane & 31, hi = lane >> 5;
+    return LaneAt{lds_at<PITCH>(l32, hi * 8), lds_at<PITCH>(4 * hi + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3))};
+}
+
+// One step over a 32-key block at sK, sV (32 rows), whose first key is key0 of
+// the sequence. MASK: some lane does not see all of its keys.
+template <class T, int D, bool MASK>
+__device__ __forceinline__ void attend(Row<T, D>& st, const T* sK, const T* sV, int key0, float c, LaneAt at, int hi) {
+    using G = Geo<D>;
+    typedef typename Num<T>::v8 v8;
+    float16_t s = {};
+#pragma unroll
+    for (int kk = 0; kk < G::KK; ++kk) s = Num<T>::mfma(*(const v8*)(sK + (at.k ^ (kk << 4))), st.qf[kk], s);
+    v8 va[G::CT][2];
+#pragma unroll
+    for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const T* p = sV + ks * 16 * G::PITCH;
+            va[ct][ks] = __builtin_shufflevector(read_tr(p + (at.v ^ (ct << 5))),
+                                                 read_tr(p + (at.v ^ (ct << 5) ^ 16) + 8 * G::PITCH), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    if constexpr (MASK) {
+        const int left = st.limit - key0 - 4 * hi;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) >= left) s[r] = -__builtin_inff();
+    }
+    float p[16];
+    auto weights = [&](float m) {
+        const float mc = m * c;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] = fast_exp2(fmaf(s[r], c, -mc));
+            sum += p[r];
+        }
+        return half_pair_sum(sum);
+    };
+    float sum = weights(st.m);
+    const bool grow = !(sum <= kLazySum);
+    if (__any(grow)) {
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        const float m = grow ? fmaxf(half_pair_max(mx), st.m) : st.m, alpha = fast_exp2((st.m - m) * c);
+        st.l *= alpha;
+#pragma unroll
+        for (int ct = 0; ct < G::CT; ++ct) st.o[ct] *= alpha;
+        st.m = m;
+        sum = weights(m);
+    }
+    st.l += sum;
+    v8 pb[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pb[ks][e] = (T)p[8 * ks + e];
+#pragma unroll
+    for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) st.o[ct] = Num<T>::mfma(va[ct][ks], pb[ks], st.o[ct]);
+}
+
+// This wave's share of a block of KB keys of one matrix: LOADS DMA loads of
+// ROWS rows each, the wave's rows being first .. first + LOADS * ROWS - 1.
+template <int D, int LOADS>
+struct Mover {
+    using G = Geo<D>;
+    const char* base;  // of the sequence's first key, this head
+    uint64_t pitch;    // bytes between rows
+    int row, chunk[LOADS];
+    bool full;         // every chunk of a row exists
+    __device__ __forceinline__ Mover(const void* first_key, uint64_t stride, int head_dim, int first, int lane)
+        : base((const char*)first_key), pitch(stride * 2), row(first + lane / G::CH), full(head_dim == G::PITCH) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) chunk[j] = (lane % G::CH) ^ slot_of<G::PITCH>(row + j * G::ROWS);
+    }
+    // Keys key0 .. of the block, `left` of them in the sequence, to LDS at `to`
+    // (the wave's own rows' place).
+    template <class T>
+    __device__ __forceinline__ void move(int key0, int left, int block, int head_dim, T* to) const {
+        const char* tile = base + (uint64_t)key0 * pitch;
+        if (full && left >= block) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j)
+                dma16(tile + ((uint32_t)(row + j * G::ROWS) * (uint32_t)pitch + chunk[j] * 16), to + j * 512);
+        } else {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                const int r = row + j * G::ROWS;
+                const bool there = r < left && chunk[j] * 8 < head_dim;
+                dma16(there ? tile + ((uint32_t)r * (uint32_t)pitch + chunk[j] * 16) : (const char*)&kZeros, to + j * 512);
+            }
+        }
+    }
+};
+
+// Q fragments of row r of the tile's sequence (zeros behind its last row and
+// its last channel) and the keys it sees.
+template <class T, int D>
+__device__ __forceinline__ void load_row(Row<T, D>& st, const T* q, const Tile& t, int r, int group, int head_dim,
+                                         int causal, uint64_t q_stride, uint64_t q_head, int hi) {
+    typedef typename Num<T>::v8 v8;
+    const int token = r / group, h = r - token * group;
+    const bool there = token < t.lq;
+    const T* p = q + (uint64_t)(t.q0 + token) * q_stride + h * q_head;
+#pragma unroll
+    for (int kk = 0; kk < Geo<D>::KK; ++kk) {
+        const int ch = kk * 16 + hi * 8;
+        st.qf[kk] = there && ch < head_dim ? *(const v8*)(p + ch) : v8{};
+    }
+#pragma unroll
+    for (int ct = 0; ct < Geo<D>::CT; ++ct) st.o[ct] = float16_t{};
+    st.limit = !there ? 0 : causal ? min(max(token + 1 + t.lk - t.lq, 0), t.lk) : t.lk;
+}
+
+// O / l of one lane's row, in 16-byte pieces; `head0` the group's first head.
+template <class T, int D>
+__device__ __forceinline__ void store_row(const Row<T, D>& st, T* out, float* lse, const Tile& t, int r, int group,
+                                          int head0, int heads, int head_dim, float c, uint64_t out_stride,
+                                          uint64_t out_head, int hi) {
+    typedef typename Num<T>::v4 v4;
+    typedef typename Num<T>::v8 v8;
+    const int token = r / group, h = r - token * group;
+    const bool there = token < t.lq;
+    const float inv = st.l > 0.f ? 1.0f / st.l : 0.f;
+    T* p = out + (uint64_t)(t.q0 + token) * out_stride + h * out_head;
+#pragma unroll
+    for (int ct = 0; ct < Geo<D>::CT; ++ct)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            v4 g0, g1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                g0[e] = (T)(st.o[ct][8 * kk + e] * inv);
+                g1[e] = (T)(st.o[ct][8 * kk + 4 + e] * inv);
+            }
+            const v8 piece = __builtin_bit_cast(v8, frag_swap(__builtin_bit_cast(half4_t, g0), __builtin_bit_cast(half4_t, g1)));
+            const int ch = ct * 32 + kk * 16 + hi * 8;
+            if (there && ch < head_dim) *(v8*)(p + ch) = piece;
+        }
+    if (lse && there && hi == 0)
+        lse[(uint64_t)(t.q0 + token) * heads + head0 + h] = st.l > 0.f ? (st.m * c + __log2f(st.l)) * kLn2 : -__builtin_inff();
+}
+
+// A tile of 128 rows, 32 per wave; the four waves share blocks of 64 keys, the
+// next one on its way while one is used.
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(DHX_PACKED_ATTENTION_PARAMS) {
+    using G = Geo<D>;
+    constexpr int KB = 64, LOADS = KB / 4 / G::ROWS;
+    __shared__ __attribute__((aligned(16))) T sK0[KB * G::PITCH], sK1[KB * G::PITCH];
+    __shared__ __attribute__((aligned(16))) T sV0[KB * G::PITCH], sV1[KB * G::PITCH];
+    const Place at = place_of(blockIdx.x, slots, kv_heads);
+    if (at.head >= kv_heads || at.slot < 0) return;
+    Tile t;
+    if (!find_tile<128>(t, at.slot, q_starts_, k_starts_, sequences, group, q_rows, k_rows)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hi = lane >> 5;
+    const int head0 = at.head * group;
+
+    Row<T, D> st;
+    const int first = t.row0 + wave * 32, row = first + l32;
+    load_row(st, (const T*)q_ + head0 * q_head, t, row, group, head_dim, causal, q_stride, q_head, hi);
+    // Keys that the tile's last row sees, those that all rows of this wave see,
+    // and those that any of them sees.
+    const int rows = t.lq * group, last = min(t.row0 + 127, rows - 1), wave_last_row = min(first + 31, rows - 1);
+    auto seen = [&](int r) { return causal ? min(max(r / group + 1 + t.lk - t.lq, 0), t.lk) : t.lk; };
+    const int keys = seen(last), all = seen(min(first, rows - 1)), any = first < rows ? seen(wave_last_row) : 0;
+    const int blocks = (keys + KB - 1) / KB;
+
+    const Mover<D, LOADS> mk((const T*)k_ + (uint64_t)t.k0 * k_stride + at.head * k_head, k_stride, head_dim, wave * (KB / 4), lane);
+    const Mover<D, LOADS> mv((const T*)v_ + (uint64_t)t.k0 * v_stride + at.head * v_head, v_stride, head_dim, wave * (KB / 4), lane);
+    const LaneAt la = lane_at<G::PITCH>(lane);
+    auto move = [&](T* k, T* v, int b) {
+        mk.move(b * KB, t.lk - b * KB, KB, head_dim, k + wave * (KB / 4) * G::PITCH);
+        mv.move(b * KB, t.lk - b * KB, KB, head_dim, v + wave * (KB / 4) * G::PITCH);
+    };
+    auto step = [&](T* k, T* v, T* next_k, T* next_v, int b) {
+        wait_vm<0>();  // block b has landed, and no wave reads the other block any more
+        wait_lgkm();
+        barrier();
+        if (b + 1 < blocks) move(next_k, next_v, b + 1);
+#pragma unroll
+        for (int i = 0; i < KB; i += 32) {
+            __builtin_amdgcn_sched_barrier(0);  // one block's registers at a time
+            const int key0 = b * KB + i;
+            if (key0 >= any) break;
+            if (key0 + 32 <= all) attend<T, D, false>(st, k + i * G::PITCH, v + i * G::PITCH, key0, c, la, hi);
+            else attend<T, D, true>(st, k + i * G::PITCH, v + i * G::PITCH, key0, c, la, hi);
+        }
+    };
+    if (blocks > 0) move(sK0, sV0, 0);
+    for (int b = 0; b < blocks; b += 2) {
+        step(sK0, sV0, sK1, sV1, b);
+        if (b + 1 < blocks) step(sK1, sV1, sK0, sV0, b + 1);
+    }
+    store_row(st, (T*)out_ + head0 * out_head, (float*)lse_, t, row, group, head0, group * kv_heads, head_dim, c, out_stride,
+              out_head, hi);
+}
+
+template <class T, int D>
+hipError_t launch(const dhx_packed_attention& p, const AttentionCut& cut, hipStream_t s) {
+    const int group = (int)(p.heads / p.kv_heads), share = xcd_share((int)p.kv_heads), m = 8 / share;
+    const uint64_t grid = 8 * (p.kv_heads / share) * ((cut.slots + m - 1) / m);
+    return enqueue(packed_attention_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v,
+                   (int)p.sequences, group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows, (int)p.causal,
+                   (int)cut.slots, (int)cut.splits, p.scale * kLog2e, p.out, p.lse, p.workspace, p.q_stride, p.k_stride,
+                   p.v_stride, p.out_stride, p.q_head_stride, p.k_head_stride, p.v_head_stride, p.out_head_stride);
+}
+
+template <class T>
+hipError_t launch_type(const dhx_packed_attention& p, const AttentionCut& cut, hipStream_t s) {
+    if (p.head_dim <= 32) return launch<T, 32>(p, cut, s);
+    if (p.head_dim <= 64) return launch<T, 64>(p, cut, s);
+    if (p.head_dim <= 96) return launch<T, 96>(p, cut, s);
+    return launch<T, 128>(p, cut, s);
+}
+
+}  // namespace
+
+AttentionCut packed_attention_cut(const dhx_packed_attention& p) {
+    AttentionCut cut{};
+    cut.splits = 1;
+    cut.slots = p.q_rows * (p.heads / p.kv_heads) / 128 + p.sequences;
+    return cut;
+}
+
+hipError_t launch_packed_attention(const dhx_packed_attention& p, hipStream_t s) {
+    const AttentionCut cut = packed_attention_cut(p);
+    return p.type == DHX_F16 ? launch_type<half_t>(p, cut, s) : launch_type<bf16_t>(p, cut, s);
+}
+
+}  // namespace dhx

@@ -17,6 +17,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from . import packed
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libdinov3_hrx.so")
 
@@ -128,6 +130,10 @@ def _load_library() -> ctypes.CDLL:
     L.dhx_copy_out.argtypes = [vp, Region, c.c_uint64, c.c_uint32]
     L.dhx_copy_out_finish.argtypes = [vp, vp, c.c_uint64, c.c_uint32]
     L.dhx_benchmark.argtypes = [vp, c.c_uint64, c.c_uint64, c.POINTER(_Timings)]
+    L.dhx_stream.argtypes = [vp]
+    L.dhx_stream.restype = vp
+    L.dhx_address.argtypes = [vp, Region, c.POINTER(vp)]
+    packed.declare(L)
     return L
 
 
@@ -469,6 +475,46 @@ class Engine:
         n = ctypes.c_uint64()
         self._c(_lib.dhx_launch_timings(self._h, int(key), int(iters), ms, kid, cap, ctypes.byref(n)))
         return [(KERNELS[kid[i]], ms[i]) for i in range(n.value)]
+
+    # -- operators on packed batches (include/dinov3_packed.h) --------------
+    @property
+    def stream(self) -> int:
+        """The engine's own stream (a hipStream_t)."""
+        return _lib.dhx_stream(self._h) or 0
+
+    def address(self, region: Region) -> int:
+        """Device address of a region."""
+        out = ctypes.c_void_p()
+        self._c(_lib.dhx_address(self._h, region, ctypes.byref(out)))
+        return out.value or 0
+
+    def packed_linear_workspace(self, call: packed.Linear) -> int:
+        """Bytes of device memory that packed_linear needs for these sizes."""
+        return packed_workspace("linear", call)
+
+    def packed_linear(self, call: packed.Linear, stream: int = 0) -> None:
+        """dhx_packed_linear_run: a shared projection and each sequence's low-rank adapter; queued on `stream` (a
+        hipStream_t, 0 = the default stream) without waiting, as the two below."""
+        self._c(_lib.dhx_packed_linear_run(self._h, ctypes.byref(call), stream))
+
+    def packed_rotate(self, call: packed.Rotation, stream: int = 0) -> None:
+        """dhx_packed_rotation_run: the position rotation of each row's heads."""
+        self._c(_lib.dhx_packed_rotation_run(self._h, ctypes.byref(call), stream))
+
+    def packed_attention_workspace(self, call: packed.Attention) -> int:
+        """Bytes of device memory that packed_attention needs for these sizes."""
+        return packed_workspace("attention", call)
+
+    def packed_attention(self, call: packed.Attention, stream: int = 0) -> None:
+        """dhx_packed_attention_run: softmax attention inside each sequence."""
+        self._c(_lib.dhx_packed_attention_run(self._h, ctypes.byref(call), stream))
+
+
+def packed_workspace(operator: str, call) -> int:
+    """Bytes of workspace of a packed.Linear ("linear") or packed.Attention ("attention") call."""
+    need = ctypes.c_uint64()
+    _check_engine(getattr(_lib, f"dhx_packed_{operator}_workspace")(ctypes.byref(call), ctypes.byref(need)), None)
+    return int(need.value)
 
 
 def region_slice(region: Region, offset: int, nbytes: int) -> Region:

@@ -127,6 +127,12 @@ int dhx_engine_open(int32_t device, dhx_engine **out);
 void dhx_engine_free(dhx_engine *e);
 const char *dhx_last_error(const dhx_engine *e);
 
+/* The engine's own stream (a hipStream_t), and the device address of a region,
+ * for calls that take device memory (dinov3_packed.h; no reference
+ * counterpart). The address is valid until the engine is freed. */
+void *dhx_stream(const dhx_engine *e);
+int dhx_address(dhx_engine *e, dhx_region r, void **out);
+
 /* engine.rs:60-64 (allocate): zero-initialised device buffer. */
 int dhx_allocate(dhx_engine *e, uint64_t bytes, dhx_region *out);
 /* engine.rs:65-70 (weight): allocate and upload. */
