@@ -41,10 +41,12 @@ struct Num<bf16_t> {
 
 // How a launch is cut; the workspace function and the launcher decide alike.
 struct AttentionCut {
-    bool few;        // 32-row workgroups whose waves share the keys out
-    uint32_t splits; // workgroups along the keys of one sequence (few only)
-    uint64_t slots;  // row tiles per key head, some of them empty
-    uint64_t bytes;  // of workspace
+    bool few;         // 32-row tiles whose waves share the keys out
+    int waves;        // of a workgroup (few only)
+    uint32_t splits;  // parts of the longest sequence's keys (few only)
+    uint64_t span;    // key blocks of 32 in a part
+    uint64_t slots;   // workgroups per key head
+    uint64_t bytes;   // of workspace
 };
 AttentionCut packed_attention_cut(const dhx_packed_attention& p);
 hipError_t launch_packed_attention(const dhx_packed_attention& p, hipStream_t s);
@@ -124,6 +126,18 @@ __device__ __forceinline__ int wave_last(int n, int64_t x, Key key) {
         if (step == 1) return lo;
         hi = min(hi, lo + step);
     }
+}
+
+// Sum over the lanes up to this one: within rows of 16 lanes, then from row to
+// row (data-parallel moves between lanes, no LDS).
+__device__ __forceinline__ uint32_t wave_sum_to(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+    return v;
 }
 
 }  // namespace dhx

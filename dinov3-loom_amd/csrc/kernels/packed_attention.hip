@@ -18,6 +18,8 @@
 // K and V blocks come by DMA straight into LDS, 128- or 256-byte rows whose
 // 16-byte chunks are XOR-swizzled by the row, so that the row reads of K and
 // the transpose reads of V spread over all banks.
+#include <algorithm>
+
 #include "packed.hpp"
 
 namespace dhx {
@@ -106,9 +108,10 @@ __device__ __forceinline__ LaneAt lane_at(int lane) {
 }
 
 // One step over a 32-key block at sK, sV (32 rows), whose first key is key0 of
-// the sequence. MASK: some lane does not see all of its keys.
-template <class T, int D, bool MASK>
-__device__ __forceinline__ void attend(Row<T, D>& st, const T* sK, const T* sV, int key0, float c, LaneAt at, int hi) {
+// the sequence. mask (wave-uniform): some lane does not see all of its keys.
+template <class T, int D>
+__device__ __forceinline__ void attend(Row<T, D>& st, const T* sK, const T* sV, int key0, bool mask, float c, LaneAt at,
+                                       int hi) {
     using G = Geo<D>;
     typedef typename Num<T>::v8 v8;
     float16_t s = {};
@@ -123,7 +126,7 @@ __device__ __forceinline__ void attend(Row<T, D>& st, const T* sK, const T* sV, 
             va[ct][ks] = __builtin_shufflevector(read_tr(p + (at.v ^ (ct << 5))),
                                                  read_tr(p + (at.v ^ (ct << 5) ^ 16) + 8 * G::PITCH), 0, 1, 2, 3, 4, 5, 6, 7);
         }
-    if constexpr (MASK) {
+    if (mask) {
         const int left = st.limit - key0 - 4 * hi;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -285,13 +288,11 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(DHX_PACKE
         wait_lgkm();
         barrier();
         if (b + 1 < blocks) move(next_k, next_v, b + 1);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < KB; i += 32) {
-            __builtin_amdgcn_sched_barrier(0);  // one block's registers at a time
             const int key0 = b * KB + i;
             if (key0 >= any) break;
-            if (key0 + 32 <= all) attend<T, D, false>(st, k + i * G::PITCH, v + i * G::PITCH, key0, c, la, hi);
-            else attend<T, D, true>(st, k + i * G::PITCH, v + i * G::PITCH, key0, c, la, hi);
+            attend<T, D>(st, k + i * G::PITCH, v + i * G::PITCH, key0, key0 + 32 > all, c, la, hi);
         }
     };
     if (blocks > 0) move(sK0, sV0, 0);
@@ -303,30 +304,310 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(DHX_PACKE
               out_head, hi);
 }
 
+// Item `item` of all (sequence, tile, part), in that order: its tile and part.
+// False behind the last one.
+struct Item {
+    Tile t;
+    int part, parts;
+};
+__device__ __forceinline__ bool find_item(Item& it, uint32_t item, const int32_t* q_starts, const int32_t* k_starts, int sequences,
+                                          int group, int q_rows, int k_rows, int splits, int span) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < sequences; s0 += 64) {
+        const int s = min(s0 + lane, sequences - 1);
+        const int q0 = start_at(q_starts, s, q_rows), q1 = start_at(q_starts, s + 1, q_rows);
+        const int k0 = start_at(k_starts, s, k_rows), k1 = start_at(k_starts, s + 1, k_rows);
+        const int lq = s0 + lane < sequences ? max(0, q1 - q0) : 0, lk = max(0, k1 - k0);
+        const uint32_t tiles = ((uint32_t)lq * (uint32_t)group + 31) >> 5;
+        const uint32_t parts = max(1, min(splits, (((lk + 31) >> 5) + span - 1) / span));
+        const uint32_t to = wave_sum_to(tiles * parts);
+        const uint64_t behind = __ballot(to > item);
+        if (behind == 0) {
+            item -= __builtin_amdgcn_readlane(to, 63);
+            continue;
+        }
+        const int j = __builtin_ctzll(behind);
+        const uint32_t n = __builtin_amdgcn_readlane(parts, j);
+        const uint32_t in = item - (__builtin_amdgcn_readlane(to, j) - (uint32_t)__builtin_amdgcn_readlane(tiles, j) * n);
+        it.t = Tile{__builtin_amdgcn_readlane(q0, j), __builtin_amdgcn_readlane(lq, j), __builtin_amdgcn_readlane(k0, j),
+                    __builtin_amdgcn_readlane(lk, j), (int)(in / n * 32)};
+        it.part = (int)(in % n);
+        it.parts = (int)n;
+        return (uint32_t)it.t.row0 < (uint32_t)(it.t.lq * group);
+    }
+    return false;
+}
+
+// A tile of 32 rows whose NW waves each walk key blocks of their own (every
+// NW-th block of 32, through a ring of two blocks in LDS that no other wave
+// touches, so without barriers) and join at the end. For launches whose rows
+// are too few to fill the chip with 128-row tiles, single tokens among them;
+// several workgroups may also share a sequence's keys, a part of `span` blocks
+// each, and leave their sums in the workspace for packed_join_kernel: of part
+// p, row i and head h D float32 of O at ((p * q_rows + i) * heads + h) * D, and
+// (m, l) likewise behind all of those. A workgroup takes items until there are
+// none, so an item costs nothing that is not there; gridDim.x counts the
+// workgroups of a key head.
+template <class T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void packed_attention_few_kernel(DHX_PACKED_ATTENTION_PARAMS, int span) {
+    using G = Geo<D>;
+    constexpr int LOADS = 32 / G::ROWS, BLK = 32 * G::PITCH;
+    __shared__ __attribute__((aligned(16))) T sK0[NW * BLK], sK1[NW * BLK];
+    __shared__ __attribute__((aligned(16))) T sV0[NW * BLK], sV1[NW * BLK];
+    __shared__ float2_t sML[NW][32];
+    const Place at = place_of(blockIdx.x, slots, kv_heads);
+    if (at.head >= kv_heads || at.slot < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hi = lane >> 5;
+    const int head0 = at.head * group, heads = group * kv_heads;
+    Item it;
+    for (uint32_t item = slots - 1 - at.slot;; item += slots) {
+    if (!find_item(it, item, q_starts_, k_starts_, sequences, group, q_rows, k_rows, splits, span)) return;
+    const Tile& t = it.t;
+
+    Row<T, D> st;
+    const int row = t.row0 + l32, rows = t.lq * group, last = min(t.row0 + 31, rows - 1);
+    load_row(st, (const T*)q_ + head0 * q_head, t, row, group, head_dim, causal, q_stride, q_head, hi);
+    auto seen = [&](int r) { return causal ? min(max(r / group + 1 + t.lk - t.lq, 0), t.lk) : t.lk; };
+    const int all = seen(t.row0), blocks = (seen(last) + 31) >> 5;
+    const int lo = min(it.part * span, blocks), hi_block = it.part == it.parts - 1 ? blocks : min(lo + span, blocks);
+
+    const Mover<D, LOADS> mk((const T*)k_ + (uint64_t)t.k0 * k_stride + at.head * k_head, k_stride, head_dim, 0, lane);
+    const Mover<D, LOADS> mv((const T*)v_ + (uint64_t)t.k0 * v_stride + at.head * v_head, v_stride, head_dim, 0, lane);
+    const LaneAt la = lane_at<G::PITCH>(lane);
+    T *k0 = sK0 + wave * BLK, *k1 = sK1 + wave * BLK, *v0 = sV0 + wave * BLK, *v1 = sV1 + wave * BLK;
+    auto move = [&](T* k, T* v, int b) {
+        mk.move(b * 32, t.lk - b * 32, 32, head_dim, k);
+        mv.move(b * 32, t.lk - b * 32, 32, head_dim, v);
+    };
+    auto step = [&](const T* k, const T* v, T* next_k, T* next_v, int b) {
+        wait_lgkm();  // the other block has been read
+        if (b + NW < hi_block) {
+            move(next_k, next_v, b + NW);
+            wait_vm<2 * LOADS>();
+        } else {
+            wait_vm<0>();
+        }
+        attend<T, D>(st, k, v, b * 32, b * 32 + 32 > all, c, la, hi);
+    };
+    int b = lo + wave;
+    if (b < hi_block) move(k0, v0, b);
+    for (; b < hi_block; b += 2 * NW) {
+        step(k0, v0, k1, v1, b);
+        if (b + NW < hi_block) step(k1, v1, k0, v0, b + NW);
+    }
+
+    if constexpr (NW > 1) {
+        // Join: each wave's O in its own first blocks as float32 [row][channel]
+        // (half of the channels in each), 16-byte pieces swizzled by the row.
+        constexpr int HALF = G::PITCH / 2, PIECES = HALF / 4;
+        wait_lgkm();
+        if (hi == 0) sML[wave][l32] = float2_t{st.m, st.l};
+#pragma unroll
+        for (int ct = 0; ct < G::CT; ++ct) {
+            float* o = (float*)(ct * 32 < HALF ? k0 : v0) + l32 * HALF;
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const int piece = (ct * 32 % HALF) / 4 + 2 * g4 + hi;
+                *(float4_t*)(o + ((piece ^ (l32 % PIECES)) << 2)) =
+                    float4_t{st.o[ct][4 * g4], st.o[ct][4 * g4 + 1], st.o[ct][4 * g4 + 2], st.o[ct][4 * g4 + 3]};
+            }
+        }
+        __syncthreads();
+        if (wave == 0) {
+        float m = kNoMax, l = 0.f, part[NW];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, sML[w][l32][0]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            part[w] = fast_exp2((sML[w][l32][0] - m) * c);
+            l += part[w] * sML[w][l32][1];
+        }
+        st.m = m;
+        st.l = l;
+#pragma unroll
+        for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const int piece = (ct * 32 % HALF) / 4 + 2 * g4 + hi;
+                float4_t sum = {};
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float* o = (const float*)((ct * 32 < HALF ? sK0 : sV0) + w * BLK) + l32 * HALF;
+                    sum += part[w] * *(const float4_t*)(o + ((piece ^ (l32 % PIECES)) << 2));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st.o[ct][4 * g4 + e] = sum[e];
+            }
+        }
+    }
+    if (NW == 1 || wave == 0) {
+        if (splits == 1) {
+            store_row(st, (T*)out_ + head0 * out_head, (float*)lse_, t, row, group, head0, heads, head_dim, c, out_stride, out_head, hi);
+        } else if (row < rows) {
+            const int token = row / group, h = row - token * group;
+            const uint64_t all_rows = (uint64_t)q_rows * heads, at_row = (uint64_t)(t.q0 + token) * heads + head0 + h;
+            float* o = (float*)part_ + (it.part * all_rows + at_row) * D;
+            float2_t* ml = (float2_t*)((float*)part_ + (uint64_t)splits * all_rows * D) + at_row;
+            if (hi == 0) ml[it.part * all_rows] = float2_t{st.m, st.l};
+            if (it.part == 0)  // the parts that the sequence does not have
+                for (int i = it.parts + hi; i < splits; i += 2) ml[i * all_rows] = float2_t{kNoMax, 0.f};
+            if (st.l != 0.f) {  // else the part is not read
+#pragma unroll
+                for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4)
+                        *(float4_t*)(o + ct * 32 + 8 * g4 + 4 * hi) =
+                            float4_t{st.o[ct][4 * g4], st.o[ct][4 * g4 + 1], st.o[ct][4 * g4 + 2], st.o[ct][4 * g4 + 3]};
+            }
+        }
+    }
+    if constexpr (NW > 1) __syncthreads();  // the blocks may be filled again
+    }
+}
+
+#define DHX_JOIN_PARAMS Addr part_, Addr q_starts_, Addr out_, Addr lse_, int sequences, int q_rows, int heads, int head_dim, int splits, float c, uint64_t out_stride, uint64_t out_head
+
+// One wave per row and head: the splits' parts, weighted by 2^(c (m - max m)).
+// The splits that saw keys of a row are the first ones. Groups of lanes take a
+// split each, four floats per lane, eight loads on their way.
+template <class T, int D>
+__global__ __launch_bounds__(kThreads) void packed_join_kernel(DHX_JOIN_PARAMS) {
+    constexpr int LANES = D > 64 ? 32 : D / 4, SIDE = 64 / LANES, DEEP = 8;
+    typedef typename Num<T>::v4 v4;
+    const int lane = threadIdx.x & 63;
+    const uint64_t r = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6), all = (uint64_t)q_rows * heads;
+    if (r >= all) return;
+    const int row = (int)(r / heads), head = (int)(r - (uint64_t)row * heads);
+    const int32_t* starts = q_starts_;
+    if (row < start_at(starts, 0, q_rows) || row >= start_at(starts, sequences, q_rows)) return;
+    const float* part = part_;
+    const float2_t* ml = (const float2_t*)(part + (uint64_t)splits * all * D) + r;
+    const int ch = (lane % LANES) * 4;
+    const float* mine = part + r * D + min(ch, D - 4);
+    float m = kNoMax, l = 0.f;
+    float4_t o = {};
+    for (int s0 = 0; s0 < splits; s0 += 64) {
+        const float2_t at = s0 + lane < splits ? ml[(s0 + lane) * all] : float2_t{kNoMax, 0.f};
+        const int n = __popcll(__ballot(at[1] != 0.f));  // also one that is not a number
+        if (n == 0) break;
+        float top = fmaxf(m, at[0]);
+#pragma unroll
+        for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+        const float w = lane < n ? fast_exp2((at[0] - top) * c) : 0.f, before = fast_exp2((m - top) * c);
+        m = top;
+        l = l * before + w * (lane < n ? at[1] : 0.f);
+        o *= before;
+        for (int j0 = 0; j0 < n; j0 += SIDE * DEEP) {
+            float4_t p[DEEP];
+            float pw[DEEP];
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) {
+                const int j = j0 + d * SIDE + lane / LANES;
+                p[d] = *(const float4_t*)(mine + (uint64_t)(s0 + min(j, n - 1)) * all * D);
+                const float wj = __shfl(w, min(j, n - 1));
+                pw[d] = j < n ? wj : 0.f;
+            }
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) o += pw[d] * p[d];
+        }
+    }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
+#pragma unroll
+    for (int i = LANES; i < 64; i <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], i);
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    if (lane < LANES && ch < head_dim) {
+        v4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+        *(v4*)((T*)out_ + (uint64_t)row * out_stride + head * out_head + ch) = y;
+    }
+    if (lse_.a && lane == 0) ((float*)lse_)[r] = l != 0.f ? (m * c + __log2f(l)) * kLn2 : -__builtin_inff();
+}
+
 template <class T, int D>
 hipError_t launch(const dhx_packed_attention& p, const AttentionCut& cut, hipStream_t s) {
     const int group = (int)(p.heads / p.kv_heads), share = xcd_share((int)p.kv_heads), m = 8 / share;
     const uint64_t grid = 8 * (p.kv_heads / share) * ((cut.slots + m - 1) / m);
-    return enqueue(packed_attention_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v,
-                   (int)p.sequences, group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows, (int)p.causal,
-                   (int)cut.slots, (int)cut.splits, p.scale * kLog2e, p.out, p.lse, p.workspace, p.q_stride, p.k_stride,
-                   p.v_stride, p.out_stride, p.q_head_stride, p.k_head_stride, p.v_head_stride, p.out_head_stride);
+    const float c = p.scale * kLog2e;
+    if (!cut.few)
+        return enqueue(packed_attention_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), 0, s, p.q_starts, p.k_starts, p.q, p.k,
+                       p.v, (int)p.sequences, group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows,
+                       (int)p.causal, (int)cut.slots, 1, c, p.out, p.lse, p.workspace, p.q_stride, p.k_stride, p.v_stride,
+                       p.out_stride, p.q_head_stride, p.k_head_stride, p.v_head_stride, p.out_head_stride);
+    auto few = [&](auto kernel, int waves) {
+        return enqueue(kernel, dim3((unsigned)grid), dim3(64 * waves), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v, (int)p.sequences,
+                       group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows, (int)p.causal, (int)cut.slots,
+                       (int)cut.splits, c, p.out, p.lse, p.workspace, p.q_stride, p.k_stride, p.v_stride, p.out_stride,
+                       p.q_head_stride, p.k_head_stride, p.v_head_stride, p.out_head_stride, (int)cut.span);
+    };
+    const hipError_t err = cut.waves == 4 ? few(packed_attention_few_kernel<T, D, 4>, 4) : few(packed_attention_few_kernel<T, D, 2>, 2);
+    if (err != hipSuccess || cut.splits == 1) return err;
+    return enqueue(packed_join_kernel<T, D>, dim3((unsigned)((p.q_rows * p.heads + 3) / 4)), dim3(kThreads), 0, s, p.workspace,
+                   p.q_starts, p.out, p.lse, (int)p.sequences, (int)p.q_rows, (int)p.heads, (int)p.head_dim, (int)cut.splits,
+                   c, p.out_stride, p.out_head_stride);
 }
+
+int padded_dim(uint32_t head_dim) { return head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : 128; }
 
 template <class T>
 hipError_t launch_type(const dhx_packed_attention& p, const AttentionCut& cut, hipStream_t s) {
-    if (p.head_dim <= 32) return launch<T, 32>(p, cut, s);
-    if (p.head_dim <= 64) return launch<T, 64>(p, cut, s);
-    if (p.head_dim <= 96) return launch<T, 96>(p, cut, s);
-    return launch<T, 128>(p, cut, s);
+    switch (padded_dim(p.head_dim)) {
+        case 32: return launch<T, 32>(p, cut, s);
+        case 64: return launch<T, 64>(p, cut, s);
+        case 96: return launch<T, 96>(p, cut, s);
+        default: return launch<T, 128>(p, cut, s);
+    }
 }
 
 }  // namespace
 
+// How a launch is cut (times in us, few-rows kernel against 128-row tiles, on
+// MI355X). Sequences of at most 32 rows have no use for more: single tokens of
+// 48 requests with 32 heads of 128 on 8, 118k keys together, 94 against 657.
+// Below 96 tiles of 128 rows most of the chip would idle: 1029 rows and keys,
+// 6 heads of 64, 14.1 against 19.4 (54 tiles); five images of 201 tokens 6.9
+// against 7.4 (72); 512 causal tokens, 32 heads of 128 on 8, 16.7 against 15.6
+// (136); 16 images 12.1 against 8.1 (246).
+constexpr uint64_t kFewRows = 32, kFewTiles = 96;
+// Four waves share a tile's keys, without parts, where at most 256 items have
+// few enough blocks: 201 x 201, 6 heads, 6.9 (two waves 7.8); four queries and
+// 1029 keys of 16 images, 12 heads of 64, 14.3 (16.3). Else two: their
+// workgroups are more and their joins smaller. A part then has a 384th of all
+// blocks and no fewer than 4: one token, 1000 keys, 32 heads of 128 on 8, 11.4
+// (16 blocks 17.2), 8192 keys 15.6 with 8 blocks (64 blocks 43); the 48 requests
+// above 93 with 64 blocks (8 blocks 103).
+constexpr uint64_t kPartShare = 384, kLeastSpan = 4, kMostParts = 256;
+// Workgroups of a launch at most: beyond what runs at once an item's own
+// workgroup balances unequal ones, beyond this they only wait.
+constexpr uint64_t kFewGroups = 2048;
+
 AttentionCut packed_attention_cut(const dhx_packed_attention& p) {
     AttentionCut cut{};
     cut.splits = 1;
-    cut.slots = p.q_rows * (p.heads / p.kv_heads) / 128 + p.sequences;
+    const uint64_t group = p.heads / p.kv_heads, rows = p.q_rows * group;
+    const uint64_t longest = std::min<uint64_t>(p.longest_q ? p.longest_q : p.q_rows, p.q_rows) * group;
+    cut.slots = rows / 128 + p.sequences;
+    cut.few = longest <= kFewRows || cut.slots * p.kv_heads < kFewTiles;
+    if (!cut.few) return cut;
+    const uint64_t tiles = std::min<uint64_t>(rows / 32 + p.sequences, rows);
+    const uint64_t keys = std::min<uint64_t>(p.longest_k ? p.longest_k : p.k_rows, p.k_rows), blocks = (keys + 31) / 32;
+    const uint64_t items = tiles * p.kv_heads;
+    cut.waves = items <= 256 && (blocks <= 16 || (items >= 128 && blocks <= 40)) ? 4 : 2;
+    if (cut.waves == 2) {
+        // Blocks that all tiles walk, if each sequence has its share of both.
+        const uint64_t per_sequence = (rows + 32ull * p.sequences - 1) / (32ull * p.sequences);
+        const uint64_t work = (p.k_rows + 31) / 32 * per_sequence * p.kv_heads;
+        cut.span = std::min<uint64_t>(std::max<uint64_t>(work / kPartShare, kLeastSpan), 1u << 20);
+        const uint64_t most = std::min<uint64_t>(kMostParts, std::max<uint64_t>(1, (1ull << 30) / tiles));
+        cut.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((blocks + cut.span - 1) / cut.span, most));
+    }
+    if (cut.splits == 1) cut.span = 1u << 20;
+    else cut.bytes = cut.splits * p.q_rows * p.heads * (padded_dim(p.head_dim) + 2) * 4;
+    cut.slots = std::max<uint64_t>(1, std::min<uint64_t>(tiles * cut.splits, kFewGroups / p.kv_heads));
     return cut;
 }
 
