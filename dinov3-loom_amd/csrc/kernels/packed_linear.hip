@@ -8,12 +8,13 @@
 // belong to runs of rows with one adapter, and run j adds rank columns
 // [u of the run's rows, 0 elsewhere] . B_a^T. So adapters cost the product
 // rank columns per run in a tile, and no pass over y.
+#include <algorithm>
+#include <type_traits>
 #include "packed.hpp"
 
 namespace dhx {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kNoAdapter = -1;   // a row of a sequence without adapter
 constexpr int kNoSequence = -2;  // a row of no sequence: its y stays as it was
 
@@ -27,73 +28,168 @@ Workspace layout(const dhx_packed_linear& p) {
     return w;
 }
 
+// The products of 16 AB rows of one matrix and 16 XB rows of another along all
+// their columns, shared out to the WAVES waves of a workgroup by steps of 64
+// columns. A wave moves its own steps into its own LDS, NST - 1 of them ahead,
+// so there is no barrier. (Loaded straight into registers, a 16x16x32 operand
+// takes 16 bytes of 16 rows per quarter-wave, 16 cache lines each: 32 rows of
+// 4096 columns out of L2 then cost 9.2 us, as much as 33 MB of weights out of
+// HBM; a DMA load takes whole lines of 8 rows.)
+template <class T, int AB, int XB, int WAVES, int NST>
+struct Stream {
+    typedef typename Num<T>::v8 v8;
+    static constexpr int ROWS = 16 * (AB + XB), STAGE = ROWS * 64, LOADS = ROWS / 8;
+    const char *a, *x;    // first rows
+    uint32_t at[LOADS];   // byte offsets of the lane's row in each load
+    int lane, wave;
+
+    // a_at(r), x_at(r): byte offset of row r.
+    template <class A, class X>
+    __device__ __forceinline__ Stream(const T* a_, const T* x_, int lane_, int wave_, A a_at, X x_at)
+        : a((const char*)a_), x((const char*)x_), lane(lane_), wave(wave_) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int r = j * 8 + (lane >> 3);
+            at[j] = j < 2 * AB ? a_at(r) : x_at(r - 16 * AB);
+        }
+    }
+    __device__ __forceinline__ void move(T* to, int step, int columns) const {
+        const bool whole = step * 64 + 64 <= columns;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int c = (lane & 7) ^ slot_of<64>(j * 8 + (lane >> 3));
+            const char* p = (j < 2 * AB ? a : x) + step * 128;
+            if (whole) dma16(p + (at[j] + c * 16), to + j * 512);
+            else dma16(step * 64 + c * 8 < columns ? p + (at[j] + c * 16) : (const char*)&kZeros, to + j * 512);
+        }
+    }
+    __device__ __forceinline__ void use(const T* from, float4_t (&acc)[AB][XB]) const {
+        const int frag = (lane & 15) * 64 + (((lane >> 4) ^ slot_of<64>(lane & 15)) << 3);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            v8 fa[AB], fx[XB];
+#pragma unroll
+            for (int i = 0; i < AB; ++i) fa[i] = *(const v8*)(from + i * 1024 + (frag ^ (kk << 5)));
+#pragma unroll
+            for (int i = 0; i < XB; ++i) fx[i] = *(const v8*)(from + (AB + i) * 1024 + (frag ^ (kk << 5)));
+#pragma unroll
+            for (int i = 0; i < AB; ++i)
+#pragma unroll
+                for (int k = 0; k < XB; ++k) acc[i][k] = Num<T>::mfma16(fa[i], fx[k], acc[i][k]);
+        }
+    }
+    // s0 .. s3: this wave's stages (NST of them).
+    __device__ __forceinline__ void run(T* s0, T* s1, T* s2, T* s3, int columns, float4_t (&acc)[AB][XB]) const {
+        const int steps = (columns + 63) / 64, n = (steps - wave + WAVES - 1) / WAVES;
+        auto column = [&](int i) { return wave + i * WAVES; };
+        auto step = [&](const T* from, T* free, int i) __attribute__((always_inline)) {
+            wait_lgkm();  // the stage before has been read
+            if (i + NST - 1 < n) {
+                move(free, column(i + NST - 1), columns);
+                wait_vm<(NST - 1) * LOADS>();
+            } else {
+                wait_vm<0>();
+            }
+            use(from, acc);
+        };
+        if (n > 0) move(s0, column(0), columns);
+        if (n > 1) move(s1, column(1), columns);
+        if (NST > 3 && n > 2) move(s2, column(2), columns);
+        for (int i = 0; i < n; i += NST) {
+            step(s0, NST > 3 ? s3 : s2, i);
+            if (i + 1 < n) step(s1, s0, i + 1);
+            if (i + 2 < n) step(s2, s1, i + 2);
+            if (NST > 3 && i + 3 < n) step(s3, s2, i + 3);
+        }
+    }
+};
+
 // --- u = scale x A^T ---------------------------------------------------------
 
 #define DHX_SHRINK_PARAMS Addr starts_, Addr adapter_, Addr x_, Addr a_, Addr scale_, int sequences, int rows, int adapters, int inputs, int rank, Addr ids_, Addr u_, uint64_t x_stride
 
-// The adapter of `row` (per lane), as above. The sequences of the tile's first
-// and last rows are found by the whole wave, a lane's own between them.
-__device__ __forceinline__ int adapter_of(int row, int first, int last, const int32_t* starts, const int32_t* adapter,
-                                          int sequences, int rows, int adapters) {
-    auto at = [&](int s) { return (int64_t)start_at(starts, s, rows); };
-    int lo = max(wave_last(sequences, first, at), 0), hi = max(wave_last(sequences, last, at), lo);
-    while (lo < hi) {  // the last s whose first row is not behind `row`
-        const int mid = lo + (hi - lo + 1) / 2;
-        if (start_at(starts, mid, rows) <= row) lo = mid;
-        else hi = mid - 1;
+// The adapter of `row` (per lane, row0 + lane % TILE), as above. A lane holds the first row of one of 64 sequences,
+// those from the one of row0 on, and a row's sequence is the last one that does
+// not begin behind it: one load's latency for batches of up to 64 sequences.
+// Rows behind the window (only where sequences in it are empty) are searched.
+template <int TILE>
+__device__ __forceinline__ int adapter_of(int row, int row0, const int32_t* starts, const int32_t* adapter, int sequences,
+                                          int rows, int adapters) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    if (sequences > 64) base = max(0, wave_last(sequences, row0, [&](int s) { return (int64_t)start_at(starts, s, rows); }));
+    const int s = min(base + lane, sequences - 1);
+    const int from = start_at(starts, s, rows), to = start_at(starts, s + 1, rows), id = adapter[s];
+    int at = 0;
+#pragma unroll
+    for (int r = 0; r < TILE; ++r) {
+        const int n = __builtin_popcountll(__ballot(base + lane < sequences && from <= row0 + r));
+        if (lane % TILE == r) at = max(n - 1, 0);
     }
-    if (row < start_at(starts, lo, rows) || row >= start_at(starts, lo + 1, rows)) return kNoSequence;
-    const int id = adapter[lo];
-    return (uint32_t)id < (uint32_t)adapters ? id : kNoAdapter;
+    int lo = __shfl(from, at), hi = __shfl(to, at), mine = __shfl(id, at);
+    if (at == 63 && row >= hi && base + 64 < sequences) {
+        int a = base + 63, b = sequences - 1;
+        while (a < b) {  // the last sequence that does not begin behind the row
+            const int mid = a + (b - a + 1) / 2;
+            if (start_at(starts, mid, rows) <= row) a = mid;
+            else b = mid - 1;
+        }
+        lo = start_at(starts, a, rows);
+        hi = start_at(starts, a + 1, rows);
+        mine = adapter[a];
+    }
+    if (row < lo || row >= hi) return kNoSequence;
+    return (uint32_t)mine < (uint32_t)adapters ? mine : kNoAdapter;
 }
 
 // A workgroup takes 32 rows and, of the runs of rows with one adapter among
-// them, every gridDim.y-th; its four waves share the columns of x out and join
-// their sums in LDS. Both operands come straight from memory: A is read once
-// per run, x once per run and tile, out of the caches after the first.
-template <class T>
-__global__ __launch_bounds__(kThreads) void packed_shrink_kernel(DHX_SHRINK_PARAMS) {
-    typedef typename Num<T>::v8 v8;
+// them, every gridDim.y-th; its waves share the columns of x out and join their
+// sums in LDS. RB: blocks of 16 columns of u at a time.
+template <class T, int RB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void packed_shrink_kernel(DHX_SHRINK_PARAMS) {
     typedef typename Num<T>::v4 v4;
-    __shared__ float sum[4][32][33];
+    constexpr int COLS = 16 * RB, XB = 2, TILE = 16 * XB;
+    typedef Stream<T, RB, XB, WAVES, 4> S;
+    __shared__ __attribute__((aligned(16))) T s0[WAVES * S::STAGE], s1[WAVES * S::STAGE], s2[WAVES * S::STAGE], s3[WAVES * S::STAGE];
+    __shared__ float sum[WAVES][TILE][COLS + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l32 = lane & 31, hi = lane >> 5;
-    const int row0 = blockIdx.x * 32, row = min(row0 + l32, rows - 1);
-    int id = adapter_of(row, row0, min(row0 + 31, rows - 1), starts_, adapter_, sequences, rows, adapters);
-    if (row0 + l32 >= rows) id = kNoSequence;
-    if (blockIdx.y == 0 && wave == 0 && hi == 0 && row0 + l32 < rows) ((int32_t*)ids_)[row] = id;
-    const int before = __shfl(id, (lane & 32) | ((l32 - 1) & 31));
-    const uint32_t starts = (uint32_t)__ballot(hi == 0 && id >= 0 && (l32 == 0 || id != before));
-    const int run = __popc(starts & (0xffffffffu >> (31 - l32))) - 1;  // of this lane's row, if id >= 0
-    const int runs = __popc(starts);
-    const T* px = (const T*)x_ + (uint64_t)row * x_stride;
-    const int steps = (inputs + 15) / 16;
+    const int at = lane % TILE, l16 = lane & 15, part = lane >> 4;
+    const int row0 = blockIdx.x * TILE;
+    int id = adapter_of<TILE>(row0 + at, row0, starts_, adapter_, sequences, rows, adapters);
+    if (row0 + at >= rows) id = kNoSequence;
+    if (blockIdx.y == 0 && wave == 0 && lane < TILE && row0 + at < rows) ((int32_t*)ids_)[row0 + at] = id;
+    const int before = __shfl(id, max(at - 1, 0));
+    const uint64_t starts = __ballot(lane < TILE && id >= 0 && (at == 0 || id != before));
+    const int run = __popcll(starts & (~0ull >> (63 - at))) - 1;  // of this lane's row, if id >= 0
+    const int runs = __popcll(starts);
     for (int j = blockIdx.y; j < runs; j += gridDim.y) {
-        const uint64_t mine = __ballot(hi == 0 && id >= 0 && run == j);
-        const int a = __shfl(id, __ffsll((long long)mine) - 1);
+        const uint64_t mine = __ballot(lane < TILE && id >= 0 && run == j);
+        const int some = __ffsll((long long)mine) - 1, a = __builtin_amdgcn_readfirstlane(__shfl(id, some));
         const float scale = ((const float*)scale_)[a];
-        for (int r0 = 0; r0 < rank; r0 += 32) {
-            const int ra = min(r0 + l32, rank - 1);
-            const T* pa = (const T*)a_ + ((uint64_t)a * rank + ra) * inputs;
-            float16_t acc = {};
-            for (int s = wave; s < steps; s += 4) {
-                const int ch = s * 16 + hi * 8;
-                const bool in = ch < inputs;
-                const v8 fa = in ? *(const v8*)(pa + ch) : v8{}, fx = in ? *(const v8*)(px + ch) : v8{};
-                acc = Num<T>::mfma(fa, fx, acc);
-            }
+        for (int r0 = 0; r0 < rank; r0 += COLS) {
+            // Rows outside the run fetch its first one: no more than is needed.
+            const S stream(
+                (const T*)a_ + ((uint64_t)a * rank + r0) * inputs, (const T*)x_ + (uint64_t)row0 * x_stride, lane, wave,
+                [&](int r) { return (uint32_t)min(r, rank - 1 - r0) * (uint32_t)inputs * 2; },
+                [&](int r) { return (uint32_t)(mine >> r & 1 ? r : some) * (uint32_t)x_stride * 2; });
+            float4_t acc[RB][XB] = {};
+            stream.run(s0 + wave * S::STAGE, s1 + wave * S::STAGE, s2 + wave * S::STAGE, s3 + wave * S::STAGE, inputs, acc);
+            // Lane: row 16 x + l16, columns 16 i + 4 part .. +3.
             __syncthreads();
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[wave][l32][8 * (r >> 2) + 4 * hi + (r & 3)] = acc[r];
+            for (int i = 0; i < RB; ++i)
+#pragma unroll
+                for (int x = 0; x < XB; ++x) *(float4_t*)&sum[wave][16 * x + l16][16 * i + 4 * part] = acc[i][x];
             __syncthreads();
-            // Thread -> row tid / 8 of the tile, 4 columns.
-            const int tr = tid >> 3, c = (tid & 7) * 4;
-            const bool write = (mine >> tr & 1) && r0 + c < rank;
-            if (write) {
+            for (int i = tid; i < TILE * (COLS / 4); i += 64 * WAVES) {  // a row of the tile, 4 columns
+                const int tr = i / (COLS / 4), c = i % (COLS / 4) * 4;
+                if (!(mine >> tr & 1) || r0 + c >= rank) continue;
+                float4_t v = {};
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) v += *(const float4_t*)&sum[w][tr][c];
                 v4 out;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    out[e] = (T)(scale * ((sum[0][tr][c + e] + sum[1][tr][c + e]) + (sum[2][tr][c + e] + sum[3][tr][c + e])));
+                for (int e = 0; e < 4; ++e) out[e] = (T)(scale * v[e]);
                 *(v4*)((T*)u_ + (uint64_t)(row0 + tr) * rank + r0 + c) = out;
             }
         }
@@ -104,152 +200,351 @@ __global__ __launch_bounds__(kThreads) void packed_shrink_kernel(DHX_SHRINK_PARA
 
 #define DHX_LINEAR_PARAMS Addr x_, Addr w_, Addr ids_, Addr u_, Addr b_, int rows, int inputs, int outputs, int rank, Addr bias_, Addr y_, uint64_t x_stride, uint64_t w_stride, uint64_t y_stride
 
-// Elements of a 64-column stage row: 128 bytes, swizzled as in packed.hpp.
-constexpr int kBK = 64;
+// The runs of rows with one adapter among `n` rows from row0 on (n at most the
+// workgroup's threads): each row's run in run[] (-1: no adapter, -2: no
+// sequence), each run's adapter in list[]; returns their number. count: one int per wave.
+template <int THREADS>
+__device__ __forceinline__ int find_runs(const int32_t* ids, int row0, int n, int rows, int* run, int* list, int* count) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool in = tid < n && row0 + tid < rows;
+    const int mine = in ? ids[row0 + tid] : kNoSequence;
+    const int before = in && tid > 0 ? ids[row0 + tid - 1] : kNoSequence;
+    const bool first = mine >= 0 && mine != before;
+    const uint64_t flags = __ballot(first);
+    if (lane == 0) count[wave] = __popcll(flags);
+    __syncthreads();
+    int at = __popcll(flags & (~0ull >> (63 - lane))) - 1, runs = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w < wave) at += count[w];
+        runs += count[w];
+    }
+    if (tid < n) {
+        run[tid] = mine >= 0 ? at : mine;
+        if (first) list[at] = mine;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(runs);
+}
 
-// Tile BM x BN, waves of WM x WN each.
-template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(kThreads, 2) void packed_linear_kernel(DHX_LINEAR_PARAMS) {
+// Chunk c of LDS row r of a stage, 64 columns (128-byte rows, as in packed.hpp)
+// or 128 (256-byte rows) or 32 (64-byte rows, four per pass over the banks).
+template <int BK>
+__device__ __forceinline__ int stage_slot(int r) {
+    if constexpr (BK == 32) return (r >> 2) & 3;
+    else return slot_of<BK>(r);
+}
+
+// Tile BM x BN in steps of BK columns, waves of WM x WN each. NST stages in
+// LDS, NST - 1 of them on their way while one is multiplied (a variable each, so
+// that the compiler can tell the stage that is read from those being filled);
+// the last fragments of a stage are multiplied behind the barrier that opens
+// the next one, whose first fragments are on their way by then.
+template <class T, int BM, int BN, int WM, int WN, int BK, int NST, bool PRE, int PER_SIMD>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_linear_kernel(DHX_LINEAR_PARAMS) {
     typedef typename Num<T>::v8 v8;
     typedef typename Num<T>::v4 v4;
-    static_assert((BM / WM) * (BN / WN) * 64 == kThreads, "four waves");
-    constexpr int XL = BM / 32, WL = BN / 32;  // DMA loads of a wave per stage, 8 rows each
-    constexpr int MB = WM / 32, NB = WN / 32;
-    __shared__ __attribute__((aligned(16))) T sX0[BM * kBK], sX1[BM * kBK];
-    __shared__ __attribute__((aligned(16))) T sW0[BN * kBK], sW1[BN * kBK];
-    __shared__ int sRun[BM], sList[BM], sCount[4];
+    constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES;
+    constexpr int CH = BK / 8, LR = 64 / CH;  // chunks of a stage row, rows of a DMA load
+    constexpr int XL = BM / LR / WAVES, WL = BN / LR / WAVES;
+    constexpr int MB = WM / 32, NB = WN / 32, KK = BK / 16;
+    static_assert(!PRE || NST % 2 == 0, "the fragments' sets take turns with the stages");
+    static_assert(XL * LR * WAVES == BM && WL * LR * WAVES == BN && BM <= THREADS && BN <= THREADS, "whole loads");
+    constexpr int XS = BM * BK, WS = BN * BK;
+    __shared__ __attribute__((aligned(16))) T sX0[XS], sX1[XS], sX2[NST > 2 ? XS : 8], sX3[NST > 3 ? XS : 8];
+    __shared__ __attribute__((aligned(16))) T sW0[WS], sW1[WS], sW2[NST > 2 ? WS : 8], sW3[NST > 3 ? WS : 8];
+    __shared__ int sRun[BM], sList[BM], sCount[WAVES];
+    __shared__ __attribute__((aligned(16))) float sBias[BN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hi = lane >> 5;
+    // Tiles in XCD-contiguous order, four row blocks at a time, so that the tiles
+    // that an XCD has under way share rows of x and rows of W in its L2.
     const int n_tiles = (outputs + BN - 1) / BN, total = n_tiles * ((rows + BM - 1) / BM);
     const int per = (total + 7) >> 3, g = blockIdx.x, t = (g & 7) * per + (g >> 3);
     if ((g >> 3) >= per || t >= total) return;
-    const int row0 = (t / n_tiles) * BM, col0 = (t % n_tiles) * BN;
+    constexpr int GROUP = 4;
+    const int block = t / (GROUP * n_tiles), in_block = t - block * GROUP * n_tiles;
+    const int tall = min(GROUP, total / n_tiles - block * GROUP), across = in_block / tall;
+    const int row0 = (block * GROUP + in_block - across * tall) * BM, col0 = across * BN;
+    const int k_steps = (inputs + BK - 1) / BK, whole = inputs / BK;
+    const T *x0 = (const T*)x_ + (uint64_t)row0 * x_stride, *w0 = (const T*)w_ + (uint64_t)col0 * w_stride;
 
-    // Runs of rows with one adapter: each row's run, each run's adapter.
-    const int32_t* ids = ids_;
-    const int mine = tid < BM && row0 + tid < rows ? ids[row0 + tid] : kNoSequence;
-    const int before = tid > 0 && tid < BM && row0 + tid < rows ? ids[row0 + tid - 1] : kNoSequence;
-    const uint64_t flags = __ballot(mine >= 0 && mine != before);
-    if (lane == 0) sCount[wave] = __popcll(flags);
-    __syncthreads();
-    int run = __popcll(flags & (~0ull >> (63 - lane))) - 1, runs = 0;
+    // Lane -> row lane / CH of a load's LR, the chunk that the swizzle puts at
+    // slot lane % CH; rows behind the last one fetch that one.
+    const int lr = lane / CH;
+    uint32_t xo[XL], wo[WL];
+    auto chunk = [&](int r) { return (lane % CH) ^ stage_slot<BK>(r); };
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) run += sCount[w];
-        runs += sCount[w];
+    for (int j = 0; j < XL; ++j) {
+        const int r = (wave * XL + j) * LR + lr;
+        xo[j] = (uint32_t)min(r, rows - 1 - row0) * (uint32_t)x_stride + chunk(r) * 8;
     }
-    if (tid < BM) {
-        sRun[tid] = mine >= 0 ? run : -1;
-        if (mine >= 0 && mine != before) sList[run] = mine;
+#pragma unroll
+    for (int j = 0; j < WL; ++j) {
+        const int r = (wave * WL + j) * LR + lr;
+        wo[j] = (uint32_t)min(r, outputs - 1 - col0) * (uint32_t)w_stride + chunk(r) * 8;
     }
-    __syncthreads();
-
-    const int k_steps = (inputs + kBK - 1) / kBK;
-    const int virtual_chunks = runs * (rank >> 3), steps = k_steps + (virtual_chunks + 7) / 8, rank8 = rank >> 3;
-    const T *x = x_, *w = w_, *u = u_, *b = b_;
-    const T *x0 = x + (uint64_t)row0 * x_stride, *w0 = w + (uint64_t)col0 * w_stride;
-    // Lane -> row lane / 8 of each load's 8, the chunk that the swizzle puts at
-    // slot lane % 8.
-    const int lr = lane >> 3;
-    auto move = [&](T* sx, T* sw, int s) {
-        const bool real = s < k_steps;
-        const int chunk0 = real ? s * 8 : (s - k_steps) * 8;
+    auto move_whole = [&](T* sx, T* sw, int s) __attribute__((always_inline)) {
+        const T *px = x0 + s * BK, *pw = w0 + s * BK;
+#pragma unroll
+        for (int j = 0; j < XL; ++j) dma16(px + xo[j], sx + (wave * XL + j) * 512);
+#pragma unroll
+        for (int j = 0; j < WL; ++j) dma16(pw + wo[j], sw + (wave * WL + j) * 512);
+    };
+    // Any stage: whole ones, the last columns of x and W, and those of u and B,
+    // where chunk c belongs to run c / (rank / 8): turn = ceil(2^18 / (rank / 8))
+    // divides every c below 2^13 by it exactly.
+    int runs = 0;
+    const int rank8 = rank >> 3;
+    const uint32_t turn = ((1u << 18) + rank8 - 1) / rank8;
+    auto move = [&](T* sx, T* sw, int s) __attribute__((always_inline)) {
+        if (s < whole) {
+            move_whole(sx, sw, s);
+            return;
+        }
+        const T* zeros = (const T*)&kZeros;
+        // What follows is taken anew in each of these few stages: held through the
+        // whole ones it would cost them registers.
+        int lane = tid & 63;
+        asm volatile("" : "+v"(lane));
+        const int lr = lane / CH;
+        auto chunk = [&](int r) { return (lane % CH) ^ stage_slot<BK>(r); };
+        if (s < k_steps) {
+#pragma unroll
+            for (int j = 0; j < XL; ++j) {
+                const bool in = s * BK + chunk((wave * XL + j) * LR + lr) * 8 < inputs;
+                dma16(in ? x0 + s * BK + xo[j] : zeros, sx + (wave * XL + j) * 512);
+            }
+#pragma unroll
+            for (int j = 0; j < WL; ++j) {
+                const bool in = s * BK + chunk((wave * WL + j) * LR + lr) * 8 < inputs;
+                dma16(in ? w0 + s * BK + wo[j] : zeros, sw + (wave * WL + j) * 512);
+            }
+            return;
+        }
+        const T *u0 = (const T*)u_ + (uint64_t)row0 * rank, *b = (const T*)b_;
+        const uint64_t adapter = (uint64_t)outputs * rank;
+        const int c0 = (s - k_steps) * CH;
 #pragma unroll
         for (int j = 0; j < XL; ++j) {
-            const int r = wave * (BM / 4) + j * 8 + lr, c = chunk0 + ((lane & 7) ^ slot_of<64>(r));
-            const int rr = min(r, rows - 1 - row0);
-            const T* p = (const T*)&kZeros;
-            if (real) {
-                if (c * 8 < inputs) p = x0 + ((uint32_t)rr * (uint32_t)x_stride + c * 8);
-            } else if (c < virtual_chunks && sRun[r] == c / rank8) {
-                p = u + ((uint64_t)(row0 + rr) * rank + (c % rank8) * 8);
-            }
-            dma16(p, sx + (wave * (BM / 4) + j * 8) * kBK);
+            const int r = (wave * XL + j) * LR + lr;
+            const uint32_t c = c0 + chunk(r), i = (c * turn) >> 18;
+            const bool in = i < (uint32_t)runs && sRun[r] == (int)i;  // no row behind the last has a run
+            dma16(in ? u0 + (uint32_t)(r * rank + (c - i * rank8) * 8) : zeros, sx + (wave * XL + j) * 512);
         }
 #pragma unroll
         for (int j = 0; j < WL; ++j) {
-            const int r = wave * (BN / 4) + j * 8 + lr, c = chunk0 + ((lane & 7) ^ slot_of<64>(r));
-            const int rr = min(r, outputs - 1 - col0);
-            const T* p = (const T*)&kZeros;
-            if (real) {
-                if (c * 8 < inputs) p = w0 + ((uint32_t)rr * (uint32_t)w_stride + c * 8);
-            } else if (c < virtual_chunks) {
-                p = b + (((uint64_t)sList[c / rank8] * outputs + col0 + rr) * rank + (c % rank8) * 8);
-            }
-            dma16(p, sw + (wave * (BN / 4) + j * 8) * kBK);
+            const int r = (wave * WL + j) * LR + lr;
+            const uint32_t c = c0 + chunk(r), i = (c * turn) >> 18;
+            const T* pb = b + (uint64_t)(uint32_t)(col0 + min(r, outputs - 1 - col0)) * rank + (c - i * rank8) * 8;
+            dma16(i < (uint32_t)runs ? pb + sList[i] * adapter : zeros, sw + (wave * WL + j) * 512);
         }
     };
 
     const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
-    const int frag = lds_at<64>(l32, hi * 8);
+    const int frag = l32 * BK + ((hi ^ stage_slot<BK>(l32)) << 3);
     float16_t acc[MB][NB] = {};
-    auto step = [&](const T* sx, const T* sw, T* next_x, T* next_w, int s) {
-        wait_vm<0>();
-        wait_lgkm();
-        barrier();
-        if (s + 1 < steps) move(next_x, next_w, s + 1);
+    constexpr int SETS = PRE ? 2 * KK : 2;
+    v8 fx[SETS][MB], fw[SETS][NB];
+    auto load = [&](const T* sx, const T* sw, int kk, int set) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            v8 fx[MB], fw[NB];
+        for (int i = 0; i < MB; ++i) fx[set][i] = *(const v8*)(sx + (wm + i * 32) * BK + (frag ^ (kk << 4)));
 #pragma unroll
-            for (int i = 0; i < MB; ++i) fx[i] = *(const v8*)(sx + (wm + i * 32) * kBK + (frag ^ (kk << 4)));
+        for (int i = 0; i < NB; ++i) fw[set][i] = *(const v8*)(sw + (wn + i * 32) * BK + (frag ^ (kk << 4)));
+    };
+    auto multiply = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i) fw[i] = *(const v8*)(sw + (wn + i * 32) * kBK + (frag ^ (kk << 4)));
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int k = 0; k < NB; ++k) acc[i][k] = Num<T>::mfma(fw[k], fx[i], acc[i][k]);
-        }
+            for (int k = 0; k < NB; ++k) acc[i][k] = Num<T>::mfma(fw[set][k], fx[set][i], acc[i][k]);
     };
     move(sX0, sW0, 0);
-    for (int s = 0; s < steps; s += 2) {
-        step(sX0, sW0, sX1, sW1, s);
-        if (s + 1 < steps) step(sX1, sW1, sX0, sW0, s + 1);
-    }
+    if (tid < BN) sBias[tid] = bias_.a && col0 + tid < outputs ? ((const float*)bias_)[col0 + tid] : 0.f;
+    runs = find_runs<THREADS>(ids_, row0, BM, rows, sRun, sList, sCount);
+    const int steps = k_steps + (runs * rank8 + CH - 1) / CH;
+    if (NST > 2 && steps > 1) move(sX1, sW1, 1);
+    if (NST > 3 && steps > 2) move(sX2, sW2, 2);
+    // Opens stage s: it has landed (the NST - 2 stages behind it may be on their
+    // way), and every wave has read the one before, whose place stage s + NST - 1
+    // takes.
+    // FAST: s + 2 (NST - 1) <= whole, so that there is a next stage, NST - 1 of
+    // them on their way, and the one to fetch is whole.
+    auto open = [&](auto fast, T* free_x, T* free_w, int s) __attribute__((always_inline)) {
+        if (fast || s + NST - 2 < steps) wait_vm<(NST - 2) * (XL + WL)>();
+        else wait_vm<0>();
+        wait_lgkm();
+        barrier();
+        if constexpr (fast) move_whole(free_x, free_w, s + NST - 1);
+        else if (s + NST - 1 < steps) move(free_x, free_w, s + NST - 1);
+    };
+    auto step = [&](auto fast, T* sx, T* sw, const T* next_x, const T* next_w, int s, int odd) __attribute__((always_inline)) {
+        if constexpr (PRE) {
+            if (fast || s + 1 < steps) {
+                open(fast, sx, sw, s + 1);
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) load(next_x, next_w, kk, (1 - odd) * KK + kk);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) multiply(odd * KK + kk);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < KK - 1; ++kk) {
+                load(sx, sw, kk + 1, (kk + 1) & 1);
+                __builtin_amdgcn_sched_barrier(0);  // the reads go ahead of the products they pass under
+                multiply(kk & 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (fast || s + 1 < steps) {
+                open(fast, sx, sw, s + 1);
+                load(next_x, next_w, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            multiply((KK - 1) & 1);
+        }
+    };
+    open(std::false_type{}, NST == 2 ? sX1 : NST == 3 ? sX2 : sX3, NST == 2 ? sW1 : NST == 3 ? sW2 : sW3, 0);
+#pragma unroll
+    for (int kk = 0; kk < (PRE ? KK : 1); ++kk) load(sX0, sW0, kk, kk);
+    int s = 0;
+    auto turn_of_stages = [&](auto fast) __attribute__((always_inline)) {
+        step(fast, sX0, sW0, sX1, sW1, s, 0);
+        if (fast || s + 1 < steps) step(fast, sX1, sW1, NST > 2 ? sX2 : sX0, NST > 2 ? sW2 : sW0, s + 1, 1);
+        if constexpr (NST > 2)
+            if (fast || s + 2 < steps) step(fast, sX2, sW2, NST > 3 ? sX3 : sX0, NST > 3 ? sW3 : sW0, s + 2, 0);
+        if constexpr (NST > 3)
+            if (fast || s + 3 < steps) step(fast, sX3, sW3, sX0, sW0, s + 3, 1);
+        s += NST;
+    };
+    while (s + 2 * NST <= whole) turn_of_stages(std::true_type{});
+    while (s < steps) turn_of_stages(std::false_type{});
 
-    const float* bias = bias_;
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
         const int row = row0 + wm + i * 32 + l32;
-        if (row >= rows || ids[row] == kNoSequence) continue;
+        const bool there = sRun[wm + i * 32 + l32] != kNoSequence;
         T* py = (T*)y_ + (uint64_t)row * y_stride;
 #pragma unroll
         for (int k = 0; k < NB; ++k)
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const int n = col0 + wn + k * 32 + kk * 16;
-                float v[8];
+                v4 o[2];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = acc[i][k][8 * kk + e];
-                // v[4g + e]: column n + 8g + 4hi + e.
+                for (int q = 0; q < 2; ++q) {  // columns n + 8q + 4hi .. +3
+                    const float4_t add = *(const float4_t*)(sBias + wn + k * 32 + kk * 16 + 8 * q + 4 * hi);
 #pragma unroll
-                for (int gq = 0; gq < 2; ++gq) {
-                    const int c = n + 8 * gq + 4 * hi;
-                    if (c >= outputs) continue;
-                    v4 o;
-                    const float4_t add = bias ? *(const float4_t*)(bias + c) : float4_t{};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = (T)(v[4 * gq + e] + add[e]);
-                    *(v4*)(py + c) = o;
+                    for (int e = 0; e < 4; ++e) o[q][e] = (T)(acc[i][k][8 * kk + 4 * q + e] + add[e]);
                 }
+                const v8 piece = __builtin_bit_cast(v8, frag_swap(__builtin_bit_cast(half4_t, o[0]), __builtin_bit_cast(half4_t, o[1])));
+                if (there && n + hi * 8 < outputs) *(v8*)(py + n + hi * 8) = piece;
             }
     }
+}
+
+// Few rows: a workgroup takes 16 columns of y and 16 MB rows, so that W, which
+// is all there is to read, streams through as many workgroups as it can; the
+// four waves share the columns of x and u out and join their sums in LDS.
+constexpr int kFewWaves = 4;
+template <class T, int MB>
+__global__ __launch_bounds__(64 * kFewWaves) void packed_linear_few_kernel(DHX_LINEAR_PARAMS) {
+    typedef typename Num<T>::v8 v8;
+    constexpr int NST = MB == 4 ? 3 : 4, ROWS = 16 * MB;
+    typedef Stream<T, 1, MB, kFewWaves, NST> S;
+    constexpr int LDS = kFewWaves * S::STAGE;
+    __shared__ __attribute__((aligned(16))) T s0[LDS], s1[LDS], s2[LDS], s3[NST > 3 ? LDS : 8];
+    __shared__ float sum[kFewWaves][ROWS][20];
+    __shared__ int sRun[ROWS], sList[ROWS], sCount[kFewWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, part = lane >> 4;
+    const int col0 = blockIdx.x * 16, row0 = blockIdx.y * ROWS;
+    const int col = min(col0 + l16, outputs - 1);
+    const S stream(
+        (const T*)w_ + (uint64_t)col0 * w_stride, (const T*)x_ + (uint64_t)row0 * x_stride, lane, wave,
+        [&](int r) { return (uint32_t)min(r, outputs - 1 - col0) * (uint32_t)w_stride * 2; },
+        [&](int r) { return (uint32_t)min(r, rows - 1 - row0) * (uint32_t)x_stride * 2; });
+    float4_t acc[1][MB] = {};
+    stream.run(s0 + wave * S::STAGE, s1 + wave * S::STAGE, s2 + wave * S::STAGE, s3 + (NST > 3 ? wave * S::STAGE : 0), inputs, acc);
+    const int runs = find_runs<64 * kFewWaves>(ids_, row0, ROWS, rows, sRun, sList, sCount), rank8 = rank >> 3;
+    const T *u = (const T*)u_, *b = (const T*)b_;
+    for (int s = wave; s * 4 < runs * rank8; s += kFewWaves) {
+        const int c = s * 4 + part, i = c / rank8, off = (c - i * rank8) * 8;
+        const bool in = i < runs;
+        const v8 fb = in ? *(const v8*)(b + ((uint64_t)sList[i] * outputs + col) * rank + off) : v8{};
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int r = m * 16 + l16;
+            const v8 fu = in && sRun[r] == i ? *(const v8*)(u + (uint64_t)(row0 + r) * rank + off) : v8{};
+            acc[0][m] = Num<T>::mfma16(fb, fu, acc[0][m]);
+        }
+    }
+    // Lane: row 16 m + l16, columns 4 part .. +3.
+#pragma unroll
+    for (int m = 0; m < MB; ++m) *(float4_t*)&sum[wave][m * 16 + l16][4 * part] = acc[0][m];
+    __syncthreads();
+    const int r = tid >> 2, c = (tid & 3) * 4, row = row0 + r;
+    if (r >= ROWS || row >= rows || col0 + c >= outputs || sRun[r] == kNoSequence) return;
+    float4_t v = {};
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) v += *(const float4_t*)&sum[w][r][c];
+    const float* bias = bias_;
+    if (bias) v += *(const float4_t*)(bias + col0 + c);
+    typename Num<T>::v4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
+    *(typename Num<T>::v4*)((T*)y_ + (uint64_t)row * y_stride + col0 + c) = o;
+}
+
+template <class T, int BM, int BN, int WM, int WN, int BK, int NST, bool PRE, int PER_SIMD>
+hipError_t tiles(const dhx_packed_linear& p, Addr ids, Addr u, hipStream_t s) {
+    const uint64_t total = ((p.rows + BM - 1) / BM) * ((p.outputs + BN - 1) / BN);
+    return enqueue(packed_linear_kernel<T, BM, BN, WM, WN, BK, NST, PRE, PER_SIMD>, dim3((unsigned)((total + 7) / 8 * 8)),
+                   dim3(64 * (BM / WM) * (BN / WN)), 0, s, p.x, p.w, ids, u, p.b, (int)p.rows, (int)p.inputs, (int)p.outputs,
+                   (int)p.rank, p.bias, p.y, p.x_stride, p.w_stride, p.y_stride);
+}
+
+template <class T, int MB>
+hipError_t few(const dhx_packed_linear& p, Addr ids, Addr u, hipStream_t s) {
+    return enqueue(packed_linear_few_kernel<T, MB>, dim3((p.outputs + 15) / 16, (unsigned)((p.rows + 16 * MB - 1) / (16 * MB))),
+                   dim3(64 * kFewWaves), 0, s, p.x, p.w, ids, u, p.b, (int)p.rows, (int)p.inputs, (int)p.outputs, (int)p.rank,
+                   p.bias, p.y, p.x_stride, p.w_stride, p.y_stride);
 }
 
 template <class T>
 hipError_t launch(const dhx_packed_linear& p, hipStream_t s) {
     const Workspace w = layout(p);
     const Addr ids(p.workspace), u(static_cast<const char*>(p.workspace) + w.u);
-    const unsigned tiles = (unsigned)((p.rows + 31) / 32);
-    // Runs side by side while there are few tiles: enough workgroups for the chip.
-    const unsigned side = tiles >= 512 ? 1 : tiles >= 128 ? 4 : 32;
-    hipError_t err = enqueue(packed_shrink_kernel<T>, dim3(tiles, side), dim3(kThreads), 0, s, p.starts, p.adapter, p.x, p.a,
-                             p.scale, (int)p.sequences, (int)p.rows, (int)p.adapters, (int)p.inputs, (int)p.rank, ids, u, p.x_stride);
+    // Two waves on a tile of 32 rows where tiles are many and rows short: 12864
+    // rows of 384 columns 7.1 us (four waves 9.2); else four: 16384 rows of 4096
+    // 48 (62 with two). Taller tiles were slower everywhere. Runs go side by side
+    // while there are few tiles.
+    const unsigned row_tiles = (unsigned)((p.rows + 31) / 32);
+    const unsigned side = row_tiles >= 128 ? 1 : (unsigned)std::min<uint64_t>(32, p.sequences * 32 / p.rows + 2);
+    auto shrink = [&](auto kernel, int waves) {
+        return enqueue(kernel, dim3(row_tiles, side), dim3(64 * waves), 0, s, p.starts, p.adapter, p.x, p.a, p.scale,
+                       (int)p.sequences, (int)p.rows, (int)p.adapters, (int)p.inputs, (int)p.rank, ids, u, p.x_stride);
+    };
+    const bool narrow = row_tiles >= 256 && p.inputs <= 512;
+    const hipError_t err = narrow ? p.rank <= 16 ? shrink(packed_shrink_kernel<T, 1, 2>, 2) : shrink(packed_shrink_kernel<T, 2, 2>, 2)
+                                  : p.rank <= 16 ? shrink(packed_shrink_kernel<T, 1, 4>, 4) : shrink(packed_shrink_kernel<T, 2, 4>, 4);
     if (err != hipSuccess) return err;
-    constexpr int BM = 128, BN = 128;
-    const uint64_t total = ((p.rows + BM - 1) / BM) * ((p.outputs + BN - 1) / BN);
-    return enqueue(packed_linear_kernel<T, BM, BN, 64, 64>, dim3((unsigned)((total + 7) / 8 * 8)), dim3(kThreads), 0, s, p.x, p.w, ids, u,
-                   p.b, (int)p.rows, (int)p.inputs, (int)p.outputs, (int)p.rank, p.bias, p.y, p.x_stride, p.w_stride, p.y_stride);
+    // Times in us, whole calls on MI355X. Up to 64 rows W alone counts: 64 rows,
+    // 4096 x 4096, 31 (64 x 64 tiles 43). Then the largest tile of which there are
+    // enough for the 256 CUs: 16384 rows, 4096 x 4096, 498 with 256 x 256 (128 x
+    // 128 597), 4096 rows 130 (152; 256 tiles); 12864 rows, 384 x 1152, 29 (31; 255
+    // tiles), 8192 rows, 1024 x 1024, 38 (30; 128 tiles); 1024 rows, 4096 x 4096,
+    // 128 x 128 53.5 (256 tiles), 128 x 64 52.1 (512); 7416 rows, 1536 x 384, 28.7
+    // (174), 27.5 (348), 64 x 64 27.2 (696); 256 rows, 4096 x 4096, 64 x 64 in four
+    // stages 31 (256 tiles), in two 43.
+    if (p.rows <= 16) return few<T, 1>(p, ids, u, s);
+    if (p.rows <= 32) return few<T, 2>(p, ids, u, s);
+    if (p.rows <= 64) return few<T, 4>(p, ids, u, s);
+    auto count = [&](uint64_t m, uint64_t n) { return (p.rows + m - 1) / m * ((p.outputs + n - 1) / n); };
+    if (count(256, 256) >= 224) return tiles<T, 256, 256, 128, 64, 64, 2, false, 2>(p, ids, u, s);
+    if (count(128, 128) >= 300) return tiles<T, 128, 128, 64, 64, 64, 2, false, 2>(p, ids, u, s);
+    if (count(128, 64) >= 400) return tiles<T, 128, 64, 64, 32, 64, 2, true, 2>(p, ids, u, s);
+    if (count(64, 64) >= 512) return tiles<T, 64, 64, 32, 32, 64, 2, true, 4>(p, ids, u, s);
+    return tiles<T, 64, 64, 32, 32, 64, 4, true, 2>(p, ids, u, s);
 }
 
 }  // namespace

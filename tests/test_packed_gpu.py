@@ -178,6 +178,48 @@ def test_linear(eng, t, lengths, inputs, outputs, rank):
     assert (y[:, outputs:] == 7.0).all()
 
 
+# One launch on each route: the few-rows kernel with 1, 2 and 4 row blocks, and
+# each tile (256 x 256, 128 x 128, 128 x 64, 64 x 64 in two stages and in four),
+# with whole and ragged last tiles and steps, runs that end inside tiles and a
+# request per row.
+ROUTES = [(16, 264, 640), (32, 264, 640), (50, 264, 640), (3700, 136, 3848), (2500, 584, 1928), (2500, 584, 1304),
+          (1500, 520, 1400), (700, 1032, 520), (8300, 72, 264), (8200, 520, 264)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("kind", ["ragged", "single"])
+@pytest.mark.parametrize("rows,inputs,outputs", ROUTES)
+def test_linear_routes(eng, t, kind, rows, inputs, outputs):
+    dt = TYPES[t][1]
+    g = gen(rows + outputs)
+    if kind == "ragged":
+        lengths = [n for i in range(rows) for n in [(37 * i * i + 11) % 300]]
+        st = [s for s in starts_of(lengths) if s < rows] + [rows]
+    else:
+        st = list(range(rows + 1))
+    adapters, rank = 7, 24
+    x, w = normal(g, dt, rows, inputs), normal(g, dt, outputs, inputs, scale=inputs ** -0.5)
+    a, b = normal(g, dt, adapters, rank, inputs, scale=inputs ** -0.5), normal(g, dt, adapters, outputs, rank, scale=rank ** -0.5)
+    scale = torch.rand(adapters, generator=g, device="cuda") + 0.5
+    bias = torch.randn(outputs, generator=g, device="cuda")
+    ids = [(s * 3) % (adapters + 1) - 1 for s in range(len(st) - 1)]
+    y = torch.full((rows, outputs), 7.0, device="cuda").to(dt)
+    run_linear(eng, x, w, bias, a, b, scale, y, ints(st), ints(ids))
+    torch.cuda.synchronize()
+    # Rows of one adapter together, so that the 64-bit form takes a few products.
+    row_ids = torch.repeat_interleave(torch.tensor(ids), torch.tensor(st).diff()).cuda()
+    order = torch.argsort(row_ids, stable=True)
+    counts = [int((row_ids == i).sum()) for i in range(-1, adapters)]
+    at = starts_of(counts)
+    spans = [(at[i], at[i + 1], i - 1) for i in range(adapters + 1)]
+    want, bound = linear_want(x[order], w, bias, a, b, scale, spans)
+    within(y[order], want, bound, dt)
+    again = torch.full_like(y, 3.0)
+    run_linear(eng, x, w, bias, a, b, scale, again, ints(st), ints(ids))
+    torch.cuda.synchronize()
+    assert torch.equal(y, again)  # the same bits from launch to launch
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("first,lengths,behind", [(0, [7, 30], 91), (13, [40, 1, 100], 5), (3, [0], 60), (130, [1, 1, 1], 130)])
 def test_linear_leaves_rows_of_no_sequence(eng, t, first, lengths, behind):
