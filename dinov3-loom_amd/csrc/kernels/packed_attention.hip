@@ -50,17 +50,16 @@ __device__ __forceinline__ typename Num<T>::v4 read_tr(const T* p) {
 
 // Tile and key head of a workgroup. Workgroups go round the 8 XCDs, each with
 // its own L2, so the key heads are dealt to the XCDs (an XCD walks one head's
-// keys and values at a time) and, where there are fewer than 8, a head's tiles
-// in turn to the XCDs that share it. From the last tile on: the longest ones
-// of a causal prompt begin first.
+// keys and values at a time) and, where there are fewer than 8, a head's items
+// in turn to the XCDs that share it.
 struct Place {
-    int head, slot;
+    int head, item;
 };
 __host__ __device__ inline int xcd_share(int kv_heads) { return kv_heads % 8 == 0 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1; }
 __device__ __forceinline__ Place place_of(int g, int slots, int kv_heads) {
     const int share = xcd_share(kv_heads), m = 8 / share, per = (slots + m - 1) / m;
     const int x = g & 7, i = g >> 3, h = i / per;
-    return Place{x % share + share * h, slots - 1 - ((i - h * per) * m + x / share)};
+    return Place{x % share + share * h, (i - h * per) * m + x / share};
 }
 
 // A workgroup's rows and its sequence.
@@ -69,20 +68,28 @@ struct Tile {
     int row0;            // first row of the tile within the sequence, in rows of the group
 };
 
-// Finds the sequence of tile slot `slot`: sequence s has the slots from
-// starts[s] * group / BQ + s on, at least as many as it has tiles of BQ rows.
-// False if the slot has no rows.
-template <int BQ>
-__device__ __forceinline__ bool find_tile(Tile& t, int slot, const int32_t* q_starts, const int32_t* k_starts,
-                                          int sequences, int group, int q_rows, int k_rows) {
-    auto base = [&](int s) { return (int64_t)((uint32_t)start_at(q_starts, s, q_rows) * (uint32_t)group / BQ) + s; };
-    const int s = wave_last(sequences, slot, base);
-    if (s < 0) return false;
-    t.q0 = __builtin_amdgcn_readfirstlane(start_at(q_starts, s, q_rows));
-    t.lq = __builtin_amdgcn_readfirstlane(max(0, start_at(q_starts, s + 1, q_rows) - t.q0));
-    t.k0 = __builtin_amdgcn_readfirstlane(start_at(k_starts, s, k_rows));
-    t.lk = __builtin_amdgcn_readfirstlane(max(0, start_at(k_starts, s + 1, k_rows) - t.k0));
-    const int64_t row0 = ((int64_t)slot - (int64_t)((uint32_t)t.q0 * (uint32_t)group / BQ) - s) * BQ;
+// Finds the tile of 128 rows of slot `slot`: sequence s has the slots from
+// starts[s] * group / 128 + s on, at least as many as it has tiles. False if the
+// slot has no rows. For up to 64 sequences a lane holds one of them: one load's
+// latency. (Tiles handed out by the keys they see, most first, were no faster:
+// 145 us against 145 for ten ragged prompts, 94 against 95 for 39 images of
+// 201 to 4101 tokens, and their search cost 1.5 us.)
+__device__ __forceinline__ bool find_tile(Tile& t, int slot, const int32_t* q_starts, const int32_t* k_starts, int sequences,
+                                          int group, int q_rows, int k_rows) {
+    const int lane = threadIdx.x & 63;
+    int s = 0;
+    auto base = [&](int s) { return (int64_t)((uint32_t)start_at(q_starts, s, q_rows) * (uint32_t)group >> 7) + s; };
+    if (sequences > 64) s = max(wave_last(sequences, slot, base), 0);
+    const int mine = min(s + lane, sequences - 1);  // of many only the first counts
+    const int q0 = start_at(q_starts, mine, q_rows), q1 = start_at(q_starts, mine + 1, q_rows);
+    const int k0 = start_at(k_starts, mine, k_rows), k1 = start_at(k_starts, mine + 1, k_rows);
+    const int64_t from = (int64_t)((uint32_t)q0 * (uint32_t)group >> 7) + mine;
+    const int j = sequences > 64 ? 0 : max(__builtin_popcountll(__ballot(lane < sequences && from <= slot)) - 1, 0);
+    t.q0 = __builtin_amdgcn_readlane(q0, j);
+    t.lq = max(0, __builtin_amdgcn_readlane(q1, j) - t.q0);
+    t.k0 = __builtin_amdgcn_readlane(k0, j);
+    t.lk = max(0, __builtin_amdgcn_readlane(k1, j) - t.k0);
+    const int64_t row0 = ((int64_t)slot - (int64_t)((uint32_t)t.q0 * (uint32_t)group >> 7) - (s + j)) * 128;
     if (row0 < 0 || row0 >= (int64_t)t.lq * group) return false;
     t.row0 = (int)row0;
     return true;
@@ -93,7 +100,7 @@ template <class T, int D>
 struct Row {
     typename Num<T>::v8 qf[Geo<D>::KK];
     float16_t o[Geo<D>::CT];
-    float m = kNoMax, l = 0.f;
+    float m = kNoMax, l = 0.f;  // l: the sum of this lane's keys only, the other half is in lane ^ 32
     int limit;  // keys 0 .. limit-1 of the sequence are seen
 };
 
@@ -105,6 +112,54 @@ template <int PITCH>
 __device__ __forceinline__ LaneAt lane_at(int lane) {
     const int l32 = lane & 31, hi = lane >> 5;
     return LaneAt{lds_at<PITCH>(l32, hi * 8), lds_at<PITCH>(4 * hi + ((lane & 15) >> 2), 16 * ((lane >> 4) & 1) + 4 * (lane & 3))};
+}
+
+// A weight of zero times a value that is not finite is not zero, and in a block
+// that some lane does not wholly see such a value may be none of its row's
+// business. So they leave zeros behind in the operands of the product, and reach
+// the rows that see their keys apart: the product of their places (1 or 0) and
+// the keys seen (1 or 0) tells which channels of which rows get an infinity or
+// no number.
+template <class T, int D>
+__device__ __forceinline__ void add_not_finite(Row<T, D>& st, typename Num<T>::v8 (&va)[Geo<D>::CT][2], int key0, int hi) {
+    using G = Geo<D>;
+    typedef typename Num<T>::v8 v8;
+    constexpr uint32_t EXP = __is_same(T, half_t) ? 0x7c00u : 0x7f80u;
+    uint32_t all = 0;  // bit 15 and 31: an exponent of ones somewhere
+#pragma unroll
+    for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                all |= (__builtin_bit_cast(uint4_t, va[ct][ks])[w] & (EXP * 0x10001u)) + (0x8000u - EXP) * 0x10001u;
+    if (__builtin_expect(!__any((all & 0x80008000u) != 0), 1)) return;
+    const int left = st.limit - key0 - 4 * hi;
+    v8 seen[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) seen[r / 8][r % 8] = (T)(8 * (r >> 2) + (r & 3) < left ? 1.f : 0.f);
+#pragma unroll
+    for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+        for (int kind = 0; kind < 3; ++kind) {
+            __builtin_amdgcn_sched_barrier(0);  // one at a time: this is no place for registers
+            const float what = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
+            float16_t f = {};
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                v8 here;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float v = (float)va[ct][ks][e];
+                    const bool is = kind < 2 ? v == what : v != v;
+                    here[e] = (T)(is ? 1.f : 0.f);
+                    if (is) va[ct][ks][e] = (T)0.f;
+                }
+                f = Num<T>::mfma(here, seen[ks], f);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st.o[ct][r] += f[r] > 0.f ? what : 0.f;
+        }
 }
 
 // One step over a 32-key block at sK, sV (32 rows), whose first key is key0 of
@@ -141,14 +196,14 @@ __device__ __forceinline__ void attend(Row<T, D>& st, const T* sK, const T* sV, 
             p[r] = fast_exp2(fmaf(s[r], c, -mc));
             sum += p[r];
         }
-        return half_pair_sum(sum);
+        return sum;
     };
     float sum = weights(st.m);
-    const bool grow = !(sum <= kLazySum);
-    if (__any(grow)) {
-        float mx = s[0];
+    if (__any(!(sum <= kLazySum))) {
+        float mx = s[0], both = half_pair_sum(sum);
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        const bool grow = !(both <= kLazySum);  // alike in both halves of the row
         const float m = grow ? fmaxf(half_pair_max(mx), st.m) : st.m, alpha = fast_exp2((st.m - m) * c);
         st.l *= alpha;
 #pragma unroll
@@ -162,6 +217,7 @@ __device__ __forceinline__ void attend(Row<T, D>& st, const T* sK, const T* sV, 
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int e = 0; e < 8; ++e) pb[ks][e] = (T)p[8 * ks + e];
+    if (mask) add_not_finite<T, D>(st, va, key0, hi);
 #pragma unroll
     for (int ct = 0; ct < G::CT; ++ct)
 #pragma unroll
@@ -250,19 +306,24 @@ __device__ __forceinline__ void store_row(const Row<T, D>& st, T* out, float* ls
         lse[(uint64_t)(t.q0 + token) * heads + head0 + h] = st.l > 0.f ? (st.m * c + __log2f(st.l)) * kLn2 : -__builtin_inff();
 }
 
-// A tile of 128 rows, 32 per wave; the four waves share blocks of 64 keys, the
-// next one on its way while one is used.
-template <class T, int D>
-__global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(DHX_PACKED_ATTENTION_PARAMS) {
+// A tile of 128 rows, 32 per wave; the four waves of a group share blocks of 64
+// keys, the next one on its way while one is used. GROUPS = 2: two such groups
+// take the blocks in turn and join at the end, which halves the time of a tile
+// alone on a CU.
+template <class T, int D, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, D <= 64 ? 4 : 2) void packed_attention_kernel(DHX_PACKED_ATTENTION_PARAMS) {
     using G = Geo<D>;
-    constexpr int KB = 64, LOADS = KB / 4 / G::ROWS;
-    __shared__ __attribute__((aligned(16))) T sK0[KB * G::PITCH], sK1[KB * G::PITCH];
-    __shared__ __attribute__((aligned(16))) T sV0[KB * G::PITCH], sV1[KB * G::PITCH];
+    constexpr int KB = 64, LOADS = KB / 4 / G::ROWS, BLK = KB * G::PITCH;
+    __shared__ __attribute__((aligned(16))) T sK0[GROUPS * BLK], sK1[GROUPS * BLK];
+    __shared__ __attribute__((aligned(16))) T sV0[GROUPS * BLK], sV1[GROUPS * BLK];
+    __shared__ float2_t sML[GROUPS > 1 ? GROUPS - 1 : 1][4][32];
     const Place at = place_of(blockIdx.x, slots, kv_heads);
-    if (at.head >= kv_heads || at.slot < 0) return;
+    if (at.head >= kv_heads || at.item >= slots) return;
     Tile t;
-    if (!find_tile<128>(t, at.slot, q_starts_, k_starts_, sequences, group, q_rows, k_rows)) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // From the last slot on: a causal prompt's longest tiles begin first.
+    if (!find_tile(t, slots - 1 - at.item, q_starts_, k_starts_, sequences, group, q_rows, k_rows)) return;
+    const int tid = threadIdx.x, lane = tid & 63, all_waves = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = all_waves & 3, part = all_waves >> 2;
     const int l32 = lane & 31, hi = lane >> 5;
     const int head0 = at.head * group;
 
@@ -279,6 +340,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(DHX_PACKE
     const Mover<D, LOADS> mk((const T*)k_ + (uint64_t)t.k0 * k_stride + at.head * k_head, k_stride, head_dim, wave * (KB / 4), lane);
     const Mover<D, LOADS> mv((const T*)v_ + (uint64_t)t.k0 * v_stride + at.head * v_head, v_stride, head_dim, wave * (KB / 4), lane);
     const LaneAt la = lane_at<G::PITCH>(lane);
+    T *k0 = sK0 + part * BLK, *k1 = sK1 + part * BLK, *v0 = sV0 + part * BLK, *v1 = sV1 + part * BLK;
     auto move = [&](T* k, T* v, int b) {
         mk.move(b * KB, t.lk - b * KB, KB, head_dim, k + wave * (KB / 4) * G::PITCH);
         mv.move(b * KB, t.lk - b * KB, KB, head_dim, v + wave * (KB / 4) * G::PITCH);
@@ -287,18 +349,58 @@ __global__ __launch_bounds__(kThreads, 2) void packed_attention_kernel(DHX_PACKE
         wait_vm<0>();  // block b has landed, and no wave reads the other block any more
         wait_lgkm();
         barrier();
-        if (b + 1 < blocks) move(next_k, next_v, b + 1);
-#pragma unroll 1
+        if (b + GROUPS < blocks) move(next_k, next_v, b + GROUPS);
+#pragma unroll(D <= 64 ? 1 : 2)
         for (int i = 0; i < KB; i += 32) {
             const int key0 = b * KB + i;
             if (key0 >= any) break;
             attend<T, D>(st, k + i * G::PITCH, v + i * G::PITCH, key0, key0 + 32 > all, c, la, hi);
         }
     };
-    if (blocks > 0) move(sK0, sV0, 0);
-    for (int b = 0; b < blocks; b += 2) {
-        step(sK0, sV0, sK1, sV1, b);
-        if (b + 1 < blocks) step(sK1, sV1, sK0, sV0, b + 1);
+    // Every wave takes part in every step's barrier, also without a block.
+    if (part < blocks) move(k0, v0, part);
+    for (int b = 0; b < blocks; b += 2 * GROUPS) {
+        step(k0, v0, k1, v1, b + part);
+        if (b + GROUPS < blocks) step(k1, v1, k0, v0, b + GROUPS + part);
+    }
+    st.l = half_pair_sum(st.l);
+    if constexpr (GROUPS > 1) {
+        // The other groups' O through their own blocks, as float32 [row][channels],
+        // a quarter (of PITCH) of them in each, 16-byte pieces swizzled by the row.
+        constexpr int WIDE = G::PITCH / 4, PIECES = WIDE / 4;
+        auto piece = [&](int of, int ct, int g4) __attribute__((always_inline)) {
+            const int ch = ct * 32 + 8 * g4, at = ch / WIDE;
+            float* o = (float*)((at == 0 ? sK0 : at == 1 ? sV0 : at == 2 ? sK1 : sV1) + of * BLK) + wave * 32 * WIDE;
+            return (float4_t*)(o + l32 * WIDE + (((ch % WIDE / 4 + hi) ^ (l32 % PIECES)) << 2));
+        };
+        wait_lgkm();
+        barrier();  // every wave has read its last block
+        if (part > 0) {
+            if (hi == 0) sML[part - 1][wave][l32] = float2_t{st.m, st.l};
+#pragma unroll
+            for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4)
+                    *piece(part, ct, g4) =
+                        float4_t{st.o[ct][4 * g4], st.o[ct][4 * g4 + 1], st.o[ct][4 * g4 + 2], st.o[ct][4 * g4 + 3]};
+        }
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int of = 1; of < GROUPS; ++of) {
+            const float2_t other = sML[of - 1][wave][l32];
+            const float m = fmaxf(st.m, other[0]), mine = fast_exp2((st.m - m) * c), its = fast_exp2((other[0] - m) * c);
+            st.l = st.l * mine + other[1] * its;
+            st.m = m;
+#pragma unroll
+            for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const float4_t o = *piece(of, ct, g4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st.o[ct][4 * g4 + e] = st.o[ct][4 * g4 + e] * mine + o[e] * its;
+                }
+        }
     }
     store_row(st, (T*)out_ + head0 * out_head, (float*)lse_, t, row, group, head0, group * kv_heads, head_dim, c, out_stride,
               out_head, hi);
@@ -356,12 +458,12 @@ __global__ __launch_bounds__(64 * NW, 1) void packed_attention_few_kernel(DHX_PA
     __shared__ __attribute__((aligned(16))) T sV0[NW * BLK], sV1[NW * BLK];
     __shared__ float2_t sML[NW][32];
     const Place at = place_of(blockIdx.x, slots, kv_heads);
-    if (at.head >= kv_heads || at.slot < 0) return;
+    if (at.head >= kv_heads || at.item >= slots) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hi = lane >> 5;
     const int head0 = at.head * group, heads = group * kv_heads;
     Item it;
-    for (uint32_t item = slots - 1 - at.slot;; item += slots) {
+    for (uint32_t item = at.item;; item += slots) {
     if (!find_item(it, item, q_starts_, k_starts_, sequences, group, q_rows, k_rows, splits, span)) return;
     const Tile& t = it.t;
 
@@ -397,6 +499,7 @@ __global__ __launch_bounds__(64 * NW, 1) void packed_attention_few_kernel(DHX_PA
         if (b + NW < hi_block) step(k1, v1, k0, v0, b + NW);
     }
 
+    st.l = half_pair_sum(st.l);
     if constexpr (NW > 1) {
         // Join: each wave's O in its own first blocks as float32 [row][channel]
         // (half of the channels in each), 16-byte pieces swizzled by the row.
@@ -533,11 +636,15 @@ hipError_t launch(const dhx_packed_attention& p, const AttentionCut& cut, hipStr
     const int group = (int)(p.heads / p.kv_heads), share = xcd_share((int)p.kv_heads), m = 8 / share;
     const uint64_t grid = 8 * (p.kv_heads / share) * ((cut.slots + m - 1) / m);
     const float c = p.scale * kLog2e;
-    if (!cut.few)
-        return enqueue(packed_attention_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), 0, s, p.q_starts, p.k_starts, p.q, p.k,
-                       p.v, (int)p.sequences, group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows,
-                       (int)p.causal, (int)cut.slots, 1, c, p.out, p.lse, p.workspace, p.q_stride, p.k_stride, p.v_stride,
-                       p.out_stride, p.q_head_stride, p.k_head_stride, p.v_head_stride, p.out_head_stride);
+    auto tile = [&](auto kernel, int groups) {
+        return enqueue(kernel, dim3((unsigned)grid), dim3(256 * groups), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v,
+                       (int)p.sequences, group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows, (int)p.causal,
+                       (int)cut.slots, 1, c, p.out, p.lse, p.workspace, p.q_stride, p.k_stride, p.v_stride, p.out_stride,
+                       p.q_head_stride, p.k_head_stride, p.v_head_stride, p.out_head_stride);
+    };
+    if constexpr (D <= 64)
+        if (!cut.few && cut.waves == 16) return tile(packed_attention_kernel<T, D, 4>, 4);
+    if (!cut.few) return cut.waves >= 8 ? tile(packed_attention_kernel<T, D, 2>, 2) : tile(packed_attention_kernel<T, D, 1>, 1);
     auto few = [&](auto kernel, int waves) {
         return enqueue(kernel, dim3((unsigned)grid), dim3(64 * waves), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v, (int)p.sequences,
                        group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows, (int)p.causal, (int)cut.slots,
@@ -573,6 +680,13 @@ hipError_t launch_type(const dhx_packed_attention& p, const AttentionCut& cut, h
 // against 7.4 (72); 512 causal tokens, 32 heads of 128 on 8, 16.7 against 15.6
 // (136); 16 images 12.1 against 8.1 (246).
 constexpr uint64_t kFewRows = 32, kFewTiles = 96;
+// Where the tiles are few enough to run at once, the time of one counts, and
+// groups of waves share its keys: 2048 causal tokens, 32 heads of 128 on 8, 46.5
+// with two groups, 52.0 with one (520 tiles), 4096 tokens 154 against 148
+// (1032); ragged prompts with 16 heads of 80 28.0, 29.6 (400); 4101 rows and keys,
+// 6 heads of 64, 42.1 with four, 50.3 with two, 72.3 with one (198), but 16 images
+// of 201 tokens 10.3, 8.2, 8.5 (246).
+constexpr uint64_t kShareTiles = 600;
 // Four waves share a tile's keys, without parts, where at most 256 items have
 // few enough blocks: 201 x 201, 6 heads, 6.9 (two waves 7.8); four queries and
 // 1029 keys of 16 images, 12 heads of 64, 14.3 (16.3). Else two: their
@@ -592,9 +706,13 @@ AttentionCut packed_attention_cut(const dhx_packed_attention& p) {
     const uint64_t longest = std::min<uint64_t>(p.longest_q ? p.longest_q : p.q_rows, p.q_rows) * group;
     cut.slots = rows / 128 + p.sequences;
     cut.few = longest <= kFewRows || cut.slots * p.kv_heads < kFewTiles;
-    if (!cut.few) return cut;
-    const uint64_t tiles = std::min<uint64_t>(rows / 32 + p.sequences, rows);
     const uint64_t keys = std::min<uint64_t>(p.longest_k ? p.longest_k : p.k_rows, p.k_rows), blocks = (keys + 31) / 32;
+    if (!cut.few) {
+        const uint64_t count = cut.slots * p.kv_heads;
+        cut.waves = count > kShareTiles ? 4 : count <= 256 && blocks >= 64 && p.head_dim <= 64 ? 16 : 8;
+        return cut;
+    }
+    const uint64_t tiles = std::min<uint64_t>(rows / 32 + p.sequences, rows);
     const uint64_t items = tiles * p.kv_heads;
     cut.waves = items <= 256 && (blocks <= 16 || (items >= 128 && blocks <= 40)) ? 4 : 2;
     if (cut.waves == 2) {

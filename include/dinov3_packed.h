@@ -107,10 +107,10 @@ int dhx_packed_rotation_run(dhx_engine *e, const dhx_packed_rotation *p, void *s
  * has the queries of q_starts and the keys of k_starts, in any numbers. With
  * `causal`, query i of lq sees the keys j <= i + lk - lq (the last query sees
  * all of them, as for a prompt, its next part or one new token), else all. A
- * query that sees no key gets zeros, and -infinity in lse. Keys that a query
- * does not see have no effect on it, whatever they hold, but that a value that
- * is not finite reaches the queries of its own sequence that share a block of
- * 32 keys with one that sees it.
+ * query that sees no key gets zeros, and -infinity in lse. Keys and values that
+ * a query does not see have no effect on it, whatever they hold; a value that is
+ * not finite makes its channel not finite (an infinity or not a number) for the
+ * queries that see it.
  * longest_q and longest_k, the rows of the longest sequence (0: not known),
  * only choose how the work is cut: a wrong number costs time, not results. */
 typedef struct dhx_packed_attention {

@@ -343,7 +343,7 @@ def check_attention(e, dt, ql, kl, heads, kv, dim, causal, *, seed=0, spread=2.0
     return out
 
 
-LENGTHS = [[1], [201], [5, 0, 17, 1], [31, 32, 33], [63, 64, 65, 127, 128, 129], [300, 1, 1, 0, 77], [1029]]
+LENGTHS = [[(7 * i) % 50 for i in range(130)], [1] * 63 + [300], [1], [201], [5, 0, 17, 1], [31, 32, 33], [63, 64, 65, 127, 128, 129], [300, 1, 1, 0, 77], [1029]]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -357,7 +357,8 @@ def test_attention(eng, t, causal, heads, kv, dim, lengths):
 # Numbers of queries and keys that differ: single tokens, pooling queries, a
 # prompt's next part, keys missing, more queries than keys (rows without keys).
 APART = [([1], [1]), ([1], [777]), ([1] * 9, [1, 2, 31, 32, 33, 0, 500, 1000, 64]), ([4] * 5, [201, 0, 3, 64, 700]),
-         ([70, 3, 200], [300, 1000, 200]), ([50, 129, 33], [20, 0, 32]), ([260], [100]), ([1, 64, 2], [4000, 4000, 4000])]
+         ([70, 3, 200], [300, 1000, 200]), ([50, 129, 33], [20, 0, 32]), ([260], [100]), ([1, 64, 2], [4000, 4000, 4000]),
+         ([i % 3 for i in range(150)], [(i * i) % 90 for i in range(150)])]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -366,6 +367,23 @@ APART = [([1], [1]), ([1], [777]), ([1] * 9, [1, 2, 31, 32, 33, 0, 500, 1000, 64
 @pytest.mark.parametrize("ql,kl", APART)
 def test_attention_apart(eng, t, causal, heads, kv, dim, ql, kl):
     check_attention(eng, TYPES[t][1], ql, kl, heads, kv, dim, causal, hints=(max(ql), max(kl)))
+
+
+# One launch on each route: 128-row tiles with one, two and four groups of waves
+# (by the number of tiles and the keys), the few-rows kernel with four waves and
+# with two, in parts or not.
+ROUTES_ATTENTION = [([700] * 8, [700] * 8, 16, 16), ([1500], [1500], 16, 8), ([4200], [4200], 6, 6), ([201], [201], 6, 6),
+                    ([1] * 40, [500] * 40, 8, 4), ([1] * 4, [9000, 0, 1, 5000], 8, 1), ([8] * 3, [1000] * 3, 4, 4)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("dim", [32, 64, 88, 128])
+@pytest.mark.parametrize("ql,kl,heads,kv", ROUTES_ATTENTION)
+def test_attention_routes(eng, t, dim, ql, kl, heads, kv):
+    causal = dim != 64
+    first = check_attention(eng, TYPES[t][1], ql, kl, heads, kv, dim, causal, hints=(max(ql), max(kl)))
+    again = check_attention(eng, TYPES[t][1], ql, kl, heads, kv, dim, causal, hints=(max(ql), max(kl)))
+    assert torch.equal(first, again)  # the same bits from launch to launch
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -385,6 +403,42 @@ def test_attention_wrong_hints_cost_time_only(eng, t):
 @pytest.mark.parametrize("spread,scale", [(30.0, None), (0.01, None), (8.0, 1.0), (100.0, 1.0)])
 def test_attention_scores_of_any_size(eng, t, spread, scale):
     check_attention(eng, TYPES[t][1], [150, 1], [150, 900], 4, 2, 64, 1, spread=spread, scale=scale)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("lq,lk", [(300, 300), (1, 300), (4, 77), (1500, 1500)])
+def test_attention_values_not_finite(eng, t, dim, lq, lk):
+    # A key or value that is not finite has no effect on queries that do not see
+    # it, and makes those that do not finite, a value in its channel alone.
+    dt = TYPES[t][1]
+    g = gen(dim + lq)
+    heads, kv = 4, 2
+    q, k, v = normal(g, dt, lq, heads, dim), normal(g, dt, lk, kv, dim), normal(g, dt, lk, kv, dim)
+    want, room, _, _ = attention_want(q, k, v, 1, dim ** -0.5)
+    at = {lk * 2 // 3: (math.inf, 3), lk * 2 // 3 + 1: (-math.inf, 7), lk * 3 // 4: (math.nan, 9), lk - 1: (-math.inf, 3)}
+    for key, (value, channel) in at.items():
+        v[key, :, channel] = value
+    out = torch.empty(lq, heads, dim, dtype=dt, device="cuda")
+    run_attention(eng, q, k, v, out, ints([0, lq]), ints([0, lk]), 1, dim ** -0.5, hints=(lq, lk))
+    torch.cuda.synchronize()
+    odd = torch.zeros(lq, dim, dtype=torch.float64, device="cuda")
+    for key, (value, channel) in at.items():
+        odd[max(0, key - (lk - lq)):, channel] += value
+    plain = (odd == 0)[:, None].expand(lq, heads, dim)
+    within(out[plain], want[plain], room[plain], dt)
+    # Not finite, be it an infinity or no number: a weight under the type's least
+    # number (2^-24 of f16) is a zero in the product, and zero times infinity is
+    # none.
+    assert not out[~plain].isfinite().any()
+    # A key that is not a number, seen by the last query only.
+    v = normal(g, dt, lk, kv, dim)
+    want, room, _, _ = attention_want(q, k, v, 1, dim ** -0.5)
+    k[lk - 1] = math.nan
+    run_attention(eng, q, k, v, out, ints([0, lq]), ints([0, lk]), 1, dim ** -0.5, hints=(lq, lk))
+    torch.cuda.synchronize()
+    assert out[lq - 1].isnan().all()
+    within(out[:lq - 1], want[:lq - 1], room[:lq - 1], dt)
 
 
 @pytest.mark.parametrize("t", TYPES)
