@@ -494,6 +494,7 @@ __global__ __launch_bounds__(64 * NW, 1) void packed_attention_few_kernel(DHX_PA
     };
     int b = lo + wave;
     if (b < hi_block) move(k0, v0, b);
+    wait_vm<0>();  // Q too, which no counted wait behind DMA loads would prove
     for (; b < hi_block; b += 2 * NW) {
         step(k0, v0, k1, v1, b);
         if (b + NW < hi_block) step(k1, v1, k0, v0, b + NW);

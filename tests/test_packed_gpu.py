@@ -8,7 +8,6 @@ Tolerances are bounds from the arithmetic. u is half a step of the type
 exact factors is off by at most (n + 1) f times the sum of their absolute
 values, whatever its order; an output is rounded once, by u of itself (and at
 most half the type's smallest number where it is subnormal)."""
-import ctypes
 import math
 
 import pytest
