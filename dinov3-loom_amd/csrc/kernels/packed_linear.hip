@@ -18,13 +18,22 @@ namespace {
 constexpr int kNoAdapter = -1;   // a row of a sequence without adapter
 constexpr int kNoSequence = -2;  // a row of no sequence: its y stays as it was
 
+// Up to so many rows the few-rows kernel takes the product.
+constexpr uint64_t kFewRows = 64;
+constexpr int kMostParts = 4;
+
 struct Workspace {
-    uint64_t ids, u, bytes;  // int32 [rows]; [rows][rank]
+    uint64_t u, bytes;  // ids, int32 [rows], are at 0
+    uint32_t parts;     // sums of u over parts of the columns, float32 [parts][rows][rank]; 1: u itself, [rows][rank]
 };
 Workspace layout(const dhx_packed_linear& p) {
     Workspace w{};
     w.u = (p.rows * 4 + 255) / 256 * 256;
-    w.bytes = w.u + p.rows * p.rank * 2;
+    // A run's columns in parts where rows are few: a CU reads no more than about
+    // 40 GB/s of A, and 24 single tokens' adapters (4096 columns, rank 16) would
+    // keep 24 of them busy.
+    w.parts = p.rows <= kFewRows ? (uint32_t)std::min<uint64_t>(std::max<uint32_t>(p.inputs / 1024, 1), kMostParts) : 1;
+    w.bytes = w.u + p.rows * p.rank * (w.parts > 1 ? 4 * w.parts : 2);
     return w;
 }
 
@@ -143,8 +152,9 @@ __device__ __forceinline__ int adapter_of(int row, int row0, const int32_t* star
 }
 
 // A workgroup takes 32 rows and, of the runs of rows with one adapter among
-// them, every gridDim.y-th; its waves share the columns of x out and join their
-// sums in LDS. RB: blocks of 16 columns of u at a time.
+// them, every gridDim.y-th, and of the columns of x one of gridDim.z parts (of
+// several, the sums of u are left to the product); its waves share those out and
+// join their sums in LDS. RB: blocks of 16 columns of u at a time.
 template <class T, int RB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void packed_shrink_kernel(DHX_SHRINK_PARAMS) {
     typedef typename Num<T>::v4 v4;
@@ -155,9 +165,12 @@ __global__ __launch_bounds__(64 * WAVES) void packed_shrink_kernel(DHX_SHRINK_PA
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int at = lane % TILE, l16 = lane & 15, part = lane >> 4;
     const int row0 = blockIdx.x * TILE;
+    // This workgroup's part of the columns, in whole steps.
+    const int per = ((inputs + 63) / 64 + gridDim.z - 1) / gridDim.z * 64, column0 = min((int)blockIdx.z * per, inputs);
+    const int columns = min(per, inputs - column0);
     int id = adapter_of<TILE>(row0 + at, row0, starts_, adapter_, sequences, rows, adapters);
     if (row0 + at >= rows) id = kNoSequence;
-    if (blockIdx.y == 0 && wave == 0 && lane < TILE && row0 + at < rows) ((int32_t*)ids_)[row0 + at] = id;
+    if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0 && lane < TILE && row0 + at < rows) ((int32_t*)ids_)[row0 + at] = id;
     const int before = __shfl(id, max(at - 1, 0));
     const uint64_t starts = __ballot(lane < TILE && id >= 0 && (at == 0 || id != before));
     const int run = __popcll(starts & (~0ull >> (63 - at))) - 1;  // of this lane's row, if id >= 0
@@ -169,11 +182,11 @@ __global__ __launch_bounds__(64 * WAVES) void packed_shrink_kernel(DHX_SHRINK_PA
         for (int r0 = 0; r0 < rank; r0 += COLS) {
             // Rows outside the run fetch its first one: no more than is needed.
             const S stream(
-                (const T*)a_ + ((uint64_t)a * rank + r0) * inputs, (const T*)x_ + (uint64_t)row0 * x_stride, lane, wave,
+                (const T*)a_ + ((uint64_t)a * rank + r0) * inputs + column0, (const T*)x_ + (uint64_t)row0 * x_stride + column0, lane, wave,
                 [&](int r) { return (uint32_t)min(r, rank - 1 - r0) * (uint32_t)inputs * 2; },
                 [&](int r) { return (uint32_t)(mine >> r & 1 ? r : some) * (uint32_t)x_stride * 2; });
             float4_t acc[RB][XB] = {};
-            stream.run(s0 + wave * S::STAGE, s1 + wave * S::STAGE, s2 + wave * S::STAGE, s3 + wave * S::STAGE, inputs, acc);
+            stream.run(s0 + wave * S::STAGE, s1 + wave * S::STAGE, s2 + wave * S::STAGE, s3 + wave * S::STAGE, columns, acc);
             // Lane: row 16 x + l16, columns 16 i + 4 part .. +3.
             __syncthreads();
 #pragma unroll
@@ -187,10 +200,15 @@ __global__ __launch_bounds__(64 * WAVES) void packed_shrink_kernel(DHX_SHRINK_PA
                 float4_t v = {};
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) v += *(const float4_t*)&sum[w][tr][c];
+                const uint64_t to = (uint64_t)(row0 + tr) * rank + r0 + c;
+                if (gridDim.z > 1) {
+                    *(float4_t*)((float*)u_ + (uint64_t)blockIdx.z * rows * rank + to) = scale * v;
+                    continue;
+                }
                 v4 out;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) out[e] = (T)(scale * v[e]);
-                *(v4*)((T*)u_ + (uint64_t)(row0 + tr) * rank + r0 + c) = out;
+                *(v4*)((T*)u_ + to) = out;
             }
         }
     }
@@ -447,7 +465,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
 // four waves share the columns of x and u out and join their sums in LDS.
 constexpr int kFewWaves = 4;
 template <class T, int MB>
-__global__ __launch_bounds__(64 * kFewWaves) void packed_linear_few_kernel(DHX_LINEAR_PARAMS) {
+__global__ __launch_bounds__(64 * kFewWaves) void packed_linear_few_kernel(DHX_LINEAR_PARAMS, int parts) {
     typedef typename Num<T>::v8 v8;
     constexpr int NST = MB == 4 ? 3 : 4, ROWS = 16 * MB;
     typedef Stream<T, 1, MB, kFewWaves, NST> S;
@@ -474,7 +492,30 @@ __global__ __launch_bounds__(64 * kFewWaves) void packed_linear_few_kernel(DHX_L
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
             const int r = m * 16 + l16;
-            const v8 fu = in && sRun[r] == i ? *(const v8*)(u + (uint64_t)(row0 + r) * rank + off) : v8{};
+            const uint64_t at = (uint64_t)(row0 + r) * rank + off;
+            v8 fu = {};
+            if (in && sRun[r] == i) {
+                if (parts == 1) {
+                    fu = *(const v8*)(u + at);
+                } else {
+                    float4_t v[kMostParts][2] = {};
+#pragma unroll
+                    for (int z = 0; z < kMostParts; ++z) {
+                        const float4_t* p = (const float4_t*)((const float*)u_ + (uint64_t)min(z, parts - 1) * rows * rank + at);
+                        v[z][0] = p[0];
+                        v[z][1] = p[1];
+                    }
+                    float4_t all[2] = {v[0][0], v[0][1]};
+#pragma unroll
+                    for (int z = 1; z < kMostParts; ++z)
+                        if (z < parts) {
+                            all[0] += v[z][0];
+                            all[1] += v[z][1];
+                        }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) fu[e] = (T)all[e / 4][e % 4];
+                }
+            }
             acc[0][m] = Num<T>::mfma16(fb, fu, acc[0][m]);
         }
     }
@@ -504,10 +545,10 @@ hipError_t tiles(const dhx_packed_linear& p, Addr ids, Addr u, hipStream_t s) {
 }
 
 template <class T, int MB>
-hipError_t few(const dhx_packed_linear& p, Addr ids, Addr u, hipStream_t s) {
+hipError_t few(const dhx_packed_linear& p, Addr ids, Addr u, uint32_t parts, hipStream_t s) {
     return enqueue(packed_linear_few_kernel<T, MB>, dim3((p.outputs + 15) / 16, (unsigned)((p.rows + 16 * MB - 1) / (16 * MB))),
                    dim3(64 * kFewWaves), 0, s, p.x, p.w, ids, u, p.b, (int)p.rows, (int)p.inputs, (int)p.outputs, (int)p.rank,
-                   p.bias, p.y, p.x_stride, p.w_stride, p.y_stride);
+                   p.bias, p.y, p.x_stride, p.w_stride, p.y_stride, (int)parts);
 }
 
 template <class T>
@@ -521,7 +562,7 @@ hipError_t launch(const dhx_packed_linear& p, hipStream_t s) {
     const unsigned row_tiles = (unsigned)((p.rows + 31) / 32);
     const unsigned side = row_tiles >= 128 ? 1 : (unsigned)std::min<uint64_t>(32, p.sequences * 32 / p.rows + 2);
     auto shrink = [&](auto kernel, int waves) {
-        return enqueue(kernel, dim3(row_tiles, side), dim3(64 * waves), 0, s, p.starts, p.adapter, p.x, p.a, p.scale,
+        return enqueue(kernel, dim3(row_tiles, side, w.parts), dim3(64 * waves), 0, s, p.starts, p.adapter, p.x, p.a, p.scale,
                        (int)p.sequences, (int)p.rows, (int)p.adapters, (int)p.inputs, (int)p.rank, ids, u, p.x_stride);
     };
     const bool narrow = row_tiles >= 256 && p.inputs <= 512;
@@ -536,9 +577,9 @@ hipError_t launch(const dhx_packed_linear& p, hipStream_t s) {
     // 128 x 128 53.5 (256 tiles), 128 x 64 52.1 (512); 7416 rows, 1536 x 384, 28.7
     // (174), 27.5 (348), 64 x 64 27.2 (696); 256 rows, 4096 x 4096, 64 x 64 in four
     // stages 31 (256 tiles), in two 43.
-    if (p.rows <= 16) return few<T, 1>(p, ids, u, s);
-    if (p.rows <= 32) return few<T, 2>(p, ids, u, s);
-    if (p.rows <= 64) return few<T, 4>(p, ids, u, s);
+    if (p.rows <= 16) return few<T, 1>(p, ids, u, w.parts, s);
+    if (p.rows <= 32) return few<T, 2>(p, ids, u, w.parts, s);
+    if (p.rows <= kFewRows) return few<T, 4>(p, ids, u, w.parts, s);
     auto count = [&](uint64_t m, uint64_t n) { return (p.rows + m - 1) / m * ((p.outputs + n - 1) / n); };
     if (count(256, 256) >= 224) return tiles<T, 256, 256, 128, 64, 64, 2, false, 2>(p, ids, u, s);
     if (count(128, 128) >= 300) return tiles<T, 128, 128, 64, 64, 64, 2, false, 2>(p, ids, u, s);
