@@ -8,7 +8,9 @@ addresses as integers, and run by an Engine any number of times:
     bytes = engine.packed_attention_workspace(call)   # the caller's device memory
     engine.packed_attention(call, stream)             # queued, not waited for
 
-The fields and their rules are those of the header."""
+The fields and their rules are those of the header. A program that uses PyTorch
+imports it before this package: the two then share PyTorch's HIP runtime, while
+the other way round each would have its own."""
 from __future__ import annotations
 
 import ctypes

@@ -14,7 +14,7 @@ import dinov3_hrx as d  # noqa: E402
 from dinov3_hrx import packed  # noqa: E402
 
 from test_kernels_gpu import K_ATTN, K_QKV, _keys  # noqa: E402
-from test_packed_gpu import (F, attention_want, gen, half_step, ints, linear_want, normal, run_attention, run_linear,  # noqa: E402
+from packed_operators import (F, attention_want, gen, half_step, ints, linear_want, normal, run_attention, run_linear,  # noqa: E402
                              run_rotation, starts_of, within)
 
 pytestmark = pytest.mark.gpu
