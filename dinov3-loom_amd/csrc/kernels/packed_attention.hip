@@ -580,56 +580,57 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(DHX_JOIN_PARAMS) 
     constexpr int LANES = D > 64 ? 32 : D / 4, SIDE = 64 / LANES, DEEP = 8;
     typedef typename Num<T>::v4 v4;
     const int lane = threadIdx.x & 63;
-    const uint64_t r = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6), all = (uint64_t)q_rows * heads;
-    if (r >= all) return;
-    const int row = (int)(r / heads), head = (int)(r - (uint64_t)row * heads);
-    const int32_t* starts = q_starts_;
-    if (row < start_at(starts, 0, q_rows) || row >= start_at(starts, sequences, q_rows)) return;
-    const float* part = part_;
-    const float2_t* ml = (const float2_t*)(part + (uint64_t)splits * all * D) + r;
-    const int ch = (lane % LANES) * 4;
-    const float* mine = part + r * D + min(ch, D - 4);
-    float m = kNoMax, l = 0.f;
-    float4_t o = {};
-    for (int s0 = 0; s0 < splits; s0 += 64) {
-        const float2_t at = s0 + lane < splits ? ml[(s0 + lane) * all] : float2_t{kNoMax, 0.f};
-        const int n = __popcll(__ballot(at[1] != 0.f));  // also one that is not a number
-        if (n == 0) break;
-        float top = fmaxf(m, at[0]);
+    const uint64_t all = (uint64_t)q_rows * heads;
+    for (uint64_t r = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < all; r += (uint64_t)gridDim.x * 4) {
+        const int row = (int)(r / heads), head = (int)(r - (uint64_t)row * heads);
+        const int32_t* starts = q_starts_;
+        if (row < start_at(starts, 0, q_rows) || row >= start_at(starts, sequences, q_rows)) continue;
+        const float* part = part_;
+        const float2_t* ml = (const float2_t*)(part + (uint64_t)splits * all * D) + r;
+        const int ch = (lane % LANES) * 4;
+        const float* mine = part + r * D + min(ch, D - 4);
+        float m = kNoMax, l = 0.f;
+        float4_t o = {};
+        for (int s0 = 0; s0 < splits; s0 += 64) {
+            const float2_t at = s0 + lane < splits ? ml[(s0 + lane) * all] : float2_t{kNoMax, 0.f};
+            const int n = __popcll(__ballot(at[1] != 0.f));  // also one that is not a number
+            if (n == 0) break;
+            float top = fmaxf(m, at[0]);
 #pragma unroll
-        for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-        const float w = lane < n ? fast_exp2((at[0] - top) * c) : 0.f, before = fast_exp2((m - top) * c);
-        m = top;
-        l = l * before + w * (lane < n ? at[1] : 0.f);
-        o *= before;
-        for (int j0 = 0; j0 < n; j0 += SIDE * DEEP) {
-            float4_t p[DEEP];
-            float pw[DEEP];
+            for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+            const float w = lane < n ? fast_exp2((at[0] - top) * c) : 0.f, before = fast_exp2((m - top) * c);
+            m = top;
+            l = l * before + w * (lane < n ? at[1] : 0.f);
+            o *= before;
+            for (int j0 = 0; j0 < n; j0 += SIDE * DEEP) {
+                float4_t p[DEEP];
+                float pw[DEEP];
 #pragma unroll
-            for (int d = 0; d < DEEP; ++d) {
-                const int j = j0 + d * SIDE + lane / LANES;
-                p[d] = *(const float4_t*)(mine + (uint64_t)(s0 + min(j, n - 1)) * all * D);
-                const float wj = __shfl(w, min(j, n - 1));
-                pw[d] = j < n ? wj : 0.f;
+                for (int d = 0; d < DEEP; ++d) {
+                    const int j = j0 + d * SIDE + lane / LANES;
+                    p[d] = *(const float4_t*)(mine + (uint64_t)(s0 + min(j, n - 1)) * all * D);
+                    const float wj = __shfl(w, min(j, n - 1));
+                    pw[d] = j < n ? wj : 0.f;
+                }
+#pragma unroll
+                for (int d = 0; d < DEEP; ++d) o += pw[d] * p[d];
             }
-#pragma unroll
-            for (int d = 0; d < DEEP; ++d) o += pw[d] * p[d];
         }
+#pragma unroll
+        for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
+#pragma unroll
+        for (int i = LANES; i < 64; i <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], i);
+        const float inv = l != 0.f ? 1.0f / l : 0.f;
+        if (lane < LANES && ch < head_dim) {
+            v4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+            *(v4*)((T*)out_ + (uint64_t)row * out_stride + head * out_head + ch) = y;
+        }
+        if (lse_.a && lane == 0) ((float*)lse_)[r] = l != 0.f ? (m * c + __log2f(l)) * kLn2 : -__builtin_inff();
     }
-#pragma unroll
-    for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
-#pragma unroll
-    for (int i = LANES; i < 64; i <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], i);
-    const float inv = l != 0.f ? 1.0f / l : 0.f;
-    if (lane < LANES && ch < head_dim) {
-        v4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
-        *(v4*)((T*)out_ + (uint64_t)row * out_stride + head * out_head + ch) = y;
-    }
-    if (lse_.a && lane == 0) ((float*)lse_)[r] = l != 0.f ? (m * c + __log2f(l)) * kLn2 : -__builtin_inff();
 }
 
 template <class T, int D>
@@ -654,7 +655,7 @@ hipError_t launch(const dhx_packed_attention& p, const AttentionCut& cut, hipStr
     };
     const hipError_t err = cut.waves == 4 ? few(packed_attention_few_kernel<T, D, 4>, 4) : few(packed_attention_few_kernel<T, D, 2>, 2);
     if (err != hipSuccess || cut.splits == 1) return err;
-    return enqueue(packed_join_kernel<T, D>, dim3((unsigned)((p.q_rows * p.heads + 3) / 4)), dim3(kThreads), 0, s, p.workspace,
+    return enqueue(packed_join_kernel<T, D>, dim3((unsigned)std::min<uint64_t>((p.q_rows * p.heads + 3) / 4, 1u << 20)), dim3(kThreads), 0, s, p.workspace,
                    p.q_starts, p.out, p.lse, (int)p.sequences, (int)p.q_rows, (int)p.heads, (int)p.head_dim, (int)cut.splits,
                    c, p.out_stride, p.out_head_stride);
 }

@@ -17,6 +17,7 @@ namespace {
 // 64 9.7 us instead of 8.0, 8192 rows of 40 heads of 128 40 instead of 36; stores
 // that bypass the caches 10.0 and 77.)
 constexpr int kItems = 256, kMostThreads = 1024;
+constexpr uint64_t kMostBlocks = 1u << 21;  // a launch has fewer than 2^32 threads; workgroups take further rows in turn
 
 #define DHX_ROTATE_PARAMS Addr x_, Addr out_, Addr cos_, Addr sin_, Addr index_, uint64_t x_stride, uint64_t out_stride, int rows, int places, int heads, int head_dim, int rotated, int copy, int block_rows
 
@@ -31,48 +32,50 @@ __global__ __launch_bounds__(kMostThreads) void packed_rotate_kernel(DHX_ROTATE_
     // out in place).
     const int turn = rotated / 16, rest = copy ? (head_dim - rotated) / 8 : 0, per_head = turn + rest;
     const int per_row = heads * per_head;
-    const int row0 = blockIdx.x * block_rows, n = min(block_rows, rows - row0) * per_row;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const int r = i / per_row, in_row = i - r * per_row, h = in_row / per_head, j = in_row - h * per_head;
-        const size_t row = (size_t)row0 + r;
-        const T* px = x + row * x_stride + h * head_dim;
-        T* po = out + row * out_stride + h * head_dim;
-        if (j >= turn) {
-            const int c = rotated + (j - turn) * 8;
-            *(v8*)(po + c) = *(const v8*)(px + c);
-            continue;
-        }
-        const int place = index[row];
-        const bool turned = (uint32_t)place < (uint32_t)places;
-        if (!turned && !copy) continue;
-        // Halves: the pieces 8j and rotated/2 + 8j, angles 8j .. 8j+7.
-        // Neighbours: the pieces 16j and 16j + 8, the same angles.
-        const int c1 = NEIGHBOURS ? 16 * j : 8 * j, c2 = NEIGHBOURS ? 16 * j + 8 : rotated / 2 + 8 * j;
-        v8 a = *(const v8*)(px + c1), b = *(const v8*)(px + c2);
-        if (turned) {
-            const float4_t* pc = (const float4_t*)(cos + (size_t)place * (rotated / 2) + 8 * j);
-            const float4_t* ps = (const float4_t*)(sin + (size_t)place * (rotated / 2) + 8 * j);
-            const float4_t c[2] = {pc[0], pc[1]}, s[2] = {ps[0], ps[1]};
-            v8 u, w;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float ce = c[e / 4][e % 4], se = s[e / 4][e % 4];
-                const float x1 = NEIGHBOURS ? (float)(e < 4 ? a[2 * (e % 4)] : b[2 * (e % 4)]) : (float)a[e];
-                const float x2 = NEIGHBOURS ? (float)(e < 4 ? a[2 * (e % 4) + 1] : b[2 * (e % 4) + 1]) : (float)b[e];
-                const T y1 = (T)(x1 * ce - x2 * se), y2 = (T)(x2 * ce + x1 * se);
-                if constexpr (NEIGHBOURS) {
-                    (e < 4 ? u : w)[2 * (e % 4)] = y1;
-                    (e < 4 ? u : w)[2 * (e % 4) + 1] = y2;
-                } else {
-                    u[e] = y1;
-                    w[e] = y2;
-                }
+    for (int64_t row0 = (int64_t)blockIdx.x * block_rows; row0 < rows; row0 += (int64_t)gridDim.x * block_rows) {
+        const int n = (int)min((int64_t)block_rows, rows - row0) * per_row;
+        for (int i = threadIdx.x; i < n; i += blockDim.x) {
+            const int r = i / per_row, in_row = i - r * per_row, h = in_row / per_head, j = in_row - h * per_head;
+            const int64_t row = row0 + r;
+            const T* px = x + row * x_stride + h * head_dim;
+            T* po = out + row * out_stride + h * head_dim;
+            if (j >= turn) {
+                const int c = rotated + (j - turn) * 8;
+                *(v8*)(po + c) = *(const v8*)(px + c);
+                continue;
             }
-            a = u;
-            b = w;
+            const int place = index[row];
+            const bool turned = (uint32_t)place < (uint32_t)places;
+            if (!turned && !copy) continue;
+            // Halves: the pieces 8j and rotated/2 + 8j, angles 8j .. 8j+7.
+            // Neighbours: the pieces 16j and 16j + 8, the same angles.
+            const int c1 = NEIGHBOURS ? 16 * j : 8 * j, c2 = NEIGHBOURS ? 16 * j + 8 : rotated / 2 + 8 * j;
+            v8 a = *(const v8*)(px + c1), b = *(const v8*)(px + c2);
+            if (turned) {
+                const float4_t* pc = (const float4_t*)(cos + (size_t)place * (rotated / 2) + 8 * j);
+                const float4_t* ps = (const float4_t*)(sin + (size_t)place * (rotated / 2) + 8 * j);
+                const float4_t c[2] = {pc[0], pc[1]}, s[2] = {ps[0], ps[1]};
+                v8 u, w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float ce = c[e / 4][e % 4], se = s[e / 4][e % 4];
+                    const float x1 = NEIGHBOURS ? (float)(e < 4 ? a[2 * (e % 4)] : b[2 * (e % 4)]) : (float)a[e];
+                    const float x2 = NEIGHBOURS ? (float)(e < 4 ? a[2 * (e % 4) + 1] : b[2 * (e % 4) + 1]) : (float)b[e];
+                    const T y1 = (T)(x1 * ce - x2 * se), y2 = (T)(x2 * ce + x1 * se);
+                    if constexpr (NEIGHBOURS) {
+                        (e < 4 ? u : w)[2 * (e % 4)] = y1;
+                        (e < 4 ? u : w)[2 * (e % 4) + 1] = y2;
+                    } else {
+                        u[e] = y1;
+                        w[e] = y2;
+                    }
+                }
+                a = u;
+                b = w;
+            }
+            *(v8*)(po + c1) = a;
+            *(v8*)(po + c2) = b;
         }
-        *(v8*)(po + c1) = a;
-        *(v8*)(po + c2) = b;
     }
 }
 
@@ -81,7 +84,7 @@ hipError_t launch(const dhx_packed_rotation& p, hipStream_t s) {
     const int copy = p.x != p.out;
     const int per_row = (int)p.heads * (int)(p.rotated / 16 + (copy ? (p.head_dim - p.rotated) / 8 : 0));
     const int block_rows = per_row >= kItems ? 1 : kItems / per_row;
-    const uint64_t blocks = (p.rows + block_rows - 1) / block_rows;
+    const uint64_t blocks = std::min<uint64_t>((p.rows + block_rows - 1) / block_rows, kMostBlocks);
     const int threads = std::min(kMostThreads, (per_row * block_rows + 63) / 64 * 64);
     return enqueue(packed_rotate_kernel<T, NEIGHBOURS>, dim3((unsigned)blocks), dim3((unsigned)threads), 0, s, p.x, p.out, p.cos,
                    p.sin, p.index, p.x_stride, p.out_stride, (int)p.rows, (int)p.places, (int)p.heads, (int)p.head_dim,

@@ -18,6 +18,9 @@ using dhx::Error;
 // that a tile of 256 rows spans fit in 32 bits.
 constexpr uint64_t kMaxRows = 0x7fffffff - 256;
 constexpr uint64_t kMaxStride = 1u << 22;
+// A launch has fewer than 2^32 threads: 256 to each 32 rows of a projection, 512
+// to a tile of 256 x 256, and 256 to each row tile of attention.
+constexpr uint64_t kMaxLinearRows = 1u << 27, kMaxLinearTiles = 1u << 22, kMaxRowTiles = 1u << 23;
 
 void positive(uint64_t v, const char* what) {
     if (v == 0) throw Error(std::string(what) + " must be positive");
@@ -60,7 +63,7 @@ void linear_sizes(const dhx_packed_linear& p) {
     type_of(p.type);
     positive(p.sequences, "sequences");
     most(p.sequences, kMaxRows, "sequences");
-    most(p.rows, kMaxRows, "rows");
+    most(p.rows, kMaxLinearRows, "rows");
     eights(p.inputs, "inputs");
     eights(p.outputs, "outputs");
     eights(p.rank, "rank");
@@ -69,6 +72,8 @@ void linear_sizes(const dhx_packed_linear& p) {
     most(p.outputs, kMaxStride, "outputs");
     most(p.rank, 256, "rank");
     most(p.adapters, kMaxRows, "adapters");
+    most(((p.rows + 255) / 256) * ((p.outputs + 255) / 256), kMaxLinearTiles,
+         "the number of tiles of 256 x 256 outputs");
 }
 
 void linear_check(const dhx_packed_linear& p) {
@@ -132,13 +137,14 @@ void attention_sizes(const dhx_packed_attention& p) {
     most(p.k_rows, kMaxRows, "k_rows");
     const uint64_t rows = p.q_rows * (p.heads / p.kv_heads);
     most(rows, kMaxRows, "q_rows * (heads / kv_heads)");
-    // One workgroup per tile of 32 rows or more and key head, and their splits.
-    most((rows / 32 + p.sequences) * p.kv_heads, 1u << 24, "the number of row tiles");
+    most(p.q_rows + p.k_rows, kMaxRows, "q_rows + k_rows");
+    most((rows / 32 + p.sequences) * p.kv_heads, kMaxRowTiles, "the number of row tiles");
 }
 
 void attention_check(const dhx_packed_attention& p) {
     attention_sizes(p);
     if (!(p.scale > 0) || !std::isfinite(p.scale)) throw Error("scale must be positive and finite");
+    if (p.scale > 1048576.0f) throw Error("scale must be at most 2^20");  // times a row's first maximum it stays finite
     pointer(p.q, 16, "q", p.q_rows > 0);
     pointer(p.k, 16, "k", p.k_rows > 0);
     pointer(p.v, 16, "v", p.k_rows > 0);

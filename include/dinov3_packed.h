@@ -33,9 +33,9 @@
  * is rounded once, to the nearest value of its type.
  *
  * A workspace belongs to the caller: 16-byte aligned device memory of at least
- * the bytes that the workspace function returns for the same sizes. Its content
- * is not read between calls. Calls that may run at the same time (other
- * streams, captured graphs that are replayed side by side) need one each.
+ * the bytes that the workspace function returns for the same sizes and hints.
+ * Its content is not read between calls. Calls that may run at the same time
+ * (other streams, captured graphs that are replayed side by side) need one each.
  */
 #ifndef DINOV3_PACKED_H
 #define DINOV3_PACKED_H
@@ -110,7 +110,8 @@ int dhx_packed_rotation_run(dhx_engine *e, const dhx_packed_rotation *p, void *s
  * query that sees no key gets zeros, and -infinity in lse. Keys and values that
  * a query does not see have no effect on it, whatever they hold; a value that is
  * not finite makes its channel not finite (an infinity or not a number) for the
- * queries that see it.
+ * queries that see it. Products q . k lie above -1e30; a query whose products
+ * are all below that counts as one that sees no key.
  * longest_q and longest_k, the rows of the longest sequence (0: not known),
  * only choose how the work is cut: a wrong number costs time, not results. */
 typedef struct dhx_packed_attention {
@@ -119,7 +120,7 @@ typedef struct dhx_packed_attention {
     uint32_t sequences, heads, kv_heads, head_dim; /* head_dim: a multiple of 8, to 128 */
     uint64_t q_rows, k_rows; /* of q and out; of k and v */
     uint32_t longest_q, longest_k;
-    float scale;             /* positive */
+    float scale;             /* positive, at most 2^20 */
     uint32_t reserved;       /* 0 */
     const void *q;           /* row i, head h at q + i q_stride + h q_head_stride */
     const void *k, *v;

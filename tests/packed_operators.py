@@ -111,6 +111,21 @@ def test_rotation(eng, t, neighbours, rows, heads, dim, rotated, extra, in_place
     assert torch.equal(rest, before[:, heads * dim:] if in_place else torch.full_like(rest, 7.0))
 
 
+def test_rotation_of_more_rows_than_workgroups(eng):
+    # More than 2^21 workgroups of one row each: workgroups take a second row.
+    rows, heads, dim = (1 << 21) + 700, 129, 16
+    x = torch.zeros(rows, heads * dim, dtype=torch.float16, device="cuda")
+    some = torch.cat([torch.arange(64, device="cuda"), torch.arange(rows - 764, rows, device="cuda")])
+    x[some] = normal(gen(9), torch.float16, some.numel(), heads * dim)
+    angle = torch.rand(50, dim // 2, generator=gen(10), device="cuda")
+    index = (torch.arange(rows, device="cuda") % 50).int()
+    want = torch.empty(some.numel(), heads * dim, dtype=torch.float16, device="cuda")
+    run_rotation(eng, x[some], want, index[some], angle.cos(), angle.sin(), heads, dim, dim, 0)
+    run_rotation(eng, x, x, index, angle.cos(), angle.sin(), heads, dim, dim, 0)
+    torch.cuda.synchronize()
+    assert torch.equal(x[some], want) and not x[64:4096].any()
+
+
 # --- projection with adapters ------------------------------------------------
 
 def run_linear(e, x, w, bias, a, b, scale, y, starts, ids, rows=None, stream=0, workspace=None):

@@ -46,6 +46,8 @@ REFUSED = [
     ("linear", dict(rank=264), "rank must be at most 256"),
     ("linear", dict(adapters=0), "adapters must be positive"),
     ("linear", dict(rows=1 << 31), "rows must be at most"),
+    ("linear", dict(rows=(1 << 27) + 1), "rows must be at most"),
+    ("linear", dict(rows=1 << 27, outputs=1 << 20), "the number of tiles of 256 x 256 outputs must be at most"),
     ("linear", dict(x=0), "x is a null device pointer"),
     ("linear", dict(w=A + 8), "w must be 16-byte aligned"),
     ("linear", dict(bias=A + 4), "bias must be 16-byte aligned"),
@@ -91,6 +93,8 @@ REFUSED = [
     ("attention", dict(k_head_stride=56), "head strides must be at least head_dim"),
     ("attention", dict(out_stride=504), "out_stride and out_head_stride make heads overlap"),
     ("attention", dict(q_rows=1 << 30), "q_rows * (heads / kv_heads) must be at most"),
+    ("attention", dict(scale=2.0 ** 21), "scale must be at most 2^20"),
+    ("attention", dict(k_rows=(1 << 31) - 300), "q_rows + k_rows must be at most"),
     ("attention", dict(sequences=1 << 24), "the number of row tiles must be at most"),
 ]
 
