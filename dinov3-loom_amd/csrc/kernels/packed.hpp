@@ -42,7 +42,8 @@ struct Num<bf16_t> {
 // How a launch is cut; the workspace function and the launcher decide alike.
 struct AttentionCut {
     bool few;         // 32-row tiles whose waves share the keys out
-    int waves;        // of a workgroup (few only)
+    int tile;         // rows of a tile (not few)
+    int waves;        // of a workgroup
     uint32_t splits;  // parts of the longest sequence's keys (few only)
     uint64_t span;    // key blocks of 32 in a part
     uint64_t slots;   // workgroups per key head

@@ -68,28 +68,29 @@ struct Tile {
     int row0;            // first row of the tile within the sequence, in rows of the group
 };
 
-// Finds the tile of 128 rows of slot `slot`: sequence s has the slots from
-// starts[s] * group / 128 + s on, at least as many as it has tiles. False if the
+// Finds the tile of 2^SHIFT rows of slot `slot`: sequence s has the slots from
+// starts[s] * group / 2^SHIFT + s on, at least as many as it has tiles. False if the
 // slot has no rows. For up to 64 sequences a lane holds one of them: one load's
 // latency. (Tiles handed out by the keys they see, most first, were no faster:
 // 145 us against 145 for ten ragged prompts, 94 against 95 for 39 images of
 // 201 to 4101 tokens, and their search cost 1.5 us.)
+template <int SHIFT>
 __device__ __forceinline__ bool find_tile(Tile& t, int slot, const int32_t* q_starts, const int32_t* k_starts, int sequences,
                                           int group, int q_rows, int k_rows) {
     const int lane = threadIdx.x & 63;
     int s = 0;
-    auto base = [&](int s) { return (int64_t)((uint32_t)start_at(q_starts, s, q_rows) * (uint32_t)group >> 7) + s; };
+    auto base = [&](int s) { return (int64_t)((uint32_t)start_at(q_starts, s, q_rows) * (uint32_t)group >> SHIFT) + s; };
     if (sequences > 64) s = max(wave_last(sequences, slot, base), 0);
     const int mine = min(s + lane, sequences - 1);  // of many only the first counts
     const int q0 = start_at(q_starts, mine, q_rows), q1 = start_at(q_starts, mine + 1, q_rows);
     const int k0 = start_at(k_starts, mine, k_rows), k1 = start_at(k_starts, mine + 1, k_rows);
-    const int64_t from = (int64_t)((uint32_t)q0 * (uint32_t)group >> 7) + mine;
+    const int64_t from = (int64_t)((uint32_t)q0 * (uint32_t)group >> SHIFT) + mine;
     const int j = sequences > 64 ? 0 : max(__builtin_popcountll(__ballot(lane < sequences && from <= slot)) - 1, 0);
     t.q0 = __builtin_amdgcn_readlane(q0, j);
     t.lq = max(0, __builtin_amdgcn_readlane(q1, j) - t.q0);
     t.k0 = __builtin_amdgcn_readlane(k0, j);
     t.lk = max(0, __builtin_amdgcn_readlane(k1, j) - t.k0);
-    const int64_t row0 = ((int64_t)slot - (int64_t)((uint32_t)t.q0 * (uint32_t)group >> 7) - (s + j)) * 128;
+    const int64_t row0 = ((int64_t)slot - (int64_t)((uint32_t)t.q0 * (uint32_t)group >> SHIFT) - (s + j)) << SHIFT;
     if (row0 < 0 || row0 >= (int64_t)t.lq * group) return false;
     t.row0 = (int)row0;
     return true;
@@ -306,24 +307,24 @@ __device__ __forceinline__ void store_row(const Row<T, D>& st, T* out, float* ls
         lse[(uint64_t)(t.q0 + token) * heads + head0 + h] = st.l > 0.f ? (st.m * c + __log2f(st.l)) * kLn2 : -__builtin_inff();
 }
 
-// A tile of 128 rows, 32 per wave; the four waves of a group share blocks of 64
-// keys, the next one on its way while one is used. GROUPS = 2: two such groups
-// take the blocks in turn and join at the end, which halves the time of a tile
-// alone on a CU.
-template <class T, int D, int GROUPS>
-__global__ __launch_bounds__(256 * GROUPS, D <= 64 ? 4 : 2) void packed_attention_kernel(DHX_PACKED_ATTENTION_PARAMS) {
+// A tile of 32 WAVES rows, 32 per wave; the waves of a group share blocks of 16
+// WAVES keys, the next one on its way while one is used. GROUPS > 1: so many such
+// groups take the blocks in turn and join at the end, which shortens a tile's
+// chain where it has a CU to itself.
+template <class T, int D, int GROUPS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES * GROUPS, D <= 64 ? 4 : 2) void packed_attention_kernel(DHX_PACKED_ATTENTION_PARAMS) {
     using G = Geo<D>;
-    constexpr int KB = 64, LOADS = KB / 4 / G::ROWS, BLK = KB * G::PITCH;
+    constexpr int KB = 16 * WAVES, LOADS = KB / WAVES / G::ROWS, BLK = KB * G::PITCH;
     __shared__ __attribute__((aligned(16))) T sK0[GROUPS * BLK], sK1[GROUPS * BLK];
     __shared__ __attribute__((aligned(16))) T sV0[GROUPS * BLK], sV1[GROUPS * BLK];
-    __shared__ float2_t sML[GROUPS > 1 ? GROUPS - 1 : 1][4][32];
+    __shared__ float2_t sML[GROUPS > 1 ? GROUPS - 1 : 1][WAVES][32];
     const Place at = place_of(blockIdx.x, slots, kv_heads);
     if (at.head >= kv_heads || at.item >= slots) return;
     Tile t;
     // From the last slot on: a causal prompt's longest tiles begin first.
-    if (!find_tile(t, slots - 1 - at.item, q_starts_, k_starts_, sequences, group, q_rows, k_rows)) return;
+    if (!find_tile<WAVES == 4 ? 7 : 6>(t, slots - 1 - at.item, q_starts_, k_starts_, sequences, group, q_rows, k_rows)) return;
     const int tid = threadIdx.x, lane = tid & 63, all_waves = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wave = all_waves & 3, part = all_waves >> 2;
+    const int wave = all_waves % WAVES, part = all_waves / WAVES;
     const int l32 = lane & 31, hi = lane >> 5;
     const int head0 = at.head * group;
 
@@ -332,18 +333,18 @@ __global__ __launch_bounds__(256 * GROUPS, D <= 64 ? 4 : 2) void packed_attentio
     load_row(st, (const T*)q_ + head0 * q_head, t, row, group, head_dim, causal, q_stride, q_head, hi);
     // Keys that the tile's last row sees, those that all rows of this wave see,
     // and those that any of them sees.
-    const int rows = t.lq * group, last = min(t.row0 + 127, rows - 1), wave_last_row = min(first + 31, rows - 1);
+    const int rows = t.lq * group, last = min(t.row0 + 32 * WAVES - 1, rows - 1), wave_last_row = min(first + 31, rows - 1);
     auto seen = [&](int r) { return causal ? min(max(r / group + 1 + t.lk - t.lq, 0), t.lk) : t.lk; };
     const int keys = seen(last), all = seen(min(first, rows - 1)), any = first < rows ? seen(wave_last_row) : 0;
     const int blocks = (keys + KB - 1) / KB;
 
-    const Mover<D, LOADS> mk((const T*)k_ + (uint64_t)t.k0 * k_stride + at.head * k_head, k_stride, head_dim, wave * (KB / 4), lane);
-    const Mover<D, LOADS> mv((const T*)v_ + (uint64_t)t.k0 * v_stride + at.head * v_head, v_stride, head_dim, wave * (KB / 4), lane);
+    const Mover<D, LOADS> mk((const T*)k_ + (uint64_t)t.k0 * k_stride + at.head * k_head, k_stride, head_dim, wave * (KB / WAVES), lane);
+    const Mover<D, LOADS> mv((const T*)v_ + (uint64_t)t.k0 * v_stride + at.head * v_head, v_stride, head_dim, wave * (KB / WAVES), lane);
     const LaneAt la = lane_at<G::PITCH>(lane);
     T *k0 = sK0 + part * BLK, *k1 = sK1 + part * BLK, *v0 = sV0 + part * BLK, *v1 = sV1 + part * BLK;
     auto move = [&](T* k, T* v, int b) {
-        mk.move(b * KB, t.lk - b * KB, KB, head_dim, k + wave * (KB / 4) * G::PITCH);
-        mv.move(b * KB, t.lk - b * KB, KB, head_dim, v + wave * (KB / 4) * G::PITCH);
+        mk.move(b * KB, t.lk - b * KB, KB, head_dim, k + wave * (KB / WAVES) * G::PITCH);
+        mv.move(b * KB, t.lk - b * KB, KB, head_dim, v + wave * (KB / WAVES) * G::PITCH);
     };
     auto step = [&](T* k, T* v, T* next_k, T* next_v, int b) {
         wait_vm<0>();  // block b has landed, and no wave reads the other block any more
@@ -519,30 +520,30 @@ __global__ __launch_bounds__(64 * NW, 1) void packed_attention_few_kernel(DHX_PA
         }
         __syncthreads();
         if (wave == 0) {
-        float m = kNoMax, l = 0.f, part[NW];
+            float m = kNoMax, l = 0.f, part[NW];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) m = fmaxf(m, sML[w][l32][0]);
+            for (int w = 0; w < NW; ++w) m = fmaxf(m, sML[w][l32][0]);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            part[w] = fast_exp2((sML[w][l32][0] - m) * c);
-            l += part[w] * sML[w][l32][1];
-        }
-        st.m = m;
-        st.l = l;
-#pragma unroll
-        for (int ct = 0; ct < G::CT; ++ct)
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4) {
-                const int piece = (ct * 32 % HALF) / 4 + 2 * g4 + hi;
-                float4_t sum = {};
-#pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    const float* o = (const float*)((ct * 32 < HALF ? sK0 : sV0) + w * BLK) + l32 * HALF;
-                    sum += part[w] * *(const float4_t*)(o + ((piece ^ (l32 % PIECES)) << 2));
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) st.o[ct][4 * g4 + e] = sum[e];
+            for (int w = 0; w < NW; ++w) {
+                part[w] = fast_exp2((sML[w][l32][0] - m) * c);
+                l += part[w] * sML[w][l32][1];
             }
+            st.m = m;
+            st.l = l;
+#pragma unroll
+            for (int ct = 0; ct < G::CT; ++ct)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int piece = (ct * 32 % HALF) / 4 + 2 * g4 + hi;
+                    float4_t sum = {};
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) {
+                        const float* o = (const float*)((ct * 32 < HALF ? sK0 : sV0) + w * BLK) + l32 * HALF;
+                        sum += part[w] * *(const float4_t*)(o + ((piece ^ (l32 % PIECES)) << 2));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st.o[ct][4 * g4 + e] = sum[e];
+                }
         }
     }
     if (NW == 1 || wave == 0) {
@@ -639,14 +640,20 @@ hipError_t launch(const dhx_packed_attention& p, const AttentionCut& cut, hipStr
     const uint64_t grid = 8 * (p.kv_heads / share) * ((cut.slots + m - 1) / m);
     const float c = p.scale * kLog2e;
     auto tile = [&](auto kernel, int groups) {
-        return enqueue(kernel, dim3((unsigned)grid), dim3(256 * groups), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v,
+        return enqueue(kernel, dim3((unsigned)grid), dim3(64 * groups), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v,
                        (int)p.sequences, group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows, (int)p.causal,
                        (int)cut.slots, 1, c, p.out, p.lse, p.workspace, p.q_stride, p.k_stride, p.v_stride, p.out_stride,
                        p.q_head_stride, p.k_head_stride, p.v_head_stride, p.out_head_stride);
     };
-    if constexpr (D <= 64)
-        if (!cut.few && cut.waves == 16) return tile(packed_attention_kernel<T, D, 4>, 4);
-    if (!cut.few) return cut.waves >= 8 ? tile(packed_attention_kernel<T, D, 2>, 2) : tile(packed_attention_kernel<T, D, 1>, 1);
+    if (!cut.few) {
+        if constexpr (D <= 64) {
+            if (cut.tile == 64) return tile(packed_attention_kernel<T, D, 8, 2>, 16);
+            if (cut.waves == 16) return tile(packed_attention_kernel<T, D, 4, 4>, 16);
+        } else {
+            if (cut.tile == 64) return tile(packed_attention_kernel<T, D, 4, 2>, 8);
+        }
+        return cut.waves == 8 ? tile(packed_attention_kernel<T, D, 2, 4>, 8) : tile(packed_attention_kernel<T, D, 1, 4>, 4);
+    }
     auto few = [&](auto kernel, int waves) {
         return enqueue(kernel, dim3((unsigned)grid), dim3(64 * waves), 0, s, p.q_starts, p.k_starts, p.q, p.k, p.v, (int)p.sequences,
                        group, (int)p.kv_heads, (int)p.head_dim, (int)p.q_rows, (int)p.k_rows, (int)p.causal, (int)cut.slots,
@@ -655,8 +662,9 @@ hipError_t launch(const dhx_packed_attention& p, const AttentionCut& cut, hipStr
     };
     const hipError_t err = cut.waves == 4 ? few(packed_attention_few_kernel<T, D, 4>, 4) : few(packed_attention_few_kernel<T, D, 2>, 2);
     if (err != hipSuccess || cut.splits == 1) return err;
-    return enqueue(packed_join_kernel<T, D>, dim3((unsigned)std::min<uint64_t>((p.q_rows * p.heads + 3) / 4, 1u << 20)), dim3(kThreads), 0, s, p.workspace,
-                   p.q_starts, p.out, p.lse, (int)p.sequences, (int)p.q_rows, (int)p.heads, (int)p.head_dim, (int)cut.splits,
+    const uint64_t joins = std::min<uint64_t>((p.q_rows * p.heads + 3) / 4, 1u << 20);
+    return enqueue(packed_join_kernel<T, D>, dim3((unsigned)joins), dim3(kThreads), 0, s, p.workspace, p.q_starts,
+                   p.out, p.lse, (int)p.sequences, (int)p.q_rows, (int)p.heads, (int)p.head_dim, (int)cut.splits,
                    c, p.out_stride, p.out_head_stride);
 }
 
@@ -674,24 +682,42 @@ hipError_t launch_type(const dhx_packed_attention& p, const AttentionCut& cut, h
 
 }  // namespace
 
-// How a launch is cut (times in us, few-rows kernel against 128-row tiles, on
-// MI355X). Sequences of at most 32 rows have no use for more: single tokens of
-// 48 requests with 32 heads of 128 on 8, 118k keys together, 94 against 657.
-// Below 96 tiles of 128 rows most of the chip would idle: 1029 rows and keys,
-// 6 heads of 64, 14.1 against 19.4 (54 tiles); five images of 201 tokens 6.9
-// against 7.4 (72); 512 causal tokens, 32 heads of 128 on 8, 16.7 against 15.6
-// (136); 16 images 12.1 against 8.1 (246).
-constexpr uint64_t kFewRows = 32, kFewTiles = 96;
-// Where the tiles are few enough to run at once, the time of one counts, and
-// groups of waves share its keys: 2048 causal tokens, 32 heads of 128 on 8, 46.5
-// with two groups, 52.0 with one (520 tiles), 4096 tokens 154 against 148
+// How a launch is cut (times in us on MI355X; causal where heads are grouped).
+//
+// Few-rows kernel: sequences of at most 32 rows have no use for taller tiles:
+// single tokens of 48 requests with 32 heads of 128 on 8, 118k keys together, 94
+// against 657. And launches of few tiles (in tiles of 64 rows) leave CUs idle
+// that parts of the keys fill. Against the best of the others, heads of 64: 1029
+// rows and keys of 6 heads 12.2 and 16.0 (102 tiles), five images of 201 tokens
+// 7.2 and 7.9 (108), 16384 keys of 1029 rows 132 and 138; but 256 tokens, 32 heads
+// on 8, 15.0 and 9.1 (128), 1400 rows and keys, 6 heads, 27.3 and 21.4 (132). Wide
+// heads have the chain of a tile shortened by half tiles already, and parts pay
+// only along more blocks than there are tiles: 32 heads of 128 on 8, 64 tokens
+// (32 tiles) behind 2048 keys 18.5 and 24.6, 1024 keys 15.8 and 16.2; 128 (64)
+// behind 4096 37 and 44, 2048 26.1 and 24.6, 512 12.6 and 11.8; 256 (128) behind
+// 8192 108 and 80, 256 16.8 and 9.9.
+constexpr uint64_t kFewRows = 32, kFewTiles = 112, kLeastParted = 16;
+// Tiles of 64 rows, their keys shared by twice the groups, where there is a CU
+// for each: a tile's chain is half as long, but a second round of them costs more
+// than that. Wide heads, against 128 rows: 512 tokens, 32 heads of 128 on 8, 12.2
+// and 14.5 (256 tiles), behind 8192 keys 86 and 121; 1024 tokens, 16 heads of 80,
+// 15.7 and 19.6 (256); but 1029 of them 29.6 and 19.8 (272). Heads up to 64, whose
+// 128 rows can have four groups too, only along many blocks, for the eight groups
+// have to join: 300 tokens, 32 heads on 8, behind 8192 keys 77 and 96 (160), 4096
+// 45 and 52, 3000 37 and 39, 2048 29 and 28, 1024 21.5 and 18.3.
+constexpr uint64_t kCUs = 256, kEightGroups = 96;
+// Where tiles of 128 rows are few enough to run at once, the time of one counts,
+// and groups of waves share its keys: 2048 causal tokens, 32 heads of 128 on 8,
+// 46.5 with two groups, 52.0 with one (520 tiles), 4096 tokens 154 against 148
 // (1032); ragged prompts with 16 heads of 80 28.0, 29.6 (400); 4101 rows and keys,
-// 6 heads of 64, 42.1 with four, 50.3 with two, 72.3 with one (198), but 16 images
-// of 201 tokens 10.3, 8.2, 8.5 (246).
-constexpr uint64_t kShareTiles = 600;
+// 6 heads of 64, 42.1 with four, 50.3 with two, 72.3 with one (198). Four groups
+// along blocks enough: 2000 rows and keys 27.2, 31.6 (two), twice 1029 18.9, 19.8,
+// three times 581 (19 blocks) 14.6, 13.6.
+constexpr uint64_t kShareTiles = 600, kFourGroups = 32;
 // Four waves share a tile's keys, without parts, where at most 256 items have
 // few enough blocks: 201 x 201, 6 heads, 6.9 (two waves 7.8); four queries and
-// 1029 keys of 16 images, 12 heads of 64, 14.3 (16.3). Else two: their
+// 1029 keys of 16 images, 12 heads of 64, 14.3 (16.3); 581 x 581, 6 heads, 9.4
+// (13.8; 114 items). Else two: their
 // workgroups are more and their joins smaller. A part then has a 384th of all
 // blocks and no fewer than 4: one token, 1000 keys, 32 heads of 128 on 8, 11.4
 // (16 blocks 17.2), 8192 keys 15.6 with 8 blocks (64 blocks 43); the 48 requests
@@ -706,17 +732,23 @@ AttentionCut packed_attention_cut(const dhx_packed_attention& p) {
     cut.splits = 1;
     const uint64_t group = p.heads / p.kv_heads, rows = p.q_rows * group;
     const uint64_t longest = std::min<uint64_t>(p.longest_q ? p.longest_q : p.q_rows, p.q_rows) * group;
-    cut.slots = rows / 128 + p.sequences;
-    cut.few = longest <= kFewRows || cut.slots * p.kv_heads < kFewTiles;
     const uint64_t keys = std::min<uint64_t>(p.longest_k ? p.longest_k : p.k_rows, p.k_rows), blocks = (keys + 31) / 32;
+    // Tiles of 64 rows, if each sequence behind the first one ends in the middle of one.
+    const uint64_t halves = (rows + 32 * (uint64_t)p.sequences + 31) / 64 * p.kv_heads;
+    const bool wide = p.head_dim > 64;  // else a wave's state leaves room for twice the waves
+    cut.few = longest <= kFewRows || (halves <= kFewTiles && (!wide || blocks > std::max(halves, kLeastParted)));
     if (!cut.few) {
+        const bool half = halves <= kCUs && (wide || blocks >= kEightGroups);
+        cut.slots = rows / (half ? 64 : 128) + p.sequences;
         const uint64_t count = cut.slots * p.kv_heads;
-        cut.waves = count > kShareTiles ? 4 : count <= 256 && blocks >= 64 && p.head_dim <= 64 ? 16 : 8;
+        cut.tile = half ? 64 : 128;
+        if (half) cut.waves = wide ? 8 : 16;
+        else cut.waves = count > kShareTiles ? 4 : count <= kCUs && blocks >= kFourGroups && !wide ? 16 : 8;
         return cut;
     }
     const uint64_t tiles = std::min<uint64_t>(rows / 32 + p.sequences, rows);
     const uint64_t items = tiles * p.kv_heads;
-    cut.waves = items <= 256 && (blocks <= 16 || (items >= 128 && blocks <= 40)) ? 4 : 2;
+    cut.waves = items <= 256 && (blocks <= 16 || (items >= 96 && blocks <= 40)) ? 4 : 2;
     if (cut.waves == 2) {
         // Blocks that all tiles walk, if each sequence has its share of both.
         const uint64_t per_sequence = (rows + 32ull * p.sequences - 1) / (32ull * p.sequences);

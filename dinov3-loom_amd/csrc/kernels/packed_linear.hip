@@ -117,10 +117,11 @@ struct Stream {
 
 #define DHX_SHRINK_PARAMS Addr starts_, Addr adapter_, Addr x_, Addr a_, Addr scale_, int sequences, int rows, int adapters, int inputs, int rank, Addr ids_, Addr u_, uint64_t x_stride
 
-// The adapter of `row` (per lane, row0 + lane % TILE), as above. A lane holds the first row of one of 64 sequences,
-// those from the one of row0 on, and a row's sequence is the last one that does
-// not begin behind it: one load's latency for batches of up to 64 sequences.
-// Rows behind the window (only where sequences in it are empty) are searched.
+// The adapter of `row` (per lane, row0 + lane % TILE), or one of the two above. A
+// lane holds the first row of one of 64 sequences, those from the one of row0 on,
+// and a row's sequence is the last one that does not begin behind it: one load's
+// latency for batches of up to 64 sequences. Rows behind the window (only where
+// sequences in it are empty) are searched.
 template <int TILE>
 __device__ __forceinline__ int adapter_of(int row, int row0, const int32_t* starts, const int32_t* adapter, int sequences,
                                           int rows, int adapters) {

@@ -400,6 +400,22 @@ def test_attention_routes(eng, t, dim, ql, kl, heads, kv):
     assert torch.equal(first, again)  # the same bits from launch to launch
 
 
+# Half tiles with four groups (wide heads) and eight (narrow ones, many keys),
+# two groups on 128 rows, and the few-rows kernel beside them.
+ROUTES_FEW_TILES = [([500], [500], 16, 8), ([300], [3300], 32, 8), ([150, 0, 77, 260], [3500, 10, 0, 3301], 16, 4),
+                    ([700] * 3, [700] * 3, 16, 16), ([581], [581], 6, 6), ([64], [4100], 8, 2), ([1400], [1399], 6, 6)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("causal", [0, 1])
+@pytest.mark.parametrize("dim", [32, 64, 80, 128])
+@pytest.mark.parametrize("ql,kl,heads,kv", ROUTES_FEW_TILES)
+def test_attention_routes_of_few_tiles(eng, t, causal, dim, ql, kl, heads, kv):
+    args = eng, TYPES[t][1], ql, kl, heads, kv, dim, causal
+    first = check_attention(*args, hints=(max(ql), max(kl)))
+    assert torch.equal(first, check_attention(*args, hints=(max(ql), max(kl))))  # the same bits from launch to launch
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("causal", [0, 1])
 def test_attention_rows_of_no_sequence(eng, t, causal):
