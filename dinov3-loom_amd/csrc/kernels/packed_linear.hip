@@ -18,8 +18,17 @@ namespace {
 constexpr int kNoAdapter = -1;   // a row of a sequence without adapter
 constexpr int kNoSequence = -2;  // a row of no sequence: its y stays as it was
 
-// Up to so many rows the few-rows kernel takes the product.
-constexpr uint64_t kFewRows = 64;
+// The few-rows kernel takes the product up to 64 rows, and up to 512 where a tile
+// would walk many columns alone and the few-rows kernel's workgroups (16 columns
+// of y and 64 rows) find a CU each. us, against tiles: 4096 columns to 1024, 256
+// rows, 21.7 and 30.5 (256 workgroups; rank 64 25.6 and 39.6), 384 rows 35.9 and
+// 30.7 (384); 2048 to 2048, 128 rows, 16.0 and 19.5 (256); 1536 to 384, 512 rows,
+// 15.4 and 16.7 (192); but 384 to 1152, 128 rows, 10.1 and 9.8 (144).
+constexpr uint64_t kFewRows = 64, kMostFewRows = 512, kLongColumns = 1024;
+bool few_rows(const dhx_packed_linear& p) {
+    return p.rows <= kFewRows || (p.rows <= kMostFewRows && p.inputs >= kLongColumns &&
+                                  (p.rows + 63) / 64 * ((p.outputs + 15) / 16) <= 256);
+}
 constexpr int kMostParts = 4;
 
 struct Workspace {
@@ -32,7 +41,7 @@ Workspace layout(const dhx_packed_linear& p) {
     // A run's columns in parts where rows are few: a CU reads no more than about
     // 40 GB/s of A, and 24 single tokens' adapters (4096 columns, rank 16) would
     // keep 24 of them busy.
-    w.parts = p.rows <= kFewRows ? (uint32_t)std::min<uint64_t>(std::max<uint32_t>(p.inputs / 1024, 1), kMostParts) : 1;
+    w.parts = few_rows(p) ? (uint32_t)std::min<uint64_t>(std::max<uint32_t>(p.inputs / 1024, 1), kMostParts) : 1;
     w.bytes = w.u + p.rows * p.rank * (w.parts > 1 ? 4 * w.parts : 2);
     return w;
 }
@@ -570,8 +579,8 @@ hipError_t launch(const dhx_packed_linear& p, hipStream_t s) {
     const hipError_t err = narrow ? p.rank <= 16 ? shrink(packed_shrink_kernel<T, 1, 2>, 2) : shrink(packed_shrink_kernel<T, 2, 2>, 2)
                                   : p.rank <= 16 ? shrink(packed_shrink_kernel<T, 1, 4>, 4) : shrink(packed_shrink_kernel<T, 2, 4>, 4);
     if (err != hipSuccess) return err;
-    // Times in us, whole calls on MI355X. Up to 64 rows W alone counts: 64 rows,
-    // 4096 x 4096, 31 (64 x 64 tiles 43). Then the largest tile of which there are
+    // Times in us, whole calls on MI355X. For few rows W alone counts: 64 rows,
+    // 4096 x 4096, 22 (64 x 64 tiles 31). Then the largest tile of which there are
     // enough for the 256 CUs: 16384 rows, 4096 x 4096, 498 with 256 x 256 (128 x
     // 128 597), 4096 rows 130 (152; 256 tiles); 12864 rows, 384 x 1152, 29 (31; 255
     // tiles), 8192 rows, 1024 x 1024, 38 (30; 128 tiles); 1024 rows, 4096 x 4096,
@@ -580,7 +589,7 @@ hipError_t launch(const dhx_packed_linear& p, hipStream_t s) {
     // stages 31 (256 tiles), in two 43.
     if (p.rows <= 16) return few<T, 1>(p, ids, u, w.parts, s);
     if (p.rows <= 32) return few<T, 2>(p, ids, u, w.parts, s);
-    if (p.rows <= kFewRows) return few<T, 4>(p, ids, u, w.parts, s);
+    if (few_rows(p)) return few<T, 4>(p, ids, u, w.parts, s);
     auto count = [&](uint64_t m, uint64_t n) { return (p.rows + m - 1) / m * ((p.outputs + n - 1) / n); };
     if (count(256, 256) >= 224) return tiles<T, 256, 256, 128, 64, 64, 2, false, 2>(p, ids, u, s);
     if (count(128, 128) >= 300) return tiles<T, 128, 128, 64, 64, 64, 2, false, 2>(p, ids, u, s);

@@ -234,6 +234,34 @@ def test_linear_routes(eng, t, kind, rows, inputs, outputs):
     assert torch.equal(y, again)  # the same bits from launch to launch
 
 
+# The few-rows kernel over several blocks of 64 rows (the last one not whole),
+# and the first sizes behind it: more rows, more workgroups, fewer columns.
+ROUTES_OF_SOME_ROWS = [(65, 1032, 264), (128, 2056, 520), (200, 4096, 1024), (511, 1536, 384), (512, 1024, 8), (513, 1536, 384),
+                       (130, 1024, 1376), (400, 1016, 264)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rank", [8, 40])
+@pytest.mark.parametrize("kind", ["ragged", "single"])
+@pytest.mark.parametrize("rows,inputs,outputs", ROUTES_OF_SOME_ROWS)
+def test_linear_of_some_rows(eng, t, rank, kind, rows, inputs, outputs):
+    dt = TYPES[t][1]
+    g = gen(rows + outputs)
+    st = list(range(rows + 1)) if kind == "single" else [0, 0, 3, 60, 70, 127, 131][:4 if rows < 131 else 7] + [rows - 1]
+    adapters = 5
+    x, w = normal(g, dt, rows, inputs), normal(g, dt, outputs, inputs, scale=inputs ** -0.5)
+    a, b = normal(g, dt, adapters, rank, inputs, scale=inputs ** -0.5), normal(g, dt, adapters, outputs, rank, scale=rank ** -0.5)
+    scale = torch.rand(adapters, generator=g, device="cuda") + 0.5
+    bias = torch.randn(outputs, generator=g, device="cuda")
+    ids = [(s * 3) % (adapters + 1) - 1 for s in range(len(st) - 1)]
+    y = torch.full((rows, outputs), 7.0, device="cuda").to(dt)
+    run_linear(eng, x, w, bias, a, b, scale, y, ints(st), ints(ids))
+    torch.cuda.synchronize()
+    want, bound = linear_want(x, w, bias, a, b, scale, [(st[s], st[s + 1], i) for s, i in enumerate(ids)])
+    within(y[:st[-1]], want[:st[-1]], bound[:st[-1]], dt)
+    assert (y[st[-1]:] == 7.0).all()  # of no sequence
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("first,lengths,behind", [(0, [7, 30], 91), (13, [40, 1, 100], 5), (3, [0], 60), (130, [1, 1, 1], 130)])
 def test_linear_leaves_rows_of_no_sequence(eng, t, first, lengths, behind):
