@@ -99,7 +99,9 @@ void rotation_check(const dhx_packed_rotation& p) {
     most(p.rows, kMaxRows, "rows");
     positive(p.heads, "heads");
     eights(p.head_dim, "head_dim");
-    if (p.rotated == 0 || p.rotated % 16 != 0) throw Error("rotated must be a positive multiple of 16");
+    const bool part = (uint64_t)p.rotated * 2 == p.head_dim || p.rotated == p.head_dim;
+    if (p.rotated == 0 || p.rotated % (part ? 8 : 16) != 0)
+        throw Error("rotated must be a positive multiple of 16, or a multiple of 8 that is head_dim or half of it");
     if (p.rotated > p.head_dim) throw Error("rotated must be at most head_dim");
     positive(p.places, "places");
     most(p.places, kMaxRows, "places");

@@ -81,8 +81,10 @@ int dhx_packed_linear_run(dhx_engine *e, const dhx_packed_linear *p, void *strea
 /* The position rotation of each row's heads, with the angles of the row's own
  * place: out = (x1 cos - x2 sin, x2 cos + x1 sin) for the pairs (x1, x2) of the
  * first `rotated` channels of every head, with cos and sin of row index[t] of
- * the tables. The pairs are the channels (j, j + rotated/2) or, with
- * `neighbours`, (2j, 2j + 1); angle j is column j of the tables. Channels from
+ * the tables. `rotated` is a multiple of 16, or a multiple of 8 that is head_dim
+ * or half of it (40 of heads of 80). The pairs are the channels (j, j +
+ * rotated/2) or, with `neighbours`, (2j, 2j + 1); angle j is column j of the
+ * tables. Channels from
  * `rotated` on are copied, and so is a row whose index is outside 0 ..
  * places-1 (the CLS and register rows of an image, say). out may be x itself
  * with the same stride (in place), for the q and k heads at the front of packed
