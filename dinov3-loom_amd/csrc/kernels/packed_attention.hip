@@ -730,6 +730,7 @@ constexpr uint64_t kFewGroups = 2048;
 AttentionCut packed_attention_cut(const dhx_packed_attention& p) {
     AttentionCut cut{};
     cut.splits = 1;
+    if (p.q_rows == 0) return cut;  // nothing is launched, and there is no tile to share keys out to
     const uint64_t group = p.heads / p.kv_heads, rows = p.q_rows * group;
     const uint64_t longest = std::min<uint64_t>(p.longest_q ? p.longest_q : p.q_rows, p.q_rows) * group;
     const uint64_t keys = std::min<uint64_t>(p.longest_k ? p.longest_k : p.k_rows, p.k_rows), blocks = (keys + 31) / 32;

@@ -7,7 +7,10 @@ import random
 
 import pytest
 
-from test_packed import message
+import dinov3_hrx as d
+from dinov3_hrx import packed
+
+from test_packed import ATTENTION, message
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -57,3 +60,15 @@ def test_the_timed_ranges_are_taken():
         assert message(name, **change) == "null engine", case
         seen[name, case.get("rotated") == 40] = seen.get((name, case.get("rotated") == 40), 0) + 1
     assert all(seen.get(k, 0) > 20 for k in (("attention", False), ("linear", False), ("rotation", False), ("rotation", True))), seen
+
+
+# --- no queries --------------------------------------------------------------
+
+@pytest.mark.parametrize("k_rows", [0, 1, 512, 513, 1 << 20])
+@pytest.mark.parametrize("longest_k", [0, 1, 513, 1 << 20])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (32, 8, 128), (1, 1, 8)])
+def test_attention_without_queries_needs_nothing(k_rows, longest_k, heads, kv, dim):
+    sizes = dict(q_rows=0, k_rows=k_rows, longest_k=longest_k, heads=heads, kv_heads=kv, head_dim=dim, q=0, out=0, q_stride=heads * dim,
+                 out_stride=heads * dim, k_stride=kv * dim, v_stride=kv * dim, workspace=0, workspace_bytes=0)
+    assert d.packed_workspace("attention", packed.Attention(**{**ATTENTION, **sizes})) == 0
+    assert message("attention", **sizes) == "null engine"
