@@ -71,6 +71,19 @@ __device__ __forceinline__ void dma16(const void* from, void* to) {
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
+// Of the two values in a word, bits 15 and 31: the value is not finite (its
+// exponent is ones only). Other bits hold anything.
+template <class T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t two) {
+    constexpr uint32_t EXP = __is_same(T, half_t) ? 0x7c00u : 0x7f80u;
+    return (two & (EXP * 0x10001u)) + (0x8000u - EXP) * 0x10001u;
+}
+template <class T>
+__device__ __forceinline__ bool any_not_finite(typename Num<T>::v8 v) {
+    const uint4_t w = __builtin_bit_cast(uint4_t, v);
+    return ((not_finite<T>(w[0]) | not_finite<T>(w[1]) | not_finite<T>(w[2]) | not_finite<T>(w[3])) & 0x80008000u) != 0;
+}
+
 // s_waitcnt vmcnt(N) that the compiler's own wait insertion can see.
 template <int N>
 __device__ __forceinline__ void wait_vm() {

@@ -125,15 +125,13 @@ template <class T, int D>
 __device__ __forceinline__ void add_not_finite(Row<T, D>& st, typename Num<T>::v8 (&va)[Geo<D>::CT][2], int key0, int hi) {
     using G = Geo<D>;
     typedef typename Num<T>::v8 v8;
-    constexpr uint32_t EXP = __is_same(T, half_t) ? 0x7c00u : 0x7f80u;
-    uint32_t all = 0;  // bit 15 and 31: an exponent of ones somewhere
+    uint32_t all = 0;
 #pragma unroll
     for (int ct = 0; ct < G::CT; ++ct)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-                all |= (__builtin_bit_cast(uint4_t, va[ct][ks])[w] & (EXP * 0x10001u)) + (0x8000u - EXP) * 0x10001u;
+            for (int w = 0; w < 4; ++w) all |= not_finite<T>(__builtin_bit_cast(uint4_t, va[ct][ks])[w]);
     if (__builtin_expect(!__any((all & 0x80008000u) != 0), 1)) return;
     const int left = st.limit - key0 - 4 * hi;
     v8 seen[2];

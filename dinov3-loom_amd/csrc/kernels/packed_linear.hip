@@ -7,7 +7,10 @@
 // product over all columns of x, continued over those of u: a tile's rows
 // belong to runs of rows with one adapter, and run j adds rank columns
 // [u of the run's rows, 0 elsewhere] . B_a^T. So adapters cost the product
-// rank columns per run in a tile, and no pass over y.
+// rank columns per run in a tile, and no pass over y. A value of B that is not
+// finite would make 0 . B of the other rows not a number: the product takes zeros
+// for such values, and their part of the run's own rows is added behind it
+// (not_finite_part).
 #include <algorithm>
 #include <type_traits>
 #include "packed.hpp"
@@ -122,6 +125,9 @@ struct Stream {
     }
 };
 
+// The lane's number, from no register that would have to hold it.
+__device__ __forceinline__ int lane_id() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+
 // --- u = scale x A^T ---------------------------------------------------------
 
 #define DHX_SHRINK_PARAMS Addr starts_, Addr adapter_, Addr x_, Addr a_, Addr scale_, int sequences, int rows, int adapters, int inputs, int rank, Addr ids_, Addr u_, uint64_t x_stride
@@ -230,29 +236,60 @@ __global__ __launch_bounds__(64 * WAVES) void packed_shrink_kernel(DHX_SHRINK_PA
 
 // The runs of rows with one adapter among `n` rows from row0 on (n at most the
 // workgroup's threads): each row's run in run[] (-1: no adapter, -2: no
-// sequence), each run's adapter in list[]; returns their number. count: one int per wave.
+// sequence), each run's adapter in list[]; returns their number, and in `bare`
+// whether a row has no adapter. count: one int per wave.
 template <int THREADS>
-__device__ __forceinline__ int find_runs(const int32_t* ids, int row0, int n, int rows, int* run, int* list, int* count) {
+__device__ __forceinline__ int find_runs(const int32_t* ids, int row0, int n, int rows, int* run, int* list, int* count, bool& bare) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bool in = tid < n && row0 + tid < rows;
     const int mine = in ? ids[row0 + tid] : kNoSequence;
     const int before = in && tid > 0 ? ids[row0 + tid - 1] : kNoSequence;
     const bool first = mine >= 0 && mine != before;
     const uint64_t flags = __ballot(first);
-    if (lane == 0) count[wave] = __popcll(flags);
+    const int none = __any(mine == kNoAdapter) << 16;  // above the number of runs
+    if (lane == 0) count[wave] = __popcll(flags) + none;
     __syncthreads();
-    int at = __popcll(flags & (~0ull >> (63 - lane))) - 1, runs = 0;
+    int at = __popcll(flags & (~0ull >> (63 - lane))) - 1, all = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) {
-        if (w < wave) at += count[w];
-        runs += count[w];
+        if (w < wave) at += count[w] & 0xffff;
+        all += count[w];
     }
+    all = __builtin_amdgcn_readfirstlane(all);
+    bare = all >> 16 != 0;
     if (tid < n) {
         run[tid] = mine >= 0 ? at : mine;
         if (first) list[at] = mine;
     }
     __syncthreads();
-    return __builtin_amdgcn_readfirstlane(runs);
+    return all & 0xffff;
+}
+
+// The values of a row of B (`rank8` pieces of 8) that are not finite, times those
+// of u (piece i: u_at(i)): what a product leaves out that takes zeros for them.
+template <class T, class U>
+__device__ __forceinline__ float not_finite_part(const T* b, int rank8, U u_at) {
+    typedef typename Num<T>::v8 v8;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < rank8; ++i) {
+        const v8 vb = *(const v8*)(b + 8 * i);
+        if (!any_not_finite<T>(vb)) continue;
+        const v8 vu = u_at(i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = (float)vb[e];
+            if (!__builtin_isfinite(f)) sum = fmaf((float)vu[e], f, sum);
+        }
+    }
+    return sum;
+}
+template <class T>
+__device__ __forceinline__ typename Num<T>::v8 zeros_for_not_finite(typename Num<T>::v8 v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (!__builtin_isfinite((float)v[e])) v[e] = (T)0.f;
+    return v;
 }
 
 // Chunk c of LDS row r of a stage, 64 columns (128-byte rows, as in packed.hpp)
@@ -284,7 +321,6 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
     __shared__ int sRun[BM], sList[BM], sCount[WAVES];
     __shared__ __attribute__((aligned(16))) float sBias[BN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l32 = lane & 31, hi = lane >> 5;
     // Tiles in XCD-contiguous order, four row blocks at a time, so that the tiles
     // that an XCD has under way share rows of x and rows of W in its L2.
     const int n_tiles = (outputs + BN - 1) / BN, total = n_tiles * ((rows + BM - 1) / BM);
@@ -299,19 +335,24 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
 
     // Lane -> row lane / CH of a load's LR, the chunk that the swizzle puts at
     // slot lane % CH; rows behind the last one fetch that one.
-    const int lr = lane / CH;
     uint32_t xo[XL], wo[WL];
-    auto chunk = [&](int r) { return (lane % CH) ^ stage_slot<BK>(r); };
+    int frag;  // the element of a stage that the lane's first fragment begins at
+    auto place = [&](int lane) __attribute__((always_inline)) {
+        const int lr = lane / CH, l32 = lane & 31, hi = lane >> 5;
+        frag = l32 * BK + ((hi ^ stage_slot<BK>(l32)) << 3);
+        auto chunk = [&](int r) { return (lane % CH) ^ stage_slot<BK>(r); };
 #pragma unroll
-    for (int j = 0; j < XL; ++j) {
-        const int r = (wave * XL + j) * LR + lr;
-        xo[j] = (uint32_t)min(r, rows - 1 - row0) * (uint32_t)x_stride + chunk(r) * 8;
-    }
+        for (int j = 0; j < XL; ++j) {
+            const int r = (wave * XL + j) * LR + lr;
+            xo[j] = (uint32_t)min(r, rows - 1 - row0) * (uint32_t)x_stride + chunk(r) * 8;
+        }
 #pragma unroll
-    for (int j = 0; j < WL; ++j) {
-        const int r = (wave * WL + j) * LR + lr;
-        wo[j] = (uint32_t)min(r, outputs - 1 - col0) * (uint32_t)w_stride + chunk(r) * 8;
-    }
+        for (int j = 0; j < WL; ++j) {
+            const int r = (wave * WL + j) * LR + lr;
+            wo[j] = (uint32_t)min(r, outputs - 1 - col0) * (uint32_t)w_stride + chunk(r) * 8;
+        }
+    };
+    place(lane);
     auto move_whole = [&](T* sx, T* sw, int s) __attribute__((always_inline)) {
         const T *px = x0 + s * BK, *pw = w0 + s * BK;
 #pragma unroll
@@ -333,7 +374,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
         const T* zeros = (const T*)&kZeros;
         // What follows is taken anew in each of these few stages: held through the
         // whole ones it would cost them registers.
-        int lane = tid & 63;
+        int lane = lane_id();
         asm volatile("" : "+v"(lane));
         const int lr = lane / CH;
         auto chunk = [&](int r) { return (lane % CH) ^ stage_slot<BK>(r); };
@@ -370,7 +411,6 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
     };
 
     const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
-    const int frag = l32 * BK + ((hi ^ stage_slot<BK>(l32)) << 3);
     float16_t acc[MB][NB] = {};
     constexpr int SETS = PRE ? 2 * KK : 2;
     v8 fx[SETS][MB], fw[SETS][NB];
@@ -388,7 +428,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
     };
     move(sX0, sW0, 0);
     if (tid < BN) sBias[tid] = bias_.a && col0 + tid < outputs ? ((const float*)bias_)[col0 + tid] : 0.f;
-    runs = find_runs<THREADS>(ids_, row0, BM, rows, sRun, sList, sCount);
+    bool bare;
+    runs = find_runs<THREADS>(ids_, row0, BM, rows, sRun, sList, sCount, bare);
     const int steps = k_steps + (runs * rank8 + CH - 1) / CH;
     if (NST > 2 && steps > 1) move(sX1, sW1, 1);
     if (NST > 3 && steps > 2) move(sX2, sW2, 2);
@@ -447,26 +488,102 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
     while (s + 2 * NST <= whole) turn_of_stages(std::true_type{});
     while (s < steps) turn_of_stages(std::false_type{});
 
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        const int row = row0 + wm + i * 32 + l32;
-        const bool there = sRun[wm + i * 32 + l32] != kNoSequence;
-        T* py = (T*)y_ + (uint64_t)row * y_stride;
+    // Rows that a run's B does not belong to are multiplied by it, as zeros. A
+    // value of B that is not finite leaves none of its column's sums finite, those
+    // of its own rows (u times it) nor the others (0 times it), so some of the rows
+    // tell. Such a tile is computed once more, with zeros for those values. (us,
+    // without this check and with it: 12864 rows, 384 x 1152, 27.8 and 27.9; 7823
+    // rows, 1536 x 384, 25.2 and 25.3; 16384 rows, 4096 x 4096, 499 and 500; with a
+    // NaN in one of eight adapters the first takes 86. Checked in front of the
+    // stores, and with the pipelined walk run twice, it cost 0.5.)
+    const bool mixed = runs > 1 || (runs == 1 && bare);
+    if (mixed) {
+        float odd = 0.f;  // no number, if a sum is not finite
 #pragma unroll
         for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const int n = col0 + wn + k * 32 + kk * 16;
-                v4 o[2];
+            for (int r = 0; r < 16; ++r) odd = fmaf(acc[0][k][r], 0.f, odd);
+        const bool mine = __any(odd != 0.f);
+        if (lane_id() == 0) sCount[wave] = mine;
+    }
+    for (bool again = false;; again = true) {
+        // As in move: taken anew, not held through the walk.
+        int last = lane_id();
+        asm volatile("" : "+v"(last));
+        const int r32 = last & 31, half = last >> 5;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {  // columns n + 8q + 4hi .. +3
-                    const float4_t add = *(const float4_t*)(sBias + wn + k * 32 + kk * 16 + 8 * q + 4 * hi);
+        for (int i = 0; i < MB; ++i) {
+            const int row = row0 + wm + i * 32 + r32;
+            const bool there = sRun[wm + i * 32 + r32] != kNoSequence;
+            T* py = (T*)y_ + (uint64_t)row * y_stride;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[q][e] = (T)(acc[i][k][8 * kk + 4 * q + e] + add[e]);
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    const int n = col0 + wn + k * 32 + kk * 16;
+                    v4 o[2];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {  // columns n + 8q + 4hi .. +3
+                        const float4_t add = *(const float4_t*)(sBias + wn + k * 32 + kk * 16 + 8 * q + 4 * half);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[q][e] = (T)(acc[i][k][8 * kk + 4 * q + e] + add[e]);
+                    }
+                    const v8 piece = __builtin_bit_cast(v8, frag_swap(__builtin_bit_cast(half4_t, o[0]), __builtin_bit_cast(half4_t, o[1])));
+                    if (there && n + half * 8 < outputs) *(v8*)(py + n + half * 8) = piece;
                 }
-                const v8 piece = __builtin_bit_cast(v8, frag_swap(__builtin_bit_cast(half4_t, o[0]), __builtin_bit_cast(half4_t, o[1])));
-                if (there && n + hi * 8 < outputs) *(v8*)(py + n + hi * 8) = piece;
+        }
+        if (!mixed || again) return;
+        wait_lgkm();
+        barrier();  // behind the stores: they are on their way
+        int any = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) any |= sCount[w];
+        if (__builtin_expect(!__builtin_amdgcn_readfirstlane(any), 1)) return;
+        // The same products in the same order, a stage at a time.
+        place(last);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int k = 0; k < NB; ++k) acc[i][k] = float16_t{};
+#pragma unroll 1
+        for (int s = 0; s < steps; ++s) {
+            move(sX0, sW0, s);
+            wait_vm<0>();
+            barrier();
+            if (s >= k_steps) {
+#pragma unroll 1
+                for (int i = (wave * 64 + last) * 8; i < WS; i += THREADS * 8) *(v8*)(sW0 + i) = zeros_for_not_finite<T>(*(const v8*)(sW0 + i));
+                wait_lgkm();
+                barrier();
             }
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                load(sX0, sW0, kk, kk & 1);
+                multiply(kk & 1);
+            }
+            wait_lgkm();
+            barrier();  // read by every wave
+        }
+        // What the zeros left out of the run's own rows.
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int row = row0 + wm + i * 32 + r32, run = sRun[wm + i * 32 + r32];
+            if (run < 0) continue;
+            const T *u = (const T*)u_ + (uint64_t)row * rank, *b = (const T*)b_ + (uint64_t)sList[run] * outputs * rank;
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int col = col0 + wn + k * 32 + 8 * g4 + 4 * half;
+                    if (col >= outputs) continue;
+#pragma unroll 1
+                    for (int e = 0; e < 4; ++e) {
+                        const float part = not_finite_part<T>(b + (uint64_t)(col + e) * rank, rank8, [&](int at) { return *(const v8*)(u + 8 * at); });
+#pragma unroll
+                        for (int to = 0; to < 4; ++to) acc[i][k][4 * g4 + to] += to == e ? part : 0.f;
+                    }
+                }
+        }
     }
 }
 
@@ -482,7 +599,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void packed_linear_few_kernel(DHX_L
     constexpr int LDS = kFewWaves * S::STAGE;
     __shared__ __attribute__((aligned(16))) T s0[LDS], s1[LDS], s2[LDS], s3[NST > 3 ? LDS : 8];
     __shared__ float sum[kFewWaves][ROWS][20];
-    __shared__ int sRun[ROWS], sList[ROWS], sCount[kFewWaves];
+    __shared__ int sRun[ROWS], sList[ROWS], sCount[kFewWaves], sOdd;  // sOdd: some value of B is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, part = lane >> 4;
     const int col0 = blockIdx.x * 16, row0 = blockIdx.y * ROWS;
@@ -493,53 +610,68 @@ __global__ __launch_bounds__(64 * kFewWaves) void packed_linear_few_kernel(DHX_L
         [&](int r) { return (uint32_t)min(r, rows - 1 - row0) * (uint32_t)x_stride * 2; });
     float4_t acc[1][MB] = {};
     stream.run(s0 + wave * S::STAGE, s1 + wave * S::STAGE, s2 + wave * S::STAGE, s3 + (NST > 3 ? wave * S::STAGE : 0), inputs, acc);
-    const int runs = find_runs<64 * kFewWaves>(ids_, row0, ROWS, rows, sRun, sList, sCount), rank8 = rank >> 3;
+    if (tid == 0) sOdd = 0;
+    bool bare;
+    const int runs = find_runs<64 * kFewWaves>(ids_, row0, ROWS, rows, sRun, sList, sCount, bare), rank8 = rank >> 3;
     const T *u = (const T*)u_, *b = (const T*)b_;
+    auto u_at = [&](uint64_t at) {  // 8 values
+        if (parts == 1) return *(const v8*)(u + at);
+        float4_t v[kMostParts][2] = {};
+#pragma unroll
+        for (int z = 0; z < kMostParts; ++z) {
+            const float4_t* p = (const float4_t*)((const float*)u_ + (uint64_t)min(z, parts - 1) * rows * rank + at);
+            v[z][0] = p[0];
+            v[z][1] = p[1];
+        }
+        float4_t all[2] = {v[0][0], v[0][1]};
+#pragma unroll
+        for (int z = 1; z < kMostParts; ++z)
+            if (z < parts) {
+                all[0] += v[z][0];
+                all[1] += v[z][1];
+            }
+        v8 sum;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = (T)all[e / 4][e % 4];
+        return sum;
+    };
     for (int s = wave; s * 4 < runs * rank8; s += kFewWaves) {
         const int c = s * 4 + part, i = c / rank8, off = (c - i * rank8) * 8;
         const bool in = i < runs;
-        const v8 fb = in ? *(const v8*)(b + ((uint64_t)sList[i] * outputs + col) * rank + off) : v8{};
+        v8 fb = in ? *(const v8*)(b + ((uint64_t)sList[i] * outputs + col) * rank + off) : v8{};
+        v8 fu[MB];
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
             const int r = m * 16 + l16;
-            const uint64_t at = (uint64_t)(row0 + r) * rank + off;
-            v8 fu = {};
-            if (in && sRun[r] == i) {
-                if (parts == 1) {
-                    fu = *(const v8*)(u + at);
-                } else {
-                    float4_t v[kMostParts][2] = {};
-#pragma unroll
-                    for (int z = 0; z < kMostParts; ++z) {
-                        const float4_t* p = (const float4_t*)((const float*)u_ + (uint64_t)min(z, parts - 1) * rows * rank + at);
-                        v[z][0] = p[0];
-                        v[z][1] = p[1];
-                    }
-                    float4_t all[2] = {v[0][0], v[0][1]};
-#pragma unroll
-                    for (int z = 1; z < kMostParts; ++z)
-                        if (z < parts) {
-                            all[0] += v[z][0];
-                            all[1] += v[z][1];
-                        }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) fu[e] = (T)all[e / 4][e % 4];
-                }
-            }
-            acc[0][m] = Num<T>::mfma16(fb, fu, acc[0][m]);
+            fu[m] = in && sRun[r] == i ? u_at((uint64_t)(row0 + r) * rank + off) : v8{};
         }
+        if (__builtin_expect(__any(any_not_finite<T>(fb)), 0)) {  // behind the loads of u: they are on their way together
+            fb = zeros_for_not_finite<T>(fb);
+            sOdd = 1;
+        }
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[0][m] = Num<T>::mfma16(fb, fu[m], acc[0][m]);
     }
     // Lane: row 16 m + l16, columns 4 part .. +3.
 #pragma unroll
     for (int m = 0; m < MB; ++m) *(float4_t*)&sum[wave][m * 16 + l16][4 * part] = acc[0][m];
     __syncthreads();
-    const int r = tid >> 2, c = (tid & 3) * 4, row = row0 + r;
+    const int r = tid >> 2, c = (tid & 3) * 4, row = row0 + r, odd = sOdd;
     if (r >= ROWS || row >= rows || col0 + c >= outputs || sRun[r] == kNoSequence) return;
     float4_t v = {};
 #pragma unroll
     for (int w = 0; w < kFewWaves; ++w) v += *(const float4_t*)&sum[w][r][c];
     const float* bias = bias_;
     if (bias) v += *(const float4_t*)(bias + col0 + c);
+    if (__builtin_expect(odd, 0) && sRun[r] >= 0) {
+        const T* row_of_b = b + ((uint64_t)sList[sRun[r]] * outputs + col0 + c) * rank;
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+            const float part = not_finite_part<T>(row_of_b + e * rank, rank8, [&](int i) { return u_at((uint64_t)row * rank + 8 * i); });
+#pragma unroll
+            for (int to = 0; to < 4; ++to) v[to] += to == e ? part : 0.f;
+        }
+    }
     typename Num<T>::v4 o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = (T)v[e];

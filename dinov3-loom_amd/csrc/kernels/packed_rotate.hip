@@ -4,7 +4,7 @@
 // arithmetic to speak of, so the kernel is bound by memory: 16-byte pieces, a
 // piece of x1 and its partner of x2 per thread, or pieces of 8 bytes where
 // rotated is no multiple of 16 (the second half then begins between two 16-byte
-// pieces). The table rows are shared by a row's heads and by rows at the same
+// pieces; 12864 rows of 12 heads of 80: 40 rotated 11.4 us, 48 11.0). The table rows are shared by a row's heads and by rows at the same
 // place of other sequences, and come from the caches.
 #include <algorithm>
 #include <type_traits>

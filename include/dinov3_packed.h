@@ -54,8 +54,9 @@ enum { DHX_F16 = 0, DHX_BF16 = 1 };
  * for every row t of sequence s. An id outside 0 .. adapters-1 (-1, say) means
  * no adapter. The rank-sized product scale[a] a[a] x[t] is held in the type of
  * x between its two kernels (one rounding; a value past the type's range
- * becomes infinite there). Rows and adapters of any number, also a request per
- * row. */
+ * becomes infinite there). An adapter has no effect on rows of others, whatever
+ * it holds; a value of b that is not finite enters its own rows as its product
+ * with theirs. Rows and adapters of any number, also a request per row. */
 typedef struct dhx_packed_linear {
     uint32_t type; /* DHX_F16 or DHX_BF16: x, w, a, b, y */
     uint32_t sequences;

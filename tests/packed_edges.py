@@ -1,13 +1,15 @@
 """The operators on packed batches at edges of their definitions, against
-float64: rotations of heads' first channels where 16-byte pieces do not fit.
-Tolerances as in packed_operators.py."""
+float64: rotations of heads' first channels where 16-byte pieces do not fit;
+adapters that are not finite. Tolerances as in packed_operators.py."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import dinov3_hrx as d  # noqa: E402
 
-from packed_operators import F, TYPES, gen, normal, run_rotation, within  # noqa: E402
+from packed_operators import F, TYPES, gen, ints, normal, run_linear, run_rotation, starts_of, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +57,84 @@ def test_rotation_of_an_odd_number_of_eights(eng, t, neighbours, rows, heads, di
     assert torch.equal(got[..., rotated:], v[..., rotated:])
     rest = out[:, heads * dim:]
     assert torch.equal(rest, before[:, heads * dim:] if in_place else torch.full_like(rest, 7.0))
+
+
+# --- projection: an adapter that is not finite ---------------------------------
+
+# A launch on each route: few rows (one, two and four row blocks; columns in
+# parts), and each tile.
+B_ROUTES = [(12, 264, 136), (30, 264, 136), (60, 264, 136), (60, 2056, 136), (130, 1032, 264), (700, 136, 520), (2500, 136, 1928),
+            (2500, 136, 1304), (1500, 136, 1400), (8300, 136, 264), (8200, 136, 264), (3700, 136, 3848)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("kind", ["ragged", "single"])
+@pytest.mark.parametrize("rank", [8, 40])
+@pytest.mark.parametrize("rows,inputs,outputs", B_ROUTES)
+def test_an_adapter_that_is_not_finite_stays_with_its_rows(eng, t, kind, rank, rows, inputs, outputs):
+    # Infinities and NaN in B of two adapters: rows of other adapters and rows
+    # without one keep every bit; rows of the two are not finite in those columns,
+    # an infinity of the right sign where a single infinity meets a nonzero u, and
+    # keep every bit in the others.
+    dt = TYPES[t][1]
+    g = gen(rows + outputs + rank)
+    adapters = 5
+    if kind == "single":
+        st = list(range(rows + 1))
+    else:
+        st = [s for s in starts_of([(37 * i * i + 11) % 90 for i in range(rows)]) if s < rows - 1] + [rows - 1]  # the last row in none
+    ids = [(s * 5 + 2) % (adapters + 1) - 1 for s in range(len(st) - 1)]
+    x, w = normal(g, dt, rows, inputs), normal(g, dt, outputs, inputs, scale=inputs ** -0.5)
+    a, b = normal(g, dt, adapters, rank, inputs, scale=inputs ** -0.5), normal(g, dt, adapters, outputs, rank, scale=rank ** -0.5)
+    scale = torch.rand(adapters, generator=g, device="cuda") + 0.5
+    bias = torch.randn(outputs, generator=g, device="cuda")
+
+    def run(b):
+        y = torch.full((rows, outputs), 7.0, device="cuda").to(dt)
+        run_linear(eng, x, w, bias, a, b, scale, y, ints(st), ints(ids))
+        torch.cuda.synchronize()
+        return y
+
+    plain = run(b)
+    bad = b.clone()
+    # [adapter][column][rank column]; adapter 3's column 5 has both infinities.
+    places = {(1, 0, 1): math.inf, (1, outputs - 1, rank - 1): math.nan, (3, 5, 0): math.inf, (3, 5, 2): -math.inf, (3, 64, 7): -math.inf}
+    for at, value in places.items():
+        bad[at] = value
+    y = run(bad)
+    row_ids = torch.repeat_interleave(torch.tensor(ids), torch.tensor(st).diff()).cuda()
+    n = row_ids.numel()
+    hit = torch.zeros(rows, outputs, dtype=torch.bool, device="cuda")
+    for adapter, column, _ in places:
+        hit[:n, column] |= row_ids == adapter
+    assert hit.any() and torch.equal(y[~hit], plain[~hit])
+    assert not y[hit].isfinite().any()
+    # The sum of the infinities times u = scale a x, where u is far enough from
+    # zero to have its sign.
+    for adapter, column in {p[:2] for p in places}:
+        rows_of = (row_ids == adapter).nonzero()[:, 0]
+        u = x[rows_of].double() @ a[adapter].double().t().contiguous()
+        want = sum(u[:, r] * value for (i, c, r), value in places.items() if (i, c) == (adapter, column))
+        clear = (u.abs() > 1e-2).all(1)
+        assert torch.equal(y[rows_of, column][clear].double().nan_to_num(9.0), want[clear].nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [10, 300, 4000])
+def test_an_adapter_without_a_finite_value(eng, t, rows):
+    # All of B, and rows of one adapter alone in their tiles.
+    dt = TYPES[t][1]
+    g = gen(rows)
+    x, w = normal(g, dt, rows, 128), normal(g, dt, 256, 128)
+    a, b = normal(g, dt, 3, 16, 128), normal(g, dt, 3, 256, 16)
+    scale = torch.ones(3, device="cuda")
+    st, ids = [0, rows // 3, rows // 2, rows], [0, 1, 2]
+    ys = []
+    for b1 in (b[1], torch.full_like(b[1], math.nan)):
+        b[1] = b1
+        ys.append(torch.empty(rows, 256, dtype=dt, device="cuda"))
+        run_linear(eng, x, w, None, a, b, scale, ys[-1], ints(st), ints(ids))
+    torch.cuda.synchronize()
+    inside = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    inside[st[1]:st[2]] = True
+    assert torch.equal(ys[0][~inside], ys[1][~inside]) and ys[1][inside].isnan().all()
