@@ -285,7 +285,7 @@ __device__ __forceinline__ void store_row(const Row<T, D>& st, T* out, float* ls
     typedef typename Num<T>::v8 v8;
     const int token = r / group, h = r - token * group;
     const bool there = token < t.lq;
-    const float inv = st.l > 0.f ? 1.0f / st.l : 0.f;
+    const float inv = st.l != 0.f ? 1.0f / st.l : 0.f;  // a sum that is not a number stays one, also below
     T* p = out + (uint64_t)(t.q0 + token) * out_stride + h * out_head;
 #pragma unroll
     for (int ct = 0; ct < Geo<D>::CT; ++ct)
@@ -302,7 +302,7 @@ __device__ __forceinline__ void store_row(const Row<T, D>& st, T* out, float* ls
             if (there && ch < head_dim) *(v8*)(p + ch) = piece;
         }
     if (lse && there && hi == 0)
-        lse[(uint64_t)(t.q0 + token) * heads + head0 + h] = st.l > 0.f ? (st.m * c + __log2f(st.l)) * kLn2 : -__builtin_inff();
+        lse[(uint64_t)(t.q0 + token) * heads + head0 + h] = st.l != 0.f ? (st.m * c + __log2f(st.l)) * kLn2 : -__builtin_inff();
 }
 
 // A tile of 32 WAVES rows, 32 per wave; the waves of a group share blocks of 16

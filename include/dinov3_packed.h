@@ -111,9 +111,10 @@ int dhx_packed_rotation_run(dhx_engine *e, const dhx_packed_rotation *p, void *s
  * `causal`, query i of lq sees the keys j <= i + lk - lq (the last query sees
  * all of them, as for a prompt, its next part or one new token), else all. A
  * query that sees no key gets zeros, and -infinity in lse. Keys and values that
- * a query does not see have no effect on it, whatever they hold; a value that is
- * not finite makes its channel not finite (an infinity or not a number) for the
- * queries that see it. Products q . k lie above -1e30; a query whose products
+ * a query does not see have no effect on it, whatever they hold; a product q . k
+ * that is infinity or not a number makes the query's outputs and lse not a number,
+ * and a value that is not finite makes its channel not finite (an infinity or not
+ * a number) for the queries that see it. Products q . k lie above -1e30; a query whose products
  * are all below that counts as one that sees no key.
  * longest_q and longest_k, the rows of the longest sequence (0: not known),
  * only choose how the work is cut: a wrong number costs time, not results. */

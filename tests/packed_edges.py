@@ -1,6 +1,7 @@
 """The operators on packed batches at edges of their definitions, against
 float64: rotations of heads' first channels where 16-byte pieces do not fit;
-adapters that are not finite. Tolerances as in packed_operators.py."""
+adapters that are not finite; rows of attention that are not a number. Tolerances
+as in packed_operators.py."""
 import math
 
 import pytest
@@ -9,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 import dinov3_hrx as d  # noqa: E402
 
-from packed_operators import F, TYPES, gen, ints, normal, run_linear, run_rotation, starts_of, within  # noqa: E402
+from packed_operators import F, TYPES, gen, ints, normal, run_attention, run_linear, run_rotation, starts_of, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +139,35 @@ def test_an_adapter_without_a_finite_value(eng, t, rows):
     inside = torch.zeros(rows, dtype=torch.bool, device="cuda")
     inside[st[1]:st[2]] = True
     assert torch.equal(ys[0][~inside], ys[1][~inside]) and ys[1][inside].isnan().all()
+
+
+# --- attention: rows that are not a number -------------------------------------
+
+# The few-rows kernel with two waves, with four, and in parts of the keys; tiles
+# with several groups of waves and with one.
+NAN_ROUTES = [(1, 300, 4, 2), (4, 77, 4, 2), (300, 300, 4, 2), (2, 9000, 8, 2), (1500, 1500, 4, 2), (2500, 2500, 32, 16)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("product", [math.nan, math.inf])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("lq,lk,heads,kv", NAN_ROUTES)
+def test_log_sum_of_a_row_that_is_not_a_number(eng, t, product, dim, lq, lk, heads, kv):
+    # A product that is infinity or not a number, with a key that the last query
+    # alone sees: its outputs and its log-sums are not numbers on every route; the
+    # other rows keep every bit.
+    dt = TYPES[t][1]
+    g = gen(dim + lq)
+    q, k, v = normal(g, dt, lq, heads, dim), normal(g, dt, lk, kv, dim), normal(g, dt, lk, kv, dim)
+    q[..., 0] = 1
+    outs, sums = [], []
+    for _ in range(2):
+        outs.append(torch.empty(lq, heads, dim, dtype=dt, device="cuda"))
+        sums.append(torch.zeros(lq, heads, device="cuda"))
+        run_attention(eng, q, k, v, outs[-1], ints([0, lq]), ints([0, lk]), 1, dim ** -0.5, sums[-1], hints=(lq, lk))
+        torch.cuda.synchronize()
+        k[lk - 1] = 0
+        k[lk - 1, :, 0] = product
+    assert outs[0].isfinite().all() and sums[0].isfinite().all()
+    assert torch.equal(outs[0][:-1], outs[1][:-1]) and torch.equal(sums[0][:-1], sums[1][:-1])
+    assert outs[1][-1].isnan().all() and sums[1][-1].isnan().all()
