@@ -462,7 +462,11 @@ __global__ __launch_bounds__(64 * NW, 1) void packed_attention_few_kernel(DHX_PA
     const int l32 = lane & 31, hi = lane >> 5;
     const int head0 = at.head * group, heads = group * kv_heads;
     Item it;
-    for (uint32_t item = at.item;; item += slots) {
+    // Starts that decrease may make any number of items, more than 32 bits count;
+    // none beyond what these rows and sequences can have otherwise is taken.
+    const uint32_t all_rows_of_group = (uint32_t)q_rows * (uint32_t)group;
+    const uint32_t most = min(all_rows_of_group / 32 + (uint32_t)sequences, all_rows_of_group) * (uint32_t)splits;
+    for (uint32_t item = at.item; item < most; item += slots) {
     if (!find_item(it, item, q_starts_, k_starts_, sequences, group, q_rows, k_rows, splits, span)) return;
     const Tile& t = it.t;
 

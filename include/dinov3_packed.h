@@ -8,8 +8,8 @@
  * int32 in device memory: sequence s has the rows starts[s] .. starts[s+1]-1,
  * none if the two are equal. The array must not decrease; it is read by the
  * kernels only, so it may change between the replays of a captured graph.
- * Whatever it holds, no kernel reads or writes outside 0 .. rows-1 (a value
- * outside is taken as the nearest end). Rows in front of starts[0] and from
+ * Whatever it holds, every call ends and no kernel reads or writes outside 0 ..
+ * rows-1 (a value outside is taken as the nearest end). Rows in front of starts[0] and from
  * starts[sequences] on belong to no sequence: their outputs are left as they
  * were.
  *

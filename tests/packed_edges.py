@@ -171,3 +171,20 @@ def test_log_sum_of_a_row_that_is_not_a_number(eng, t, product, dim, lq, lk, hea
     assert outs[0].isfinite().all() and sums[0].isfinite().all()
     assert torch.equal(outs[0][:-1], outs[1][:-1]) and torch.equal(sums[0][:-1], sums[1][:-1])
     assert outs[1][-1].isnan().all() and sums[1][-1].isnan().all()
+
+
+# --- attention: starts that decrease -------------------------------------------
+
+def test_starts_that_decrease_end(eng):
+    # 2^15 sequences of 2^22 rows each in an array of 2^22 rows: 2^32 tiles of 32
+    # rows, where sequences in order have 2^17 + 2^16 at most. The call ends, and
+    # writes nothing outside the rows.
+    rows, sequences, dim = 1 << 22, 1 << 16, 8
+    g = gen(1)
+    q = normal(g, torch.float16, rows, 1, dim)
+    k, v = normal(g, torch.float16, 64, 1, dim), normal(g, torch.float16, 64, 1, dim)
+    guard = torch.full((rows + 200, 1, dim), 7.0, dtype=torch.float16, device="cuda")
+    turns = torch.arange(sequences + 1, device="cuda") % 2
+    run_attention(eng, q, k, v, guard[100:100 + rows], (turns * rows).int(), (turns * 64).int(), 0, dim ** -0.5, hints=(1, 64))
+    torch.cuda.synchronize()
+    assert (guard[:100] == 7.0).all() and (guard[100 + rows:] == 7.0).all()
