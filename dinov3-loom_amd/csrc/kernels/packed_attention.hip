@@ -575,9 +575,10 @@ __global__ __launch_bounds__(64 * NW, 1) void packed_attention_few_kernel(DHX_PA
 
 #define DHX_JOIN_PARAMS Addr part_, Addr q_starts_, Addr out_, Addr lse_, int sequences, int q_rows, int heads, int head_dim, int splits, float c, uint64_t out_stride, uint64_t out_head
 
-// One wave per row and head: the splits' parts, weighted by 2^(c (m - max m)).
-// The splits that saw keys of a row are the first ones. Groups of lanes take a
-// split each, four floats per lane, eight loads on their way.
+// One wave per row and head: the splits' parts, weighted by 2^(c (m - max m)). A
+// split without a sum (its keys are not seen, or weigh nothing) has stored no O.
+// Groups of lanes take a split each, four floats per lane, eight loads on their
+// way.
 template <class T, int D>
 __global__ __launch_bounds__(kThreads) void packed_join_kernel(DHX_JOIN_PARAMS) {
     constexpr int LANES = D > 64 ? 32 : D / 4, SIDE = 64 / LANES, DEEP = 8;
@@ -596,14 +597,15 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(DHX_JOIN_PARAMS) 
         float4_t o = {};
         for (int s0 = 0; s0 < splits; s0 += 64) {
             const float2_t at = s0 + lane < splits ? ml[(s0 + lane) * all] : float2_t{kNoMax, 0.f};
-            const int n = __popcll(__ballot(at[1] != 0.f));  // also one that is not a number
-            if (n == 0) break;
+            const uint64_t some = __ballot(at[1] != 0.f);  // also one that is not a number
+            if (some == 0) continue;
+            const int first = __builtin_ctzll(some), n = 64 - __builtin_clzll(some);
             float top = fmaxf(m, at[0]);
 #pragma unroll
             for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-            const float w = lane < n ? fast_exp2((at[0] - top) * c) : 0.f, before = fast_exp2((m - top) * c);
+            const float w = some >> lane & 1 ? fast_exp2((at[0] - top) * c) : 0.f, before = fast_exp2((m - top) * c);
             m = top;
-            l = l * before + w * (lane < n ? at[1] : 0.f);
+            l = l * before + w * at[1];
             o *= before;
             for (int j0 = 0; j0 < n; j0 += SIDE * DEEP) {
                 float4_t p[DEEP];
@@ -611,9 +613,10 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(DHX_JOIN_PARAMS) 
 #pragma unroll
                 for (int d = 0; d < DEEP; ++d) {
                     const int j = j0 + d * SIDE + lane / LANES;
-                    p[d] = *(const float4_t*)(mine + (uint64_t)(s0 + min(j, n - 1)) * all * D);
-                    const float wj = __shfl(w, min(j, n - 1));
-                    pw[d] = j < n ? wj : 0.f;
+                    const int from = j < n && (some >> j & 1) ? j : first;
+                    p[d] = *(const float4_t*)(mine + (uint64_t)(s0 + from) * all * D);
+                    const float wj = __shfl(w, from);
+                    pw[d] = from == j ? wj : 0.f;
                 }
 #pragma unroll
                 for (int d = 0; d < DEEP; ++d) o += pw[d] * p[d];

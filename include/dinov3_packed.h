@@ -114,8 +114,9 @@ int dhx_packed_rotation_run(dhx_engine *e, const dhx_packed_rotation *p, void *s
  * a query does not see have no effect on it, whatever they hold; a product q . k
  * that is infinity or not a number makes the query's outputs and lse not a number,
  * and a value that is not finite makes its channel not finite (an infinity or not
- * a number) for the queries that see it. Products q . k lie above -1e30; a query whose products
- * are all below that counts as one that sees no key.
+ * a number) for the queries that see it. A key whose product q . k lies below
+ * -1e30 weighs nothing (its value should be finite); a query whose products all
+ * do counts as one that sees no key.
  * longest_q and longest_k, the rows of the longest sequence (0: not known),
  * only choose how the work is cut: a wrong number costs time, not results. */
 typedef struct dhx_packed_attention {

@@ -1,7 +1,7 @@
 """The operators on packed batches at edges of their definitions, against
 float64: rotations of heads' first channels where 16-byte pieces do not fit;
-adapters that are not finite; rows of attention that are not a number. Tolerances
-as in packed_operators.py."""
+adapters that are not finite; rows of attention that are not a number, keys that
+weigh nothing, starts that decrease. Tolerances as in packed_operators.py."""
 import math
 
 import pytest
@@ -10,7 +10,8 @@ torch = pytest.importorskip("torch")
 
 import dinov3_hrx as d  # noqa: E402
 
-from packed_operators import F, TYPES, gen, ints, normal, run_attention, run_linear, run_rotation, starts_of, within  # noqa: E402
+from packed_operators import (F, TYPES, attention_want, gen, ints, normal, run_attention, run_linear, run_rotation,  # noqa: E402
+                              starts_of, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -171,6 +172,32 @@ def test_log_sum_of_a_row_that_is_not_a_number(eng, t, product, dim, lq, lk, hea
     assert outs[0].isfinite().all() and sums[0].isfinite().all()
     assert torch.equal(outs[0][:-1], outs[1][:-1]) and torch.equal(sums[0][:-1], sums[1][:-1])
     assert outs[1][-1].isnan().all() and sums[1][-1].isnan().all()
+
+
+# --- attention: keys of no weight ----------------------------------------------
+
+@pytest.mark.parametrize("t,product", [("f16", -math.inf), ("bf16", -math.inf), ("bf16", -3e30)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lq,lk,heads,kv", [(1, 9000, 8, 2), (8, 5000, 4, 4), (1, 300, 4, 2), (300, 900, 4, 2), (1500, 1500, 4, 2)])
+@pytest.mark.parametrize("where", ["front", "middle", "back"])
+def test_keys_of_no_weight(eng, t, product, dim, lq, lk, heads, kv, where):
+    # Products below -1e30 over whole parts of the keys: the result is that of
+    # the other keys, whichever part they lie in.
+    dt = TYPES[t][1]
+    g = gen(dim + lq)
+    q, k, v = normal(g, dt, lq, heads, dim), normal(g, dt, lk, kv, dim), normal(g, dt, lk, kv, dim)
+    q[..., 0] = 1
+    at = {"front": slice(0, lk // 3), "middle": slice(lk // 4, lk * 3 // 4), "back": slice(lk // 2, lk)}[where]
+    kept = torch.ones(lk, dtype=torch.bool, device="cuda")
+    kept[at] = False
+    want, room, want_lse, lse_room = attention_want(q, k[kept], v[kept], 0, dim ** -0.5)
+    k[at] = 0
+    k[at, :, 0] = product
+    out, lse = torch.empty_like(q), torch.zeros(lq, heads, device="cuda")
+    run_attention(eng, q, k, v, out, ints([0, lq]), ints([0, lk]), 0, dim ** -0.5, lse, hints=(lq, lk))
+    torch.cuda.synchronize()
+    within(out, want, room, dt)
+    assert ((lse.double() - want_lse).abs() <= lse_room).all()
 
 
 # --- attention: starts that decrease -------------------------------------------
