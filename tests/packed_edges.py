@@ -1,7 +1,7 @@
 """The operators on packed batches at edges of their definitions, against
 float64: rotations of heads' first channels where 16-byte pieces do not fit;
 adapters that are not finite; rows of attention that are not a number, keys that
-weigh nothing, starts that decrease. Tolerances as in packed_operators.py."""
+weigh nothing, starts that decrease, many sequences. Tolerances as in packed_operators.py."""
 import math
 
 import pytest
@@ -10,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 import dinov3_hrx as d  # noqa: E402
 
-from packed_operators import (F, TYPES, attention_want, gen, ints, normal, run_attention, run_linear, run_rotation,  # noqa: E402
+from packed_operators import (F, TYPES, attention_want, gen, half_step, ints, normal, run_attention, run_linear, run_rotation,  # noqa: E402
                               starts_of, within)
 
 pytestmark = pytest.mark.gpu
@@ -215,3 +215,48 @@ def test_starts_that_decrease_end(eng):
     run_attention(eng, q, k, v, guard[100:100 + rows], (turns * rows).int(), (turns * 64).int(), 0, dim ** -0.5, hints=(1, 64))
     torch.cuda.synchronize()
     assert (guard[:100] == 7.0).all() and (guard[100 + rows:] == 7.0).all()
+
+
+# --- attention: many sequences -------------------------------------------------
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (1, 1, 128)])
+@pytest.mark.parametrize("sequences", [64, 65, 2100, 9000])
+def test_more_sequences_than_workgroups(eng, t, heads, kv, dim, sequences):
+    # Single tokens (some sequences without one) with 0 to 6 keys each, then one
+    # with many: a workgroup's items lie in windows of 64 sequences far apart.
+    dt = TYPES[t][1]
+    g = gen(sequences)
+    ql = [1 if s % 5 else 0 for s in range(sequences - 1)] + [3]
+    kl = [s * s % 7 for s in range(sequences - 1)] + [700]
+    qs, ks = starts_of(ql), starts_of(kl)
+    q, k, v = normal(g, dt, qs[-1], heads, dim), normal(g, dt, ks[-1], kv, dim), normal(g, dt, ks[-1], kv, dim)
+    out, lse = torch.full_like(q, 7.0), torch.full((qs[-1], heads), 7.0, device="cuda")
+    run_attention(eng, q, k, v, out, ints(qs), ints(ks), 1, dim ** -0.5, lse, hints=(3, 700))
+    torch.cuda.synchronize()
+    # Sequences of one query, all at once: each query's keys padded to 6.
+    one = torch.tensor([s for s in range(sequences - 1) if ql[s]], device="cuda")
+    at = torch.tensor(ks, device="cuda")[one][:, None] + torch.arange(6, device="cuda")
+    there = torch.arange(6, device="cuda") < torch.tensor(kl, device="cuda")[one][:, None]
+    at = at.clamp_max(ks[-1] - 1)
+    q64 = q[:one.numel()].double().view(one.numel(), kv, heads // kv, dim)
+    k64, v64 = k[at].double(), v[at].double()  # [query][6][kv][dim]
+    s = (q64[:, None] * k64[:, :, :, None]).sum(-1) * dim ** -0.5  # [query][6][kv][group]
+    size = (q64[:, None] * k64[:, :, :, None]).abs().sum(-1) * dim ** -0.5
+    s = s.masked_fill(~there[:, :, None, None], -math.inf)
+    top = s.amax(1, keepdim=True).clamp_min(-1e300)
+    w = torch.exp(s - top)
+    total = w.sum(1).clamp_min(1e-300)[..., None]
+    want = (w[..., None] * v64[:, :, :, None]).sum(1) / total
+    mean = (w[..., None] * v64[:, :, :, None].abs()).sum(1) / total
+    # As attention_want: a score's error, P's rounding, the sums of 6.
+    off = ((dim + 1) * F * size + 4 * F * (s.abs() + s.abs().nan_to_num(0, 0, 0).amax(1, keepdim=True))).masked_fill(~there[:, :, None, None], 0)
+    rel = 2 * torch.expm1(off.amax(1)) + half_step(dt) + 28 * F
+    floor = F * (v64.abs() * there[:, :, None, None]).sum(1)[:, :, None] / total
+    within(out[:one.numel()], want.flatten(1, 2), (rel[..., None] * mean + floor).flatten(1, 2), dt)
+    empty = ~there.any(1)
+    assert empty.any() and (out[:one.numel()][empty] == 0).all() and (lse[:one.numel()][empty] == -math.inf).all()
+    assert lse[:one.numel()][~empty].isfinite().all()
+    want, room, want_lse, lse_room = attention_want(q[-3:], k[-700:], v[-700:], 1, dim ** -0.5)
+    within(out[-3:], want, room, dt)
+    assert ((lse[-3:].double() - want_lse).abs() <= lse_room).all()
