@@ -314,6 +314,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
     constexpr int XL = BM / LR / WAVES, WL = BN / LR / WAVES;
     constexpr int MB = WM / 32, NB = WN / 32, KK = BK / 16;
     static_assert(!PRE || NST % 2 == 0, "the fragments' sets take turns with the stages");
+    static_assert(NB <= 2, "a lane's columns of 32 rows are the bits of a word");
     static_assert(XL * LR * WAVES == BM && WL * LR * WAVES == BN && BM <= THREADS && BN <= THREADS, "whole loads");
     constexpr int XS = BM * BK, WS = BN * BK;
     __shared__ __attribute__((aligned(16))) T sX0[XS], sX1[XS], sX2[NST > 2 ? XS : 8], sX3[NST > 3 ? XS : 8];
@@ -491,11 +492,13 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
     // Rows that a run's B does not belong to are multiplied by it, as zeros. A
     // value of B that is not finite leaves none of its column's sums finite, those
     // of its own rows (u times it) nor the others (0 times it), so some of the rows
-    // tell. Such a tile is computed once more, with zeros for those values. (us,
-    // without this check and with it: 12864 rows, 384 x 1152, 27.8 and 27.9; 7823
-    // rows, 1536 x 384, 25.2 and 25.3; 16384 rows, 4096 x 4096, 499 and 500; with a
-    // NaN in one of eight adapters the first takes 86. Checked in front of the
-    // stores, and with the pipelined walk run twice, it cost 0.5.)
+    // tell, and all of them where they are not finite (rows of x may not be). Such
+    // a tile is computed once more, with zeros for those values. (us, without this
+    // check and with it: 12864 rows, 384 x 1152, 28.3 and 28.4; 7823 rows, 1536 x
+    // 384, 25.6 and 25.75; 16384 rows, 4096 x 4096, 502 and 502; with a NaN in one of
+    // eight adapters the first takes 87, with all of every eighth request's x NaN as
+    // long as without. Checked in front of the stores it cost 0.5, and the pipelined
+    // walk run twice registers.)
     const bool mixed = runs > 1 || (runs == 1 && bare);
     if (mixed) {
         float odd = 0.f;  // no number, if a sum is not finite
@@ -503,7 +506,22 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
         for (int k = 0; k < NB; ++k)
 #pragma unroll
             for (int r = 0; r < 16; ++r) odd = fmaf(acc[0][k][r], 0.f, odd);
-        const bool mine = __any(odd != 0.f);
+        bool mine = __any(odd != 0.f);
+        if (__builtin_expect(mine, 0)) {  // a column without a finite sum?
+            uint32_t none = ~0u;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                uint32_t here = 0;
+#pragma unroll
+                for (int k = 0; k < NB; ++k)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) here |= (uint32_t)!__builtin_isfinite(acc[i][k][r]) << (16 * k + r);
+                none &= here;
+            }
+#pragma unroll
+            for (int i = 16; i; i >>= 1) none &= __shfl_xor(none, i);
+            mine = __any(none != 0);
+        }
         if (lane_id() == 0) sCount[wave] = mine;
     }
     for (bool again = false;; again = true) {
@@ -537,7 +555,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_l
         barrier();  // behind the stores: they are on their way
         int any = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) any |= sCount[w];
+        for (int n = 0; n < BN / WN; ++n) {  // in all rows of its columns
+            int all = 1;
+#pragma unroll
+            for (int m = 0; m < BM / WM; ++m) all &= sCount[m * (BN / WN) + n];
+            any |= all;
+        }
         if (__builtin_expect(!__builtin_amdgcn_readfirstlane(any), 1)) return;
         // The same products in the same order, a stage at a time.
         place(last);

@@ -10,8 +10,8 @@ torch = pytest.importorskip("torch")
 
 import dinov3_hrx as d  # noqa: E402
 
-from packed_operators import (F, TYPES, attention_want, gen, half_step, ints, normal, run_attention, run_linear, run_rotation,  # noqa: E402
-                              starts_of, within)
+from packed_operators import (F, TYPES, attention_want, gen, half_step, ints, linear_want, normal, run_attention,  # noqa: E402
+                              run_linear, run_rotation, starts_of, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -140,6 +140,60 @@ def test_an_adapter_without_a_finite_value(eng, t, rows):
     inside = torch.zeros(rows, dtype=torch.bool, device="cuda")
     inside[st[1]:st[2]] = True
     assert torch.equal(ys[0][~inside], ys[1][~inside]) and ys[1][inside].isnan().all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("odd", [1, 100])
+@pytest.mark.parametrize("bad", [False, True])
+@pytest.mark.parametrize("rows,inputs,outputs", [r for r in B_ROUTES if r[0] > 100])
+def test_rows_that_are_not_finite_beside_an_adapter_that_is_not(eng, t, odd, bad, rows, inputs, outputs):
+    # Rows of x that are not a number (a few, or whole blocks of the tile), with
+    # and without such values in B: the other rows keep every bit.
+    dt = TYPES[t][1]
+    g = gen(rows + outputs + odd)
+    x, w = normal(g, dt, rows, inputs), normal(g, dt, outputs, inputs, scale=inputs ** -0.5)
+    a, b = normal(g, dt, 3, 16, inputs, scale=inputs ** -0.5), normal(g, dt, 3, outputs, 16, scale=0.25)
+    scale = torch.ones(3, device="cuda")
+    st, ids = list(range(0, rows, 10)) + [rows], [s % 3 for s in range((rows + 9) // 10)]
+    row_ids = torch.repeat_interleave(torch.tensor(ids), torch.tensor(st).diff()).cuda()
+    ys = []
+    for _ in range(2):
+        ys.append(torch.empty(rows, outputs, dtype=dt, device="cuda"))
+        run_linear(eng, x, w, None, a, b, scale, ys[-1], ints(st), ints(ids))
+        torch.cuda.synchronize()
+        x[20:20 + odd] = math.nan
+        if bad:
+            b[1, 9, 3] = math.nan
+    hit = torch.zeros(rows, outputs, dtype=torch.bool, device="cuda")
+    hit[20:20 + odd] = True
+    if bad:
+        hit[:, 9] |= row_ids == 1
+    assert torch.equal(ys[0][~hit], ys[1][~hit]) and ys[1][hit].isnan().all()
+
+
+# --- projection: sequences without rows ----------------------------------------
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [40, 300, 2500])
+def test_linear_with_many_sequences_without_rows(eng, t, rows):
+    # Up to 199 empty sequences between two that are not: a tile's rows belong to
+    # sequences further apart than the 64 that a wave looks at together.
+    dt = TYPES[t][1]
+    g = gen(rows)
+    lengths, left = [], rows
+    while left:
+        lengths += [0] * (len(lengths) * 7 % 200) + [min(left, 1 + len(lengths) % 9)]
+        left -= lengths[-1]
+    st, adapters = starts_of(lengths), 5
+    ids = [(s * 5 + 2) % (adapters + 1) - 1 for s in range(len(lengths))]
+    x, w = normal(g, dt, rows, 136), normal(g, dt, 200, 136, scale=136 ** -0.5)
+    a, b = normal(g, dt, adapters, 8, 136, scale=136 ** -0.5), normal(g, dt, adapters, 200, 8, scale=8 ** -0.5)
+    scale = torch.rand(adapters, generator=g, device="cuda") + 0.5
+    y = torch.full((rows, 200), 7.0, device="cuda").to(dt)
+    run_linear(eng, x, w, None, a, b, scale, y, ints(st), ints(ids))
+    torch.cuda.synchronize()
+    want, bound = linear_want(x, w, None, a, b, scale, [(st[s], st[s + 1], i) for s, i in enumerate(ids)])
+    within(y, want, bound, dt)
 
 
 # --- attention: rows that are not a number -------------------------------------
