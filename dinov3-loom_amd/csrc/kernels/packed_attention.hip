@@ -699,7 +699,7 @@ hipError_t launch_type(const dhx_packed_attention& p, const AttentionCut& cut, h
 // How a launch is cut (times in us on MI355X; causal where heads are grouped).
 //
 // Few-rows kernel: sequences of at most 32 rows have no use for taller tiles:
-// single tokens of 48 requests with 32 heads of 128 on 8, 118k keys together, 94
+// single tokens of 48 requests with 32 heads of 128 on 8, 116.6k keys together, 94
 // against 657. And launches of few tiles (in tiles of 64 rows) leave CUs idle
 // that parts of the keys fill. Against the best of the others, heads of 64: 1029
 // rows and keys of 6 heads 12.2 and 16.0 (102 tiles), five images of 201 tokens

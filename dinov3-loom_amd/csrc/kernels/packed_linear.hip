@@ -739,8 +739,8 @@ hipError_t launch(const dhx_packed_linear& p, hipStream_t s) {
     // enough for the 256 CUs: 16384 rows, 4096 x 4096, 498 with 256 x 256 (128 x
     // 128 597), 4096 rows 130 (152; 256 tiles); 12864 rows, 384 x 1152, 29 (31; 255
     // tiles), 8192 rows, 1024 x 1024, 38 (30; 128 tiles); 1024 rows, 4096 x 4096,
-    // 128 x 128 53.5 (256 tiles), 128 x 64 52.1 (512); 7416 rows, 1536 x 384, 28.7
-    // (174), 27.5 (348), 64 x 64 27.2 (696); 256 rows, 4096 x 4096, 64 x 64 in four
+    // 128 x 128 53.5 (256 tiles), 128 x 64 52.1 (512); 7823 rows, 1536 x 384, 29.1
+    // (186), 28.9 (372), 64 x 64 28.1 (738); 256 rows, 4096 x 4096, 64 x 64 in four
     // stages 31 (256 tiles), in two 43.
     if (p.rows <= 16) return few<T, 1>(p, ids, u, w.parts, s);
     if (p.rows <= 32) return few<T, 2>(p, ids, u, w.parts, s);

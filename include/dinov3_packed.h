@@ -30,7 +30,8 @@
  * elements); rows, strides and addresses are multiples of 16 bytes, so sizes
  * along a row are multiples of 8 elements. Outputs must not overlap inputs,
  * but where said. Sums, softmax statistics and angles are float32; an output
- * is rounded once, to the nearest value of its type.
+ * is rounded once, to the nearest value of its type, and so is what stands
+ * between two products (the adapters' a x, the weights of attention), as said.
  *
  * A workspace belongs to the caller: 16-byte aligned device memory of at least
  * the bytes that the workspace function returns for the same sizes and hints.
@@ -117,6 +118,9 @@ int dhx_packed_rotation_run(dhx_engine *e, const dhx_packed_rotation *p, void *s
  * a number) for the queries that see it. A key whose product q . k lies below
  * -1e30 weighs nothing (its value should be finite); a query whose products all
  * do counts as one that sees no key.
+ * The weights are rounded to the type of v for their product with it (f16 loses
+ * those under 2^-25 of a row's largest); their sum keeps float32. Products, and
+ * scale times them, are float32 too.
  * longest_q and longest_k, the rows of the longest sequence (0: not known),
  * only choose how the work is cut: a wrong number costs time, not results. */
 typedef struct dhx_packed_attention {
