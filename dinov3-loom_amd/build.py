@@ -30,7 +30,11 @@ SOURCES = [
     "kernels/attention.hip",
     "kernels/norm.hip",
     "kernels/packed_attention.hip",
+    "kernels/packed_gated.hip",
     "kernels/packed_linear.hip",
+    "kernels/packed_norm.hip",
+    "kernels/packed_quantise.hip",
+    "kernels/packed_quantised.hip",
     "kernels/packed_rotate.hip",
     "engine.cpp",
     "model.cpp",

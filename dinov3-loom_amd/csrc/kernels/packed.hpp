@@ -57,6 +57,23 @@ hipError_t launch_packed_linear(const dhx_packed_linear& p, hipStream_t s);
 
 hipError_t launch_packed_rotation(const dhx_packed_rotation& p, hipStream_t s);
 
+hipError_t launch_packed_norm(const dhx_packed_norm& p, hipStream_t s);
+
+hipError_t launch_packed_quantise(const dhx_packed_quantisation& p, hipStream_t s);
+hipError_t launch_packed_dequantise(const dhx_packed_quantisation& p, hipStream_t s);
+
+uint64_t packed_quantised_linear_bytes(const dhx_packed_quantised_linear& p);
+hipError_t launch_packed_quantised_linear(const dhx_packed_quantised_linear& p, hipStream_t s);
+
+uint64_t packed_gated_bytes(const dhx_packed_gated& p);
+hipError_t launch_packed_gated(const dhx_packed_gated& p, hipStream_t s);
+
+// 4-bit rows: a block of 32 values has 16 bytes of codes and a scale byte; a row of
+// scales is read 16 bytes at a time.
+constexpr uint64_t blocks_of(uint64_t columns) { return (columns + 31) / 32; }
+constexpr uint64_t code_bytes(uint64_t columns) { return blocks_of(columns) * 16; }
+constexpr uint64_t scale_bytes(uint64_t columns) { return (blocks_of(columns) + 15) / 16 * 16; }
+
 // --- device pieces ---------------------------------------------------------
 
 // 16 bytes of zeros in global memory: what a lane of a DMA load fetches for a

@@ -1,0 +1,229 @@
+// The residual step behind a block of a packed batch, with the norms before and
+// behind it (include/dinov3_packed.h): x' = x + gate[s] scale post(y), h =
+// pre(x'). Each row of x and y is read once and held in registers through both
+// norms, x' and h are written once, and there is little arithmetic, so the kernel
+// is bound by memory (few rows: by one row's chain of loads, sums and stores).
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "packed.hpp"
+
+namespace dhx {
+namespace {
+
+#define DHX_NORM_PARAMS Addr x_, Addr y_, Addr x_out_, Addr h_, int rows, int channels, uint64_t x_stride, uint64_t y_stride, Addr starts_, Addr scale_, Addr gate_, Addr post_weight_, Addr post_bias_, Addr pre_weight_, Addr pre_bias_, uint64_t x_out_stride, uint64_t h_stride, uint64_t gate_stride, int sequences, int post, int pre, float post_eps, float pre_eps
+
+// The sum of v over the G lanes (G <= 64: of a wave, else of the workgroup) that
+// hold a row, in all of them, by the same tree in each: inside rows of 16 lanes by
+// moves between lanes, then across them. part: a float per wave.
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+    auto move = [](float a, auto ctrl) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, a), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    v += move(v, std::integral_constant<int, 0xb1>{});   // quad_perm 1, 0, 3, 2
+    v += move(v, std::integral_constant<int, 0x4e>{});   // quad_perm 2, 3, 0, 1
+    v += move(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+    v += move(v, std::integral_constant<int, 0x140>{});  // row_mirror
+    if constexpr (G >= 64) {
+        v += __shfl_xor(v, 16);
+        v = half_pair_sum(v);
+    }
+    if constexpr (G > 64) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        if (lane == 0) part[wave] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < G / 64; ++w) v += part[w];
+    }
+    return v;
+}
+
+// The last sequence that does not begin behind row0 + mine, one of the ROWS rows
+// from row0 on that a wave holds; -1: none.
+template <int ROWS>
+__device__ __forceinline__ int sequence_of(const int32_t* starts, int sequences, int rows, int row0, int mine) {
+    int at = -1;
+    if (sequences <= 64) {
+        const int lane = threadIdx.x & 63, first = lane < sequences ? start_at(starts, lane, rows) : INT_MAX;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int n = __builtin_popcountll(__ballot(first <= row0 + r));
+            if (mine == r) at = n - 1;
+        }
+    } else {
+        for (int r = 0; r < ROWS; ++r) {
+            const int last = wave_last(sequences, row0 + r, [&](int s) { return (int64_t)start_at(starts, s, rows); });
+            if (mine == r) at = last;
+        }
+    }
+    return at;
+}
+
+template <class S>
+__device__ __forceinline__ void load8(const S* p, float (&v)[8]) {
+    if constexpr (std::is_same_v<S, float>) {
+        const float4_t a = *(const float4_t*)p, b = *(const float4_t*)(p + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < 4 ? a[e] : b[e - 4];
+    } else {
+        const typename Num<S>::v8 a = *(const typename Num<S>::v8*)p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)a[e];
+    }
+}
+template <class S>
+__device__ __forceinline__ void store8(S* p, const float (&v)[8]) {
+    if constexpr (std::is_same_v<S, float>) {
+        *(float4_t*)p = float4_t{v[0], v[1], v[2], v[3]};
+        *(float4_t*)(p + 4) = float4_t{v[4], v[5], v[6], v[7]};
+    } else {
+        typename Num<S>::v8 a;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = (S)v[e];
+        *(typename Num<S>::v8*)p = a;
+    }
+}
+
+// v[p] times (product) or plus a channel vector's piece, where there is one.
+template <bool PRODUCT>
+__device__ __forceinline__ void with_vector(const float* vector, int c, float (&v)[8]) {
+    if (!vector) return;
+    float w[8];
+    load8(vector + c, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = PRODUCT ? v[e] * w[e] : v[e] + w[e];
+}
+
+// One norm of the row whose P pieces of 8 channels a lane holds (zeros where a
+// piece does not exist). The mean first, then the sum of squared deviations from
+// it, both from registers. part: 2 G / 64 floats, taken in turn.
+template <int G, int P>
+__device__ __forceinline__ void normalise(float (&v)[P][8], const bool (&there)[P], const int (&at)[P], int kind, float eps, int channels,
+                                          const float* weight, const float* bias, float* part) {
+    const float each = 1.0f / (float)channels;
+    if (kind == DHX_NORM_LAYER) {
+        float sum = 0.f;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += v[p][e];
+        const float mean = row_sum<G>(sum, part) * each;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[p][e] = there[p] ? v[p][e] - mean : 0.f;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(v[p][e], v[p][e], sum);
+    const float scale = rsqrtf(fmaf(row_sum<G>(sum, part + (G > 64 ? G / 64 : 0)), each, eps));
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[p][e] *= scale;
+        if (there[p]) {
+            with_vector<true>(weight, at[p], v[p]);
+            with_vector<false>(bias, at[p], v[p]);
+        }
+    }
+}
+
+// T: y and h, S: x and x'. G lanes hold a row, P pieces of 8 channels each: piece p
+// of lane l is G p + l of the row.
+template <class T, class S, int G, int P>
+__global__ __launch_bounds__(G <= 64 ? 256 : G) void packed_norm_kernel(DHX_NORM_PARAMS) {
+    constexpr int THREADS = G <= 64 ? 256 : G, ROWS = THREADS / G, WAVE_ROWS = G <= 64 ? 64 / G : 1;
+    __shared__ float part[G > 64 ? 4 * G / 64 : 1];
+    const S* x = x_;
+    const T* y = y_;
+    const int tid = threadIdx.x, lane = tid % G, in_wave = G <= 64 ? (tid & 63) / G : 0;
+    const int pieces = channels >> 3;
+    bool there[P];
+    int at[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        there[p] = G * p + lane < pieces;
+        at[p] = (G * p + lane) * 8;
+    }
+    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < rows; first += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = first + tid / G;
+        const int32_t* starts = starts_;
+        bool in = row < rows;
+        int s = 0;
+        if (gate_.a) {
+            s = sequence_of<WAVE_ROWS>(starts, sequences, rows, (int)(row - in_wave), in_wave);
+            in = in && s >= 0 && row < start_at(starts, s + 1, rows);
+        } else if (starts_.a) {
+            in = in && row >= start_at(starts, 0, rows) && row < start_at(starts, sequences, rows);
+        }
+        float v[P][8], z[P][8];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[p][e] = z[p][e] = 0.f;
+            if (in && there[p]) {
+                load8(x + row * x_stride + at[p], v[p]);
+                if (y) load8(y + row * y_stride + at[p], z[p]);
+            }
+        }
+        if (y) {
+            if (post != DHX_NORM_NONE) normalise<G, P>(z, there, at, post, post_eps, channels, post_weight_, post_bias_, part);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (in && there[p]) {
+                    with_vector<true>(scale_, at[p], z[p]);
+                    if (gate_.a) with_vector<true>((const float*)gate_ + s * gate_stride, at[p], z[p]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[p][e] += z[p][e];
+                    store8((S*)x_out_ + row * x_out_stride + at[p], v[p]);
+                }
+        }
+        if (pre != DHX_NORM_NONE) {
+            normalise<G, P>(v, there, at, pre, pre_eps, channels, pre_weight_, pre_bias_, part + (G > 64 ? 2 * G / 64 : 0));
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (in && there[p]) store8((T*)h_ + row * h_stride + at[p], v[p]);
+        }
+        if (G > 64) __syncthreads();  // part, for the next row
+    }
+}
+
+constexpr uint64_t kMostBlocks = 1u << 21;  // a launch has fewer than 2^32 threads; workgroups take further rows in turn
+
+template <class T, class S, int G, int P>
+hipError_t launch(const dhx_packed_norm& p, hipStream_t s) {
+    constexpr int THREADS = G <= 64 ? 256 : G, ROWS = THREADS / G;
+    const uint64_t blocks = std::min<uint64_t>((p.rows + ROWS - 1) / ROWS, kMostBlocks);
+    return enqueue(packed_norm_kernel<T, S, G, P>, dim3((unsigned)blocks), dim3(THREADS), 0, s, p.x, p.y, p.x_out, p.h, (int)p.rows,
+                   (int)p.channels, p.x_stride, p.y_stride, p.starts, p.scale, p.gate, p.post_weight, p.post_bias, p.pre_weight,
+                   p.pre_bias, p.x_out_stride, p.h_stride, p.gate_stride, (int)p.sequences, (int)p.post, (int)p.pre, p.post_eps,
+                   p.pre_eps);
+}
+
+template <class T, class S>
+hipError_t launch_pieces(const dhx_packed_norm& p, hipStream_t s) {
+    const uint32_t pieces = p.channels / 8;
+    if (pieces <= 16) return launch<T, S, 16, 1>(p, s);
+    if (pieces <= 64) return launch<T, S, 16, 4>(p, s);
+    if (pieces <= 256) return launch<T, S, 64, 4>(p, s);
+    if (pieces <= 1024) return launch<T, S, 256, 4>(p, s);
+    return launch<T, S, 1024, 4>(p, s);
+}
+
+template <class T>
+hipError_t launch_type(const dhx_packed_norm& p, hipStream_t s) {
+    return p.stream_type == DHX_F32 ? launch_pieces<T, float>(p, s) : launch_pieces<T, T>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_packed_norm(const dhx_packed_norm& p, hipStream_t s) {
+    return p.type == DHX_F16 ? launch_type<half_t>(p, s) : launch_type<bf16_t>(p, s);
+}
+
+}  // namespace dhx

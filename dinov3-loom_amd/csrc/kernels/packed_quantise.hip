@@ -1,0 +1,121 @@
+// Rows of a packed batch to 4-bit codes with a scale per block of 32 values, and
+// back (include/dinov3_packed.h). Every value is read once and every code written
+// once, or the other way round; there is little arithmetic, so both are bound by
+// memory. A lane takes 8 values (16 bytes), four lanes a block.
+#include <algorithm>
+
+#include "packed.hpp"
+
+namespace dhx {
+namespace {
+
+#define DHX_QUANTISE_PARAMS Addr x_, Addr codes_, Addr scales_, int rows, int columns, uint64_t x_stride, uint64_t codes_stride, uint64_t scales_stride, Addr starts_, int sequences, int block_rows
+
+// The float whose exponent is scale byte b's (what the conversions take).
+__device__ __forceinline__ float scale_of(uint32_t b) { return __builtin_bit_cast(float, b << 23); }
+
+// Codes of two values; which byte of `to` they go into is a constant.
+template <int BYTE>
+__device__ __forceinline__ uint32_t two_codes(uint32_t to, half2_t v, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(to, v, scale, BYTE);
+}
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+template <int BYTE>
+__device__ __forceinline__ uint32_t two_codes(uint32_t to, bf16x2_t v, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(to, v, scale, BYTE);
+}
+
+// Whether the rows of the call hold `row`.
+__device__ __forceinline__ bool counts(const int32_t* starts, int sequences, int rows, int64_t row) {
+    return !starts || (row >= start_at(starts, 0, rows) && row < start_at(starts, sequences, rows));
+}
+
+// A workgroup takes block_rows rows at a time; an item is 8 columns of a row. The
+// items of a row are whole blocks and, behind them, what fills the scales up to 16.
+template <class T>
+__global__ __launch_bounds__(256) void packed_quantise_kernel(DHX_QUANTISE_PARAMS) {
+    typedef typename Num<T>::v8 v8;
+    typedef T v2 __attribute__((ext_vector_type(2)));
+    const int blocks = (columns + 31) >> 5, per_row = ((blocks + 15) & ~15) * 4;
+    for (int64_t row0 = (int64_t)blockIdx.x * block_rows; row0 < rows; row0 += (int64_t)gridDim.x * block_rows) {
+        const int n = (int)min((int64_t)block_rows, rows - row0) * per_row;
+        for (int i = threadIdx.x; i < n; i += 256) {  // n is a multiple of 64: whole waves
+            const int r = i / per_row, piece = i - r * per_row;
+            const int64_t row = row0 + r;
+            v8 v = {};
+            const bool in = counts(starts_, sequences, rows, row);
+            if (in && piece * 8 < columns) v = *(const v8*)((const T*)x_ + row * x_stride + piece * 8);
+            // The largest magnitude of the block's 32 values, as the bits of a T: those of
+            // magnitudes are in order, and what is not finite lies above all others.
+            const uint4_t w = __builtin_bit_cast(uint4_t, v);
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 top = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+            uint32_t m = max((uint32_t)top[0], (uint32_t)top[1]);
+            m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, false));  // quad_perm 1, 0, 3, 2
+            m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, false));  // quad_perm 2, 3, 0, 1
+            const float largest = (float)__builtin_bit_cast(T, (uint16_t)m);
+            const int exponent = (int)(__builtin_bit_cast(uint32_t, largest) >> 23);
+            const bool odd = exponent == 255;
+            const uint32_t byte = odd ? 255 : (uint32_t)max(exponent - 2, 0);
+            const float scale = scale_of(byte);
+            uint32_t c = 0;
+            c = two_codes<0>(c, v2{v[0], v[1]}, scale);
+            c = two_codes<1>(c, v2{v[2], v[3]}, scale);
+            c = two_codes<2>(c, v2{v[4], v[5]}, scale);
+            c = two_codes<3>(c, v2{v[6], v[7]}, scale);
+            if (!in) continue;
+            if (piece < blocks * 4) *(uint32_t*)((char*)codes_ + row * codes_stride + piece * 4) = odd ? 0 : c;
+            if ((piece & 3) == 0) *((uint8_t*)scales_ + row * scales_stride + (piece >> 2)) = piece < blocks * 4 ? (uint8_t)byte : 0;
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void packed_dequantise_kernel(DHX_QUANTISE_PARAMS) {
+    typedef typename Num<T>::v8 v8;
+    const int per_row = columns >> 3;
+    for (int64_t row0 = (int64_t)blockIdx.x * block_rows; row0 < rows; row0 += (int64_t)gridDim.x * block_rows) {
+        const int n = (int)min((int64_t)block_rows, rows - row0) * per_row;
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const int r = i / per_row, piece = i - r * per_row;
+            const int64_t row = row0 + r;
+            if (!counts(starts_, sequences, rows, row)) continue;
+            const uint32_t c = *(const uint32_t*)((const char*)codes_ + row * codes_stride + piece * 4);
+            const float scale = scale_of(*((const uint8_t*)scales_ + row * scales_stride + (piece >> 2)));
+            v8 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2_t two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c >> (8 * e), scale, 0);
+                v[2 * e] = (T)two[0];
+                v[2 * e + 1] = (T)two[1];
+            }
+            *(v8*)((T*)x_ + row * x_stride + piece * 8) = v;
+        }
+    }
+}
+
+constexpr uint64_t kMostBlocks = 1u << 21;  // a launch has fewer than 2^32 threads; workgroups take further rows in turn
+
+template <class K>
+hipError_t launch(K kernel, const dhx_packed_quantisation& p, uint64_t per_row, hipStream_t s) {
+    const int block_rows = (int)std::max<uint64_t>(256 / per_row, 1);
+    const uint64_t blocks = std::min<uint64_t>((p.rows + block_rows - 1) / block_rows, kMostBlocks);
+    return enqueue(kernel, dim3((unsigned)blocks), dim3(256), 0, s, p.x, p.codes, p.scales, (int)p.rows, (int)p.columns, p.x_stride,
+                   p.codes_stride, p.scales_stride, p.starts, (int)p.sequences, block_rows);
+}
+
+}  // namespace
+
+hipError_t launch_packed_quantise(const dhx_packed_quantisation& p, hipStream_t s) {
+    const uint64_t per_row = scale_bytes(p.columns) * 4;
+    return p.type == DHX_F16 ? launch(packed_quantise_kernel<half_t>, p, per_row, s) : launch(packed_quantise_kernel<bf16_t>, p, per_row, s);
+}
+
+hipError_t launch_packed_dequantise(const dhx_packed_quantisation& p, hipStream_t s) {
+    const uint64_t per_row = p.columns / 8;
+    return p.type == DHX_F16 ? launch(packed_dequantise_kernel<half_t>, p, per_row, s) : launch(packed_dequantise_kernel<bf16_t>, p, per_row, s);
+}
+
+}  // namespace dhx

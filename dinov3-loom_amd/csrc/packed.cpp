@@ -4,6 +4,7 @@
 
 #include <cmath>
 #include <string>
+#include <utility>
 
 #include "../../include/dinov3_packed.h"
 #include "engine_internal.hpp"
@@ -171,6 +172,138 @@ void attention_check(const dhx_packed_attention& p) {
     workspace(p.workspace, p.workspace_bytes, dhx::packed_attention_cut(p).bytes);
 }
 
+// Starts may be missing in the calls of the feed-forward half: then all rows count.
+void optional_starts(const int32_t* starts, uint32_t sequences) {
+    most(sequences, kMaxRows, "sequences");
+    if (starts) {
+        positive(sequences, "sequences");
+        pointer(starts, 4, "starts");
+    } else if (sequences != 0) {
+        throw Error("starts is a null device pointer");
+    }
+}
+
+void norm_check(const dhx_packed_norm& p) {
+    type_of(p.type);
+    if (p.stream_type != p.type && p.stream_type != DHX_F32) throw Error("stream_type must be type or DHX_F32");
+    for (uint32_t kind : {p.post, p.pre})
+        if (kind > DHX_NORM_LAYER) throw Error("post and pre must be DHX_NORM_NONE, DHX_NORM_RMS or DHX_NORM_LAYER");
+    most(p.rows, kMaxRows, "rows");
+    eights(p.channels, "channels");
+    most(p.channels, 32768, "channels");
+    for (float eps : {p.post_eps, p.pre_eps})
+        if (!(eps >= 0) || !std::isfinite(eps)) throw Error("post_eps and pre_eps must be finite and not negative");
+    optional_starts(p.starts, p.sequences);
+    const bool work = p.rows > 0;
+    pointer(p.x, 16, "x", work);
+    stride(p.x_stride, p.channels, "x_stride");
+    if (p.y) {
+        pointer(p.y, 16, "y");
+        pointer(p.x_out, 16, "x_out", work);
+        stride(p.y_stride, p.channels, "y_stride");
+        stride(p.x_out_stride, p.channels, "x_out_stride");
+        if (work && p.x == p.x_out && p.x_stride != p.x_out_stride) throw Error("in place, x_out_stride must be x_stride");
+    } else if (work && (p.post != DHX_NORM_NONE || p.pre == DHX_NORM_NONE || p.scale || p.gate || p.x_out)) {
+        throw Error("without y there are no post, scale, gate and x_out, and pre is needed");
+    }
+    if (p.pre != DHX_NORM_NONE) {
+        pointer(p.h, 16, "h", work);
+        stride(p.h_stride, p.channels, "h_stride");
+        if (p.h && p.h == p.y && p.h_stride != p.y_stride) throw Error("in place, h_stride must be y_stride");
+    } else if (p.h) {
+        throw Error("h needs a norm in pre");
+    }
+    const std::pair<const float*, const char*> vectors[] = {{p.post_weight, "post_weight"}, {p.post_bias, "post_bias"},
+                                                            {p.pre_weight, "pre_weight"},   {p.pre_bias, "pre_bias"},
+                                                            {p.scale, "scale"},             {p.gate, "gate"}};
+    for (const auto& [v, what] : vectors) pointer(v, 16, what, false);
+    if (p.post == DHX_NORM_NONE && (p.post_weight || p.post_bias)) throw Error("post_weight and post_bias need a norm in post");
+    if (p.pre == DHX_NORM_NONE && (p.pre_weight || p.pre_bias)) throw Error("pre_weight and pre_bias need a norm in pre");
+    if (p.gate) {
+        if (!p.starts) throw Error("gate needs starts");
+        stride(p.gate_stride, p.channels, "gate_stride");
+    }
+}
+
+// A stride in bytes, of codes or scales.
+void byte_stride(uint64_t v, uint64_t least, const char* what) {
+    if (v % 16 != 0) throw Error(std::string(what) + " must be a multiple of 16");
+    if (v < least) throw Error(std::string(what) + " must be at least " + std::to_string(least));
+    most(v, 2 * kMaxStride, what);
+}
+
+void quantisation_check(const dhx_packed_quantisation& p) {
+    type_of(p.type);
+    if (p.reserved != 0) throw Error("reserved must be 0");
+    most(p.rows, kMaxRows, "rows");
+    eights(p.columns, "columns");
+    most(p.columns, kMaxStride, "columns");
+    optional_starts(p.starts, p.sequences);
+    pointer(p.x, 16, "x", p.rows > 0);
+    pointer(p.codes, 16, "codes", p.rows > 0);
+    pointer(p.scales, 16, "scales", p.rows > 0);
+    stride(p.x_stride, p.columns, "x_stride");
+    byte_stride(p.codes_stride, dhx::code_bytes(p.columns), "codes_stride");
+    byte_stride(p.scales_stride, dhx::scale_bytes(p.columns), "scales_stride");
+}
+
+// What the two products of the feed-forward half have in common.
+void product_sizes(uint32_t type, uint64_t rows, uint32_t inputs, uint32_t outputs) {
+    type_of(type);
+    most(rows, kMaxLinearRows, "rows");
+    eights(inputs, "inputs");
+    eights(outputs, "outputs");
+    most(inputs, kMaxStride, "inputs");
+    most(outputs, kMaxStride, "outputs");
+    most(((rows + 255) / 256) * ((outputs + 127) / 128), kMaxLinearTiles, "the number of tiles of 256 x 128 outputs");
+}
+
+void quantised_linear_sizes(const dhx_packed_quantised_linear& p) { product_sizes(p.type, p.rows, p.inputs, p.outputs); }
+
+void quantised_linear_check(const dhx_packed_quantised_linear& p) {
+    quantised_linear_sizes(p);
+    optional_starts(p.starts, p.sequences);
+    pointer(p.x, 16, "x", p.rows > 0);
+    pointer(p.w, 16, "w");
+    pointer(p.w_scales, 16, "w_scales");
+    pointer(p.bias, 16, "bias", false);
+    pointer(p.y, 16, "y", p.rows > 0);
+    stride(p.x_stride, p.inputs, "x_stride");
+    stride(p.y_stride, p.outputs, "y_stride");
+    byte_stride(p.w_stride, dhx::code_bytes(p.inputs), "w_stride");
+    byte_stride(p.scales_stride, dhx::scale_bytes(p.inputs), "scales_stride");
+    workspace(p.workspace, p.workspace_bytes, dhx::packed_quantised_linear_bytes(p));
+}
+
+void gated_sizes(const dhx_packed_gated& p) {
+    product_sizes(p.type, p.rows, p.inputs, p.outputs);
+    if (!p.gate_scales != !p.up_scales) throw Error("gate_scales and up_scales come together");
+}
+
+void gated_check(const dhx_packed_gated& p) {
+    gated_sizes(p);
+    if (p.activation > DHX_SIGMOID) throw Error("activation must be one of DHX_SILU to DHX_SIGMOID");
+    if (p.reserved != 0) throw Error("reserved must be 0");
+    optional_starts(p.starts, p.sequences);
+    pointer(p.x, 16, "x", p.rows > 0);
+    pointer(p.gate, 16, "gate");
+    pointer(p.up, 16, "up");
+    pointer(p.gate_bias, 16, "gate_bias", false);
+    pointer(p.up_bias, 16, "up_bias", false);
+    pointer(p.out, 16, "out", p.rows > 0);
+    stride(p.x_stride, p.inputs, "x_stride");
+    stride(p.out_stride, p.outputs, "out_stride");
+    if (p.gate_scales) {
+        pointer(p.gate_scales, 16, "gate_scales");
+        pointer(p.up_scales, 16, "up_scales");
+        byte_stride(p.w_stride, dhx::code_bytes(p.inputs), "w_stride");
+        byte_stride(p.scales_stride, dhx::scale_bytes(p.inputs), "scales_stride");
+    } else {
+        stride(p.w_stride, p.inputs, "w_stride");
+    }
+    workspace(p.workspace, p.workspace_bytes, dhx::packed_gated_bytes(p));
+}
+
 // The caller's current device again on every way out.
 class KeepDevice {
 public:
@@ -265,6 +398,72 @@ int dhx_packed_attention_run(dhx_engine* e, const dhx_packed_attention* p, void*
             return a.q_rows > 0;
         },
         [](const dhx_packed_attention& a, hipStream_t s) { return dhx::launch_packed_attention(with_head_strides(a), s); });
+}
+
+int dhx_packed_norm_run(dhx_engine* e, const dhx_packed_norm* p, void* stream) {
+    return run(
+        e, p, stream,
+        [](const dhx_packed_norm& a) {
+            norm_check(a);
+            return a.rows > 0;
+        },
+        dhx::launch_packed_norm);
+}
+
+int dhx_packed_quantise_run(dhx_engine* e, const dhx_packed_quantisation* p, void* stream) {
+    return run(
+        e, p, stream,
+        [](const dhx_packed_quantisation& a) {
+            quantisation_check(a);
+            return a.rows > 0;
+        },
+        dhx::launch_packed_quantise);
+}
+
+int dhx_packed_dequantise_run(dhx_engine* e, const dhx_packed_quantisation* p, void* stream) {
+    return run(
+        e, p, stream,
+        [](const dhx_packed_quantisation& a) {
+            quantisation_check(a);
+            return a.rows > 0;
+        },
+        dhx::launch_packed_dequantise);
+}
+
+int dhx_packed_quantised_linear_workspace(const dhx_packed_quantised_linear* p, uint64_t* bytes) {
+    return guarded(nullptr, [&] {
+        if (!p || !bytes) throw Error("null argument");
+        quantised_linear_sizes(*p);
+        *bytes = dhx::packed_quantised_linear_bytes(*p);
+    });
+}
+
+int dhx_packed_quantised_linear_run(dhx_engine* e, const dhx_packed_quantised_linear* p, void* stream) {
+    return run(
+        e, p, stream,
+        [](const dhx_packed_quantised_linear& a) {
+            quantised_linear_check(a);
+            return a.rows > 0;
+        },
+        dhx::launch_packed_quantised_linear);
+}
+
+int dhx_packed_gated_workspace(const dhx_packed_gated* p, uint64_t* bytes) {
+    return guarded(nullptr, [&] {
+        if (!p || !bytes) throw Error("null argument");
+        gated_sizes(*p);
+        *bytes = dhx::packed_gated_bytes(*p);
+    });
+}
+
+int dhx_packed_gated_run(dhx_engine* e, const dhx_packed_gated* p, void* stream) {
+    return run(
+        e, p, stream,
+        [](const dhx_packed_gated& a) {
+            gated_check(a);
+            return a.rows > 0;
+        },
+        dhx::launch_packed_gated);
 }
 
 }  // extern "C"

@@ -509,9 +509,38 @@ class Engine:
         """dhx_packed_attention_run: softmax attention inside each sequence."""
         self._c(_lib.dhx_packed_attention_run(self._h, ctypes.byref(call), stream))
 
+    def packed_norm(self, call: packed.Norm, stream: int = 0) -> None:
+        """dhx_packed_norm_run: the residual step behind a block, with the norms before and behind it."""
+        self._c(_lib.dhx_packed_norm_run(self._h, ctypes.byref(call), stream))
+
+    def packed_quantise(self, call: packed.Quantisation, stream: int = 0) -> None:
+        """dhx_packed_quantise_run: rows to 4-bit codes with a scale per 32 values."""
+        self._c(_lib.dhx_packed_quantise_run(self._h, ctypes.byref(call), stream))
+
+    def packed_dequantise(self, call: packed.Quantisation, stream: int = 0) -> None:
+        """dhx_packed_dequantise_run: the values of such codes, written to x."""
+        self._c(_lib.dhx_packed_dequantise_run(self._h, ctypes.byref(call), stream))
+
+    def packed_quantised_linear_workspace(self, call: packed.QuantisedLinear) -> int:
+        """Bytes of device memory that packed_quantised_linear needs for these sizes."""
+        return packed_workspace("quantised_linear", call)
+
+    def packed_quantised_linear(self, call: packed.QuantisedLinear, stream: int = 0) -> None:
+        """dhx_packed_quantised_linear_run: a projection whose weights are held in 4 bits."""
+        self._c(_lib.dhx_packed_quantised_linear_run(self._h, ctypes.byref(call), stream))
+
+    def packed_gated_workspace(self, call: packed.Gated) -> int:
+        """Bytes of device memory that packed_gated needs for these sizes (0 without codes)."""
+        return packed_workspace("gated", call)
+
+    def packed_gated(self, call: packed.Gated, stream: int = 0) -> None:
+        """dhx_packed_gated_run: both projections of a gated feed-forward block, the activation and the product."""
+        self._c(_lib.dhx_packed_gated_run(self._h, ctypes.byref(call), stream))
+
 
 def packed_workspace(operator: str, call) -> int:
-    """Bytes of workspace of a packed.Linear ("linear") or packed.Attention ("attention") call."""
+    """Bytes of workspace of a packed.Linear ("linear"), packed.Attention ("attention"), packed.Gated ("gated") or
+    packed.QuantisedLinear ("quantised_linear") call."""
     need = ctypes.c_uint64()
     _check_engine(getattr(_lib, f"dhx_packed_{operator}_workspace")(ctypes.byref(call), ctypes.byref(need)), None)
     return int(need.value)

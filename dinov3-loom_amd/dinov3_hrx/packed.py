@@ -1,6 +1,7 @@
 """The operators on packed batches (include/dinov3_packed.h): a projection with
-low-rank adapters, the position rotation, and attention, over the rows of many
-sequences that lie back to back. A call is described once, with device
+low-rank adapters, the position rotation, attention, and the feed-forward half of a
+block (norms with the residual step between them, the gated projection, rows and
+weights in 4 bits), over the rows of many sequences that lie back to back. A call is described once, with device
 addresses as integers, and run by an Engine any number of times:
 
     from dinov3_hrx import Engine, packed
@@ -15,9 +16,11 @@ from __future__ import annotations
 
 import ctypes
 
-F16, BF16 = 0, 1
+F16, BF16, F32 = 0, 1, 2
+NONE, RMS, LAYER = 0, 1, 2  # norms
+SILU, GELU, GELU_TANH, RELU, SIGMOID = 0, 1, 2, 3, 4
 
-_u32, _u64, _p = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p
+_u32, _u64, _p, _f32 = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_float
 
 
 class Linear(ctypes.Structure):
@@ -45,9 +48,42 @@ class Attention(ctypes.Structure):
                 ("lse", _p), ("q_starts", _p), ("k_starts", _p), ("workspace", _p), ("workspace_bytes", _u64)]
 
 
+class Norm(ctypes.Structure):
+    """dhx_packed_norm."""
+    _fields_ = [("type", _u32), ("stream_type", _u32), ("post", _u32), ("pre", _u32), ("rows", _u64), ("channels", _u32),
+                ("sequences", _u32), ("post_eps", _f32), ("pre_eps", _f32), ("x", _p), ("y", _p), ("x_out", _p), ("h", _p),
+                ("post_weight", _p), ("post_bias", _p), ("pre_weight", _p), ("pre_bias", _p), ("scale", _p), ("gate", _p),
+                ("x_stride", _u64), ("y_stride", _u64), ("x_out_stride", _u64), ("h_stride", _u64), ("gate_stride", _u64),
+                ("starts", _p)]
+
+
+class Quantisation(ctypes.Structure):
+    """dhx_packed_quantisation."""
+    _fields_ = [("type", _u32), ("sequences", _u32), ("rows", _u64), ("columns", _u32), ("reserved", _u32), ("x", _p),
+                ("codes", _p), ("scales", _p), ("x_stride", _u64), ("codes_stride", _u64), ("scales_stride", _u64),
+                ("starts", _p)]
+
+
+class QuantisedLinear(ctypes.Structure):
+    """dhx_packed_quantised_linear."""
+    _fields_ = [("type", _u32), ("sequences", _u32), ("rows", _u64), ("inputs", _u32), ("outputs", _u32), ("x", _p), ("w", _p),
+                ("w_scales", _p), ("bias", _p), ("y", _p), ("x_stride", _u64), ("y_stride", _u64), ("w_stride", _u64),
+                ("scales_stride", _u64), ("starts", _p), ("workspace", _p), ("workspace_bytes", _u64)]
+
+
+class Gated(ctypes.Structure):
+    """dhx_packed_gated."""
+    _fields_ = [("type", _u32), ("activation", _u32), ("rows", _u64), ("inputs", _u32), ("outputs", _u32), ("sequences", _u32),
+                ("reserved", _u32), ("x", _p), ("gate", _p), ("up", _p), ("gate_scales", _p), ("up_scales", _p),
+                ("gate_bias", _p), ("up_bias", _p), ("out", _p), ("x_stride", _u64), ("out_stride", _u64), ("w_stride", _u64),
+                ("scales_stride", _u64), ("starts", _p), ("workspace", _p), ("workspace_bytes", _u64)]
+
+
 def declare(lib) -> None:
     """Argument types of the C functions."""
-    for name, call in (("linear", Linear), ("rotation", Rotation), ("attention", Attention)):
+    calls = {"linear": Linear, "rotation": Rotation, "attention": Attention, "norm": Norm, "quantise": Quantisation,
+             "dequantise": Quantisation, "quantised_linear": QuantisedLinear, "gated": Gated}
+    for name, call in calls.items():
         getattr(lib, f"dhx_packed_{name}_run").argtypes = [_p, ctypes.POINTER(call), _p]
-        if call is not Rotation:
+        if any(field == "workspace" for field, _ in call._fields_):
             getattr(lib, f"dhx_packed_{name}_workspace").argtypes = [ctypes.POINTER(call), ctypes.POINTER(_u64)]

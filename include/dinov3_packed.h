@@ -47,7 +47,7 @@
 extern "C" {
 #endif
 
-enum { DHX_F16 = 0, DHX_BF16 = 1 };
+enum { DHX_F16 = 0, DHX_BF16 = 1, DHX_F32 = 2 };
 
 /* A projection that all sequences share, and beside it the low-rank adapter
  * of each sequence's own request:
@@ -144,6 +144,133 @@ typedef struct dhx_packed_attention {
 
 int dhx_packed_attention_workspace(const dhx_packed_attention *p, uint64_t *bytes);
 int dhx_packed_attention_run(dhx_engine *e, const dhx_packed_attention *p, void *stream);
+
+/* --- the feed-forward half of a block ---------------------------------------
+ *
+ * In these calls `starts` may be NULL, with `sequences` 0: then every row counts
+ * (the norm without a gate of its own per sequence). With starts, rows in front
+ * of starts[0] and from starts[sequences] on are left as they were, as above. */
+
+/* The residual step behind a block, with the norm of the block's output before
+ * it and the norm of the next block's input behind it:
+ *   z = post(y[t]),  x_out[t] = x[t] + gate[s] * scale * z,  h[t] = pre(x_out[t])
+ * for every row t of sequence s, per channel. A norm is DHX_NORM_RMS, v /
+ * sqrt(mean(v^2) + eps) * weight + bias, DHX_NORM_LAYER, the same of v - mean(v),
+ * or DHX_NORM_NONE: z is y, or there is no h (h is NULL then, and only then).
+ * Without y (NULL; no post, scale, gate or x_out) h is pre(x), as in front of the
+ * first block. The channel vectors are float32, NULL: ones for weight, scale and
+ * gate, zeros for bias. Statistics, sums and the x_out that pre takes are float32:
+ * h does not see x_out's rounding to its type. A row with a value that is not
+ * finite has outputs that are not, others are not touched by it; a row whose
+ * squares pass the range of float32 gives zeros (v / infinity) or NaN.
+ * x_out may be x and h may be y, with the same stride (in place). */
+enum { DHX_NORM_NONE = 0, DHX_NORM_RMS = 1, DHX_NORM_LAYER = 2 };
+
+typedef struct dhx_packed_norm {
+    uint32_t type;        /* DHX_F16 or DHX_BF16: y, h */
+    uint32_t stream_type; /* the same, or DHX_F32: x, x_out */
+    uint32_t post, pre;   /* DHX_NORM_ */
+    uint64_t rows;
+    uint32_t channels;    /* to 32768 */
+    uint32_t sequences;
+    float post_eps, pre_eps; /* not negative */
+    const void *x;        /* [rows][channels] */
+    const void *y;        /* [rows][channels]; NULL: h = pre(x) */
+    void *x_out;          /* [rows][channels] */
+    void *h;              /* [rows][channels]; NULL where pre is none */
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias, *scale; /* [channels] */
+    const float *gate;    /* [sequences][channels], gate_stride apart */
+    uint64_t x_stride, y_stride, x_out_stride, h_stride, gate_stride;
+    const int32_t *starts; /* [sequences + 1] */
+} dhx_packed_norm;
+
+int dhx_packed_norm_run(dhx_engine *e, const dhx_packed_norm *p, void *stream);
+
+/* 4-bit values with a scale per block of 32 along a row (microscaled e2m1, "MXFP4"
+ * of the OCP Microscaling Formats specification, version 1.0). A code's low three
+ * bits stand for 0, 0.5, 1, 1.5, 2, 3, 4, 6, its bit 3 for the sign; a byte holds two
+ * codes, the first in its low half. A scale byte b stands for 2^(b - 127), 255 for
+ * not a number. Of a block whose largest magnitude is m, b - 127 = floor(log2 m) - 2,
+ * held inside -127 .. 127 (m = 0: -127); a value becomes the nearest code times the
+ * scale, ties to the even code, what is past 6 times the scale 6. A block with a
+ * value that is not finite has codes 0 and scale byte 255. A row's last block may be
+ * short (columns is a multiple of 8): it is filled up with zeros.
+ * A row of codes has 16 bytes per block; a row of scales has a byte per block and,
+ * up to the next multiple of 16, bytes that are written as 0 and whose values are
+ * never looked at. Both strides are in bytes and multiples of 16.
+ * dequantise writes the values to x, each rounded to its type. */
+typedef struct dhx_packed_quantisation {
+    uint32_t type; /* DHX_F16 or DHX_BF16: x */
+    uint32_t sequences;
+    uint64_t rows;
+    uint32_t columns, reserved; /* 0 */
+    void *x;         /* [rows][columns]: read by quantise, written by dequantise */
+    uint8_t *codes;  /* [rows][16 ceil(columns / 32)] */
+    uint8_t *scales; /* [rows][16 ceil(columns / 512)] */
+    uint64_t x_stride, codes_stride, scales_stride;
+    const int32_t *starts; /* [sequences + 1] */
+} dhx_packed_quantisation;
+
+int dhx_packed_quantise_run(dhx_engine *e, const dhx_packed_quantisation *p, void *stream);
+int dhx_packed_dequantise_run(dhx_engine *e, const dhx_packed_quantisation *p, void *stream);
+
+/* A projection whose weights are held in 4 bits:
+ *   y[t] = w Q(x[t]) + bias,
+ * Q(x) the row quantised as above within the call (so the products are of 4-bit
+ * values, which the matrix units multiply at four times the rate of 16-bit ones;
+ * products and sums are float32). A block of x or w that is not a number makes
+ * its row's or column's outputs not a number. */
+typedef struct dhx_packed_quantised_linear {
+    uint32_t type; /* DHX_F16 or DHX_BF16: x, y */
+    uint32_t sequences;
+    uint64_t rows;
+    uint32_t inputs, outputs;
+    const void *x;           /* [rows][inputs] */
+    const uint8_t *w;        /* [outputs][16 ceil(inputs / 32)]: codes */
+    const uint8_t *w_scales; /* [outputs][16 ceil(inputs / 512)] */
+    const float *bias;       /* [outputs]; NULL: none */
+    void *y;                 /* [rows][outputs] */
+    uint64_t x_stride, y_stride;      /* elements */
+    uint64_t w_stride, scales_stride; /* bytes */
+    const int32_t *starts;   /* [sequences + 1] */
+    void *workspace;
+    uint64_t workspace_bytes;
+} dhx_packed_quantised_linear;
+
+int dhx_packed_quantised_linear_workspace(const dhx_packed_quantised_linear *p, uint64_t *bytes);
+int dhx_packed_quantised_linear_run(dhx_engine *e, const dhx_packed_quantised_linear *p, void *stream);
+
+/* The gated projections of a feed-forward block, in one kernel:
+ *   out[t] = act(gate x[t] + gate_bias) * (up x[t] + up_bias),
+ * act(g) = g / (1 + e^-g) (SILU), g (1 + erf(g / sqrt 2)) / 2 (GELU), its form
+ * g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 (GELU_TANH), max(g, 0) (RELU) or
+ * 1 / (1 + e^-g) (SIGMOID). Both sums stay float32 up to the product, which is
+ * rounded once. Where a sum is infinite or not a number, so may be the output.
+ * The weights are of the type of x, or, with gate_scales and up_scales, 4-bit
+ * codes as above; then x is quantised alike within the call, and only then is
+ * there a workspace. The matrices may be the halves of one. */
+enum { DHX_SILU = 0, DHX_GELU = 1, DHX_GELU_TANH = 2, DHX_RELU = 3, DHX_SIGMOID = 4 };
+
+typedef struct dhx_packed_gated {
+    uint32_t type; /* DHX_F16 or DHX_BF16: x, out, and gate and up without scales */
+    uint32_t activation;
+    uint64_t rows;
+    uint32_t inputs, outputs;
+    uint32_t sequences, reserved; /* 0 */
+    const void *x;          /* [rows][inputs] */
+    const void *gate, *up;  /* [outputs][inputs], or codes [outputs][16 ceil(inputs / 32)] */
+    const uint8_t *gate_scales, *up_scales; /* [outputs][16 ceil(inputs / 512)]; NULL, both: no codes */
+    const float *gate_bias, *up_bias;       /* [outputs]; NULL: none */
+    void *out;              /* [rows][outputs] */
+    uint64_t x_stride, out_stride;    /* elements */
+    uint64_t w_stride, scales_stride; /* of gate and up: elements, or bytes of codes; bytes */
+    const int32_t *starts;  /* [sequences + 1] */
+    void *workspace;
+    uint64_t workspace_bytes;
+} dhx_packed_gated;
+
+int dhx_packed_gated_workspace(const dhx_packed_gated *p, uint64_t *bytes);
+int dhx_packed_gated_run(dhx_engine *e, const dhx_packed_gated *p, void *stream);
 
 #ifdef __cplusplus
 }
