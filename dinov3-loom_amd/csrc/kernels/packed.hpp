@@ -59,7 +59,9 @@ hipError_t launch_packed_rotation(const dhx_packed_rotation& p, hipStream_t s);
 
 hipError_t launch_packed_norm(const dhx_packed_norm& p, hipStream_t s);
 
-hipError_t launch_packed_quantise(const dhx_packed_quantisation& p, hipStream_t s);
+// group_stride: from the scales of a row's 32 blocks to those of the next 32 (32: a
+// row's scales are one piece).
+hipError_t launch_packed_quantise(const dhx_packed_quantisation& p, hipStream_t s, uint64_t group_stride = 32);
 hipError_t launch_packed_dequantise(const dhx_packed_quantisation& p, hipStream_t s);
 
 uint64_t packed_quantised_linear_bytes(const dhx_packed_quantised_linear& p);

@@ -5,14 +5,6 @@
 #include "packed_product.hpp"
 
 namespace dhx {
-namespace {
-
-template <class T, bool FOUR>
-hipError_t launch(const Product& p, hipStream_t s) {
-    return launch_tiles<T, FOUR, true, 64, 64, 32, 64, 4, 1>(p, s);
-}
-
-}  // namespace
 
 uint64_t packed_gated_bytes(const dhx_packed_gated& p) { return p.gate_scales ? quantised_rows_bytes(p.rows, p.inputs) : 0; }
 
@@ -37,13 +29,13 @@ hipError_t launch_packed_gated(const dhx_packed_gated& p, hipStream_t s) {
         a.ws_stride = p.scales_stride;
         const hipError_t err = quantise_rows(p.type, p.x, p.x_stride, p.rows, p.inputs, p.workspace, &a, s);
         if (err != hipSuccess) return err;
-        return p.type == DHX_F16 ? launch<half_t, true>(a, s) : launch<bf16_t, true>(a, s);
+        return p.type == DHX_F16 ? launch_product<half_t, true, true>(a, s) : launch_product<bf16_t, true, true>(a, s);
     }
     a.x = p.x;
     a.x_stride = p.x_stride * 2;
     a.w_stride = p.w_stride * 2;
     a.pieces = p.inputs / 8;
-    return p.type == DHX_F16 ? launch<half_t, false>(a, s) : launch<bf16_t, false>(a, s);
+    return p.type == DHX_F16 ? launch_product<half_t, false, true>(a, s) : launch_product<bf16_t, false, true>(a, s);
 }
 
 }  // namespace dhx

@@ -12,7 +12,8 @@
 
 namespace dhx {
 
-// What a launcher hands on; strides are in bytes but that of out.
+// What a launcher hands on; strides are in bytes but that of out. xs_stride: from 32
+// blocks' scales of all rows to the next 32's.
 struct Product {
     uint32_t type, activation, rows, pieces, outputs, sequences;
     const void *x, *w, *up;             // up: gated only
@@ -23,13 +24,13 @@ struct Product {
     uint64_t x_stride, w_stride, xs_stride, ws_stride, out_stride;
 };
 
-#define DHX_PRODUCT_PARAMS Addr x_, Addr w_, Addr up_, int rows, int pieces, int outputs, uint32_t x_stride, uint32_t w_stride, Addr starts_, Addr xs_, Addr ws_, Addr us_, Addr bias_, Addr up_bias_, Addr out_, uint64_t out_stride, int sequences, int activation, uint32_t xs_stride, uint32_t ws_stride
+#define DHX_PRODUCT_PARAMS Addr x_, Addr w_, Addr up_, int rows, int pieces, int outputs, uint32_t x_stride, uint32_t w_stride, Addr starts_, Addr xs_, Addr ws_, Addr us_, Addr bias_, Addr up_bias_, Addr out_, uint64_t out_stride, int sequences, int activation, uint64_t xs_stride, uint32_t ws_stride
 
 template <class K>
 hipError_t enqueue_product(K kernel, dim3 grid, dim3 block, hipStream_t s, const Product& p) {
     return enqueue(kernel, grid, block, 0, s, p.x, p.w, p.up, (int)p.rows, (int)p.pieces, (int)p.outputs, (uint32_t)p.x_stride,
                    (uint32_t)p.w_stride, p.starts, p.xs, p.ws, p.us, p.bias, p.up_bias, p.out, p.out_stride, (int)p.sequences,
-                   (int)p.activation, (uint32_t)p.xs_stride, (uint32_t)p.ws_stride);
+                   (int)p.activation, p.xs_stride, (uint32_t)p.ws_stride);
 }
 
 // --- device pieces ---------------------------------------------------------
@@ -49,13 +50,28 @@ __device__ __forceinline__ float16_t product32(uint4_t a, uint4_t b, float16_t c
     }
 }
 
+// The lane's number, from no register that would have to hold it.
+__device__ __forceinline__ int lane_anew() {
+    int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 template <int ACT>
 __device__ __forceinline__ float activated(float g) {
     // e^-g past the range of float32 is infinite, and its reciprocal 0.
     if constexpr (ACT == DHX_SILU) return g * fast_rcp(1.0f + fast_exp2(-kLog2e * g));
     if constexpr (ACT == DHX_SIGMOID) return fast_rcp(1.0f + fast_exp2(-kLog2e * g));
     if constexpr (ACT == DHX_RELU) return g < 0.0f ? 0.0f : g;  // NaN stays
-    if constexpr (ACT == DHX_GELU) return 0.5f * g * (1.0f + erff(0.70710678f * g));
+    if constexpr (ACT == DHX_GELU) {
+        // erfc(|x|), x = g / sqrt 2, by Abramowitz and Stegun's formula 7.1.26 (within 1.5e-7),
+        // and (1 + erf x) / 2 from it: no difference of near values where g is negative.
+        // (2299 rows, 1000 -> 2728 with 4-bit weights take 23.8 us with erff, 20.5 so.)
+        const float x = 0.70710678f * fabsf(g), t = fast_rcp(fmaf(0.3275911f, x, 1.0f));
+        const float p = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+        const float half = 0.5f * p * t * fast_exp2(-kLog2e * x * x);
+        return g * (g < 0.0f ? half : 1.0f - half);
+    }
     // (1 + tanh u) / 2 = 1 / (1 + e^-2u), 2 sqrt(2 / pi) = 1.5957691
     if constexpr (ACT == DHX_GELU_TANH) return g * fast_rcp(1.0f + fast_exp2(-kLog2e * 1.5957691f * fmaf(0.044715f * g * g, g, g)));
 }
@@ -76,25 +92,31 @@ __device__ __forceinline__ void with_activation(int activation, F f) {
 // so that a lane holds both sums of an output), waves of WM x WN each. NST stages
 // of 8 pieces in LDS, NST - 1 of them on their way while one is multiplied (a
 // variable each, so that the compiler can tell the stage that is read from those
-// being filled). A lane multiplies piece 4 (lane / 32) + kk in step kk: a block of 4
-// bits then finds its scale in byte kk of the half's own word of the row's 8.
-// Scales come 16 bytes per row at a time, for two stages.
+// being filled: one that may be both would make each read wait for all loads). A
+// lane multiplies piece 4 (lane / 32) + kk in step kk: a block of 4 bits then finds
+// its scale in byte kk of the half's own word of the row's 8. Scales come 32 bytes
+// per row at a time, for four stages, with the first of them (16 bytes at a time a
+// row's line would be asked for twice as often: 16384 rows, 4096 -> 4096, take 199 us
+// then, 190 so). Those of x lie [32 blocks][row][32], so that a load's rows are one piece.
 template <class T, bool FOUR, bool GATED, int BM, int BN, int WM, int WN, int NST, int PER_SIMD>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_product_kernel(DHX_PRODUCT_PARAMS) {
     typedef typename Num<T>::v8 v8;
     typedef typename Num<T>::v4 v4;
     constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES;
     constexpr int XL = BM / 8 / WAVES, WL = BN / 8 / WAVES;  // loads of 8 rows per wave and stage
-    constexpr int SCALE_LOADS = (BM + BN) / 64, SL = FOUR ? (SCALE_LOADS + WAVES - 1) / WAVES : 0;
+    constexpr int SCALE_LOADS = (BM + BN) / 32, SL = FOUR ? (SCALE_LOADS + WAVES - 1) / WAVES : 0;  // per wave and four stages
     constexpr int MB = WM / 32, NB = WN / 32, KK = 4;
+    // Turns of four stages end after two where those are the last, but in the largest
+    // tile (with four bits), whose registers do not fit then: up to three stages of zeros
+    // are multiplied there.
+    constexpr int TURNS = FOUR || NST == 4 ? 4 : 2;
+    constexpr bool BREAK = MB * NB < 8;
     constexpr int BO = GATED ? BN / 2 : BN;  // outputs of a tile
-    constexpr int RINGS = NST > 2 ? 3 : 2;   // of scales, each for two stages
-    static_assert(NST % 2 == 0, "a stage's half of its scales is a constant");
+    constexpr int WS = BM * 128, SS = WS + BN * 128, STAGE = SS + (FOUR ? (BM + BN) * 32 : 0);  // x, weights, scales
+    static_assert(NST == 2 || NST == 4, "which of two stages a buffer holds is a constant");
     static_assert(XL * 8 * WAVES == BM && WL * 8 * WAVES == BN && BM % 64 == 0 && BN % 64 == 0 && BN <= THREADS, "whole loads");
     static_assert(!GATED || NB % 2 == 0, "both sums of an output in one lane");
-    __shared__ __attribute__((aligned(16))) char sX0[BM * 128], sX1[BM * 128], sX2[NST > 2 ? BM * 128 : 16], sX3[NST > 2 ? BM * 128 : 16];
-    __shared__ __attribute__((aligned(16))) char sW0[BN * 128], sW1[BN * 128], sW2[NST > 2 ? BN * 128 : 16], sW3[NST > 2 ? BN * 128 : 16];
-    __shared__ __attribute__((aligned(16))) char sScale[FOUR ? RINGS * (BM + BN) * 16 : 16];
+    __shared__ __attribute__((aligned(16))) char s0[STAGE], s1[SS], s2[NST > 2 ? SS : 16], s3[NST > 2 ? SS : 16];
     __shared__ __attribute__((aligned(16))) float sBias[BN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // Tiles in XCD-contiguous order, four row blocks at a time, so that the tiles
@@ -112,164 +134,198 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
         end = start_at(starts_, sequences, rows);
         if (row0 >= end || row0 + BM <= first) return;
     }
-    const int steps = (pieces + 7) / 8, whole = pieces / 8;
-    const char* x0 = (const char*)x_ + (uint64_t)row0 * x_stride;
+    const int steps = (pieces + 7) / 8;
 
     // Weight row r of the tile: which matrix, and which of its rows.
     auto of_up = [&](int r) { return GATED && (r & 32) != 0; };
     auto column = [&](int r) { return GATED ? (r >> 6) * 32 + (r & 31) : r; };
-    const char *w0 = (const char*)w_ + (uint64_t)col0 * w_stride, *up0 = (const char*)up_ + (uint64_t)col0 * w_stride;
+    // Buffers of the tile's rows: a load's address is one register per lane and one
+    // of the wave, and a lane beyond the end fetches zeros. A wave loads rows of one
+    // of the matrices.
+    static_assert(32 % (WL * 8) == 0, "of gate or of up");
+    const int columns = min(BO, outputs - col0);
+    auto rows_of = [&](Addr base, int row, int n, uint32_t stride) {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base.a + (uint64_t)row * stride), 0, (int)((uint32_t)(n - 1) * stride + pieces * 16),
+                                                 kBufferRsrcWord3);
+    };
+    const __amdgpu_buffer_rsrc_t x_rows = rows_of(x_, row0, min(BM, rows - row0), x_stride);
+    const __amdgpu_buffer_rsrc_t w_rows = rows_of(of_up(wave * WL * 8) ? up_ : w_, col0, columns, w_stride);
 
     // Lane -> row lane / 8 of a load's 8, the piece that the swizzle puts at slot
     // lane % 8; rows behind the last one fetch that one.
     uint32_t xo[XL], wo[WL];
-    const int lr = lane >> 3, l32 = lane & 31, hi = lane >> 5;
-    auto chunk = [&](int r) { return (lane & 7) ^ slot_of<64>(r); };
+    const int l32 = lane & 31, hi = lane >> 5;
 #pragma unroll
     for (int j = 0; j < XL; ++j) {
-        const int r = (wave * XL + j) * 8 + lr;
-        xo[j] = (uint32_t)min(r, rows - 1 - row0) * x_stride + chunk(r) * 16;
+        const int r = (wave * XL + j) * 8 + (lane >> 3);
+        xo[j] = (uint32_t)min(r, rows - 1 - row0) * x_stride + ((lane & 7) ^ slot_of<64>(r)) * 16;
     }
 #pragma unroll
     for (int j = 0; j < WL; ++j) {
-        const int r = (wave * WL + j) * 8 + lr;
-        wo[j] = (uint32_t)min(column(r), outputs - 1 - col0) * w_stride + chunk(r) * 16;
+        const int r = (wave * WL + j) * 8 + (lane >> 3);
+        wo[j] = (uint32_t)min(column(r), columns - 1) * w_stride + ((lane & 7) ^ slot_of<64>(r)) * 16;
     }
-    auto w_base = [&](int j) { return of_up((wave * WL + j) * 8) ? up0 : w0; };
-    // A load of scales takes 64 rows, those of x first; with more waves than loads
-    // some are made twice, so that every wave has as many on their way.
+    // A load of scales takes the 32 bytes (four stages) of 32 rows, those of x first;
+    // with more waves than loads some are made twice, so that every wave has as many
+    // on their way. A row's halves change places every 8 rows, which spreads the reads
+    // over the banks.
     const char* so[SL > 0 ? SL : 1];
     int sto[SL > 0 ? SL : 1];
+    const int half = (lane & 1) ^ ((lane >> 4) & 1);
     if constexpr (FOUR) {
 #pragma unroll
         for (int j = 0; j < SL; ++j) {
-            const int load = (wave * SL + j) % SCALE_LOADS, r = load * 64 + lane;
+            const int load = (wave * SL + j) % SCALE_LOADS, r = load * 32 + (lane >> 1);
             sto[j] = load * 1024;
-            if (load * 64 < BM) {
-                so[j] = (const char*)xs_ + (uint64_t)(row0 + min(r, rows - 1 - row0)) * xs_stride;
+            if (r < BM) {
+                so[j] = (const char*)xs_ + (uint64_t)(row0 + min(r, rows - 1 - row0)) * 32 + half * 16;
             } else {
-                const int c = col0 + min(column(r - BM), outputs - 1 - col0);
-                so[j] = (of_up(r - BM) ? (const char*)us_ : (const char*)ws_) + (uint64_t)c * ws_stride;
+                const int c = col0 + min(column(r - BM), columns - 1);
+                so[j] = (of_up(r - BM) ? (const char*)us_ : (const char*)ws_) + (uint64_t)c * ws_stride + half * 16;
             }
         }
     }
-    auto move_scales = [&](int pair) __attribute__((always_inline)) {
+    auto move_scales = [&](int s) __attribute__((always_inline)) {
         if constexpr (FOUR) {
+            const int group = min(s, steps - 1) >> 2;
+            const bool there = group * 32 + half * 16 < pieces;  // a row of weights' may end between
 #pragma unroll
-            for (int j = 0; j < SL; ++j) dma16(so[j] + pair * 16, sScale + pair % RINGS * (BM + BN) * 16 + sto[j]);
+            for (int j = 0; j < SL; ++j) {
+                const uint64_t step = sto[j] < BM * 32 ? (uint64_t)group * xs_stride : (uint64_t)(group * 32);
+                dma16(there ? so[j] + step : (const char*)&kZeros, s0 + SS + sto[j]);
+            }
         }
     };
-    auto move_whole = [&](char* sx, char* sw, int s) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < XL; ++j) dma16(x0 + s * 128 + xo[j], sx + (wave * XL + j) * 1024);
-#pragma unroll
-        for (int j = 0; j < WL; ++j) dma16(w_base(j) + s * 128 + wo[j], sw + (wave * WL + j) * 1024);
+    auto buffer_load = [](const __amdgpu_buffer_rsrc_t& from, char* to, uint32_t lane_at, int at) __attribute__((always_inline)) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, (int)lane_at, at, 0, 0);
     };
-    auto move = [&](char* sx, char* sw, int s) __attribute__((always_inline)) {
-        if ((s & 1) == 0) move_scales(s >> 1);
-        if (s < whole) {
-            move_whole(sx, sw, s);
-            return;
-        }
-        const char* zeros = (const char*)&kZeros;
+    // Stage s, also the last one, whose pieces may not all exist, and stages behind
+    // it, which have none: such lanes pass the buffer's end and fetch zeros. (One code
+    // for all stages: with the tail apart its registers did not fit.) turn: s % 4, a
+    // constant.
+    static_assert(XL % 2 == 0 || XL == 1, "rows 16 apart have their pieces at the same slots");
+    auto chunk = [&](int j) { return (lane & 7) ^ slot_of<64>((j & 1) * 8 + (lane >> 3)); };
+    const int chunk_x = chunk(wave * XL), chunk_w = chunk(wave * WL);  // of a wave's even loads; bit 1 differs in odd ones
+    auto move = [&](char* to, int s, int turn) __attribute__((always_inline)) {
+        const int left = pieces - s * 8;
+        if (turn == 0) move_scales(s);
 #pragma unroll
-        for (int j = 0; j < XL; ++j) {
-            const bool in = s * 8 + chunk((wave * XL + j) * 8 + lr) < pieces;
-            dma16(in ? x0 + s * 128 + xo[j] : zeros, sx + (wave * XL + j) * 1024);
-        }
+        for (int j = 0; j < XL; ++j) buffer_load(x_rows, to + (wave * XL + j) * 1024, (chunk_x ^ (j & 1) * 2) < left ? xo[j] : ~15u, s * 128);
 #pragma unroll
-        for (int j = 0; j < WL; ++j) {
-            const bool in = s * 8 + chunk((wave * WL + j) * 8 + lr) < pieces;
-            dma16(in ? w_base(j) + s * 128 + wo[j] : zeros, sw + (wave * WL + j) * 1024);
-        }
+        for (int j = 0; j < WL; ++j) buffer_load(w_rows, to + WS + (wave * WL + j) * 1024, (chunk_w ^ (j & 1) * 2) < left ? wo[j] : ~15u, s * 128);
     };
 
     const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
     const int frag = l32 * 128 + (((hi * 4) ^ slot_of<64>(l32)) << 4);
     float16_t acc[MB][NB] = {};
     uint4_t fx[2][MB], fw[2][NB];
-    uint32_t scale_x[2][MB], scale_w[2][NB];  // of even and odd stages
-    auto load = [&](const char* sx, const char* sw, int kk, int set) __attribute__((always_inline)) {
+    auto load = [&](const char* from, int kk, int set) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) fx[set][i] = *(const uint4_t*)(sx + (wm + i * 32) * 128 + (frag ^ (kk << 4)));
+        for (int i = 0; i < MB; ++i) fx[set][i] = *(const uint4_t*)(from + (wm + i * 32) * 128 + (frag ^ (kk << 4)));
 #pragma unroll
-        for (int i = 0; i < NB; ++i) fw[set][i] = *(const uint4_t*)(sw + (wn + i * 32) * 128 + (frag ^ (kk << 4)));
+        for (int i = 0; i < NB; ++i) fw[set][i] = *(const uint4_t*)(from + WS + (wn + i * 32) * 128 + (frag ^ (kk << 4)));
     };
-    auto load_scales = [&](int s, int odd) __attribute__((always_inline)) {
-        if constexpr (FOUR) {
-            const char* from = sScale + (s >> 1) % RINGS * (BM + BN) * 16 + odd * 8 + l32 * 16 + hi * 4;
-            // Behind the last piece there are no scales (and zeros for values).
-            const int left = pieces - s * 8 - hi * 4;
-            const uint32_t mask = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+    // The scales of stage s: two stages in a ring take them from LDS stage by stage,
+    // four take those of four stages at once, since their place is filled anew before
+    // the last of them. Their places are kept from the compiler, which would read two
+    // at once: such a read, unlike the others, it lets wait for all loads.
+    constexpr int SETS = NST == 2 ? 2 : 4;
+    uint32_t scale_x[SETS][MB], scale_w[SETS][NB];
+    int scale_at[MB + NB];
+    if constexpr (FOUR) {
 #pragma unroll
-            for (int i = 0; i < MB; ++i) scale_x[odd][i] = *(const uint32_t*)(from + (wm + i * 32) * 16) & mask;
+        for (int i = 0; i < MB + NB; ++i) {
+            scale_at[i] = SS + ((i < MB ? wm + i * 32 : BM + wn + (i - MB) * 32) + l32) * 32 + ((lane >> 3) & 1) * 16 + (NST == 2 ? hi * 4 : 0);
+            asm volatile("" : "+v"(scale_at[i]));
+        }
+    }
+    // Behind the last piece there are no scales (and zeros for values).
+    auto scale_mask = [&](int s) __attribute__((always_inline)) {
+        const int left = pieces - s * 8 - hi * 4;
+        return left >= 4 ? ~0u : (1u << (8 * max(left, 0))) - 1;
+    };
+    auto put_scale = [&](int i, int set, uint32_t v) __attribute__((always_inline)) {
+        if (i < MB) scale_x[set][i] = v;
+        else scale_w[set][i - MB] = v;
+    };
+    auto load_scales = [&](int s, int turn) __attribute__((always_inline)) {
+        if constexpr (FOUR && NST == 2) {
+            const uint32_t mask = scale_mask(s);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) scale_w[odd][i] = *(const uint32_t*)(from + (BM + wn + i * 32) * 16) & mask;
+            for (int i = 0; i < MB + NB; ++i)
+                put_scale(i, turn & 1, *(const uint32_t*)(s0 + (scale_at[i] ^ ((turn & 2) * 8)) + (turn & 1) * 8) & mask);
+        }
+        if constexpr (FOUR && NST == 4) {
+#pragma unroll
+            for (int i = 0; i < MB + NB; ++i)
+#pragma unroll
+                for (int pair = 0; pair < 2; ++pair) {
+                    const uint4_t v = *(const uint4_t*)(s0 + (scale_at[i] ^ (pair * 16)));
+                    put_scale(i, 2 * pair, (hi ? v[1] : v[0]) & scale_mask(s + 2 * pair));
+                    put_scale(i, 2 * pair + 1, (hi ? v[3] : v[2]) & scale_mask(s + 2 * pair + 1));
+                }
         }
     };
-    auto multiply = [&](auto kk, int set, int odd) __attribute__((always_inline)) {
+    auto multiply = [&](auto kk, int set, int scales) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
             for (int k = 0; k < NB; ++k)
-                acc[i][k] = product32<T, FOUR, decltype(kk)::value>(fw[set][k], fx[set][i], acc[i][k], FOUR ? scale_w[odd][k] : 0, FOUR ? scale_x[odd][i] : 0);
+                acc[i][k] = product32<T, FOUR, decltype(kk)::value>(fw[set][k], fx[set][i], acc[i][k], FOUR ? scale_w[scales][k] : 0, FOUR ? scale_x[scales][i] : 0);
     };
-    move(sX0, sW0, 0);
+    move(s0, 0, 0);
     if (tid < BN) {
         const float* bias = of_up(tid) ? up_bias_ : bias_;
         sBias[tid] = bias && col0 + column(tid) < outputs ? bias[col0 + column(tid)] : 0.f;
     }
-    if (NST > 2 && steps > 1) move(sX1, sW1, 1);
-    if (NST > 2 && steps > 2) move(sX2, sW2, 2);
+    if constexpr (NST > 2) {
+        move(s1, 1, 1);
+        move(s2, 2, 0);
+    }
     // Opens stage s: it has landed (the NST - 2 stages behind it may be on their way,
-    // one of them with scales), and every wave has read the one before, whose place
-    // stage s + NST - 1 takes.
-    auto open = [&](auto fast, char* free_x, char* free_w, int s) __attribute__((always_inline)) {
-        if (fast || s + NST - 2 < steps) wait_vm<(NST - 2) * (XL + WL) + (NST > 2 ? SL : 0)>();
-        else wait_vm<0>();
+    // with their scales), and every wave has read the one before, whose place stage
+    // s + NST - 1 takes. turn: s % 4, a constant.
+    auto open = [&](auto turn, char* free, int s) __attribute__((always_inline)) {
+        constexpr int TURN = decltype(turn)::value;
+        wait_vm<(NST - 2) * (XL + WL) + (NST == 4 && TURN >= 2 ? SL : 0)>();
         wait_lgkm();
         barrier();
-        const int next = s + NST - 1;
-        if constexpr (fast) {
-            if ((next & 1) == 0) move_scales(next >> 1);
-            move_whole(free_x, free_w, next);
-        } else if (next < steps) {
-            move(free_x, free_w, next);
-        }
+        move(free, s + NST - 1, (TURN + NST - 1) & 3);
     };
-    auto step = [&](auto fast, char* sx, char* sw, const char* next_x, const char* next_w, int s, int odd) __attribute__((always_inline)) {
+    // Multiplies a stage; the next one's first fragments are on their way under the
+    // last products.
+    auto step = [&](auto turn, char* now, const char* next, int s) __attribute__((always_inline)) {
+        constexpr int TURN = decltype(turn)::value, SET = NST == 2 ? TURN & 1 : TURN, NEXT = (TURN + 1) & 3;
         auto inner = [&](auto kk) __attribute__((always_inline)) {
-            load(sx, sw, kk + 1, (kk + 1) & 1);
+            load(now, kk + 1, (kk + 1) & 1);
+            if (NST == 2 && kk == 0 && (TURN & 1) == 0) load_scales(s + 1, TURN + 1);
             __builtin_amdgcn_sched_barrier(0);  // the reads go ahead of the products they pass under
-            multiply(kk, kk & 1, odd);
+            multiply(kk, kk & 1, SET);
             __builtin_amdgcn_sched_barrier(0);
         };
         inner(std::integral_constant<int, 0>{});
         inner(std::integral_constant<int, 1>{});
         inner(std::integral_constant<int, 2>{});
-        if (fast || s + 1 < steps) {
-            open(fast, sx, sw, s + 1);
-            load(next_x, next_w, 0, 0);
-            load_scales(s + 1, 1 - odd);
-        }
+        open(std::integral_constant<int, NEXT>{}, now, s + 1);
+        load(next, 0, 0);
+        if (NST == 2 && (TURN & 1) == 1) load_scales(s + 1, NEXT);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 3>{}, 1, odd);
+        multiply(std::integral_constant<int, 3>{}, 1, SET);
+        if (NST == 4 && TURN == 3) load_scales(s + 1, 0);
     };
-    open(std::false_type{}, NST == 2 ? sX1 : sX3, NST == 2 ? sW1 : sW3, 0);
-    load(sX0, sW0, 0, 0);
+    open(std::integral_constant<int, 0>{}, NST == 2 ? s1 : s3, 0);
+    load(s0, 0, 0);
     load_scales(0, 0);
-    int s = 0;
-    auto turn_of_stages = [&](auto fast) __attribute__((always_inline)) {
-        step(fast, sX0, sW0, sX1, sW1, s, 0);
-        if (fast || s + 1 < steps) step(fast, sX1, sW1, NST > 2 ? sX2 : sX0, NST > 2 ? sW2 : sW0, s + 1, 1);
-        if constexpr (NST > 2) {
-            if (fast || s + 2 < steps) step(fast, sX2, sW2, sX3, sW3, s + 2, 0);
-            if (fast || s + 3 < steps) step(fast, sX3, sW3, sX0, sW0, s + 3, 1);
+    for (int s = 0; s < steps; s += TURNS) {  // an odd number of stages: one of zeros behind them
+        step(std::integral_constant<int, 0>{}, s0, s1, s);
+        step(std::integral_constant<int, 1>{}, s1, NST > 2 ? s2 : s0, s + 1);
+        if constexpr (TURNS > 2) {
+            if (BREAK && s + 2 >= steps) break;
+            step(std::integral_constant<int, 2>{}, NST > 2 ? s2 : s0, NST > 2 ? s3 : s1, s + 2);
+            step(std::integral_constant<int, 3>{}, NST > 2 ? s3 : s1, s0, s + 3);
         }
-        s += NST;
-    };
-    while (s + 2 * NST <= whole) turn_of_stages(std::true_type{});
-    while (s < steps) turn_of_stages(std::false_type{});
+    }
+    wait_vm<0>();  // no load may come when the LDS is another workgroup's
 
     // Lane: row l32 of a block, columns 8 g + 4 hi .. +3 of its 32 in register group
     // g; both halves exchange groups, so that each stores 8 columns at once.
@@ -324,6 +380,41 @@ hipError_t launch_tiles(const Product& p, hipStream_t s) {
     const uint64_t total = ((uint64_t)p.rows + BM - 1) / BM * ((p.outputs + BO - 1) / BO);
     return enqueue_product(packed_product_kernel<T, FOUR, GATED, BM, BN, WM, WN, NST, PER_SIMD>, dim3((unsigned)((total + 7) / 8 * 8)),
                            dim3(64 * (BM / WM) * (BN / WN)), s, p);
+}
+
+// The tile of a call, from the number of workgroups that each would make and the
+// number of its stages. us on MI355X (two of 128 x 128 or smaller tiles run on a CU, one
+// of 256 x 256 and of those with four stages; products with 4-bit weights hold the
+// launch that quantises x):
+// - 256 x 256 where they fill the CUs once or in rounds of which the last is not
+//   mostly empty: gated, 4096 -> 8192, 1024 rows (256 tiles) 116, 128 x 128 148; 512 rows
+//   (128 tiles) 98 and 77; 1024 -> 2728, 2048 rows (176) 27.4 and 30.5, 4096 rows (352)
+//   55.9 and 51.8; 384 -> 1536, 12864 rows (612) 46.7 and 45.8; four bits, two stages
+//   (384 -> 1536, 4096 rows) 17.4 and 15.1;
+// - long rows and a CU for every tile: four stages in flight, of the smallest such tile:
+//   gated, 4096 -> 8192, 48 rows, 64 x 64 34.1 (two stages 49.9), 128 rows, 128 x 64 38.9
+//   (55.6), 256 rows, 128 x 128 49.4 (60.8; four bits 20.8 and 19.2); short rows gain
+//   nothing (384 -> 1536, 256 rows, 4.8 and 4.4);
+// - else the smallest of which two rounds run at once: linear, four bits, 1024 -> 1024,
+//   2048 rows, 64 x 64 8.9, 128 x 128 9.8, 4096 rows 12.2 and 11.9; gated, 384 -> 1536,
+//   1024 rows, 64 x 64 7.0, 128 x 64 6.4, 2048 rows 13.3, 10.2 and (128 x 128) 10.1.
+template <class T, bool FOUR, bool GATED>
+hipError_t launch_product(const Product& p, hipStream_t s) {
+    auto count = [&](uint64_t m, uint64_t n) { return (p.rows + m - 1) / m * ((p.outputs + n - 1) / n) * (GATED ? 2 : 1); };
+    const uint64_t largest = (p.rows + 255ull) / 256 * ((p.outputs + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+    const uint32_t steps = (p.pieces + 7) / 8;
+    constexpr int WM = GATED ? 32 : 64, WN = GATED ? 64 : 32;  // of a 128 x 64 tile: a wave of the gated one holds both sums
+    const bool fills = largest <= 256 ? largest >= 160 : largest * 20 >= (largest + 255) / 256 * 256 * 17;
+    if (fills && (!FOUR || steps > 2)) return launch_tiles<T, FOUR, GATED, 256, 256, 128, 64, 2, 2>(p, s);
+    if (steps >= 12) {
+        if (count(64, 64) <= 256) return launch_tiles<T, FOUR, GATED, 64, 64, 32, GATED ? 64 : 32, 4, GATED ? 1 : 2>(p, s);
+        if (count(128, 64) <= 256) return launch_tiles<T, FOUR, GATED, 128, 64, WM, WN, 4, 1>(p, s);
+        if constexpr (!FOUR)
+            if (count(128, 128) <= 256) return launch_tiles<T, FOUR, GATED, 128, 128, 64, 64, 4, 1>(p, s);
+    }
+    if (count(64, 64) <= 512) return launch_tiles<T, FOUR, GATED, 64, 64, 32, GATED ? 64 : 32, 2, GATED ? 2 : 4>(p, s);
+    if (count(128, 64) <= 512) return launch_tiles<T, FOUR, GATED, 128, 64, WM, WN, 2, 2>(p, s);
+    return launch_tiles<T, FOUR, GATED, 128, 128, 64, 64, 2, 2>(p, s);
 }
 
 // x of a call, quantised into its workspace (codes, then scales) on the stream: the

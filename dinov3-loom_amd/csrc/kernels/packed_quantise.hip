@@ -9,7 +9,7 @@
 namespace dhx {
 namespace {
 
-#define DHX_QUANTISE_PARAMS Addr x_, Addr codes_, Addr scales_, int rows, int columns, uint64_t x_stride, uint64_t codes_stride, uint64_t scales_stride, Addr starts_, int sequences, int block_rows
+#define DHX_QUANTISE_PARAMS Addr x_, Addr codes_, Addr scales_, int rows, int columns, uint64_t x_stride, uint64_t codes_stride, uint64_t scales_stride, uint64_t group_stride, Addr starts_, int sequences, int block_rows
 
 // The float whose exponent is scale byte b's (what the conversions take).
 __device__ __forceinline__ float scale_of(uint32_t b) { return __builtin_bit_cast(float, b << 23); }
@@ -67,7 +67,10 @@ __global__ __launch_bounds__(256) void packed_quantise_kernel(DHX_QUANTISE_PARAM
             c = two_codes<3>(c, v2{v[6], v[7]}, scale);
             if (!in) continue;
             if (piece < blocks * 4) *(uint32_t*)((char*)codes_ + row * codes_stride + piece * 4) = odd ? 0 : c;
-            if ((piece & 3) == 0) *((uint8_t*)scales_ + row * scales_stride + (piece >> 2)) = piece < blocks * 4 ? (uint8_t)byte : 0;
+            if ((piece & 3) == 0) {
+                const int b = piece >> 2;
+                *((uint8_t*)scales_ + (b >> 5) * group_stride + row * scales_stride + (b & 31)) = b < blocks ? (uint8_t)byte : 0;
+            }
         }
     }
 }
@@ -99,23 +102,25 @@ __global__ __launch_bounds__(256) void packed_dequantise_kernel(DHX_QUANTISE_PAR
 constexpr uint64_t kMostBlocks = 1u << 21;  // a launch has fewer than 2^32 threads; workgroups take further rows in turn
 
 template <class K>
-hipError_t launch(K kernel, const dhx_packed_quantisation& p, uint64_t per_row, hipStream_t s) {
+hipError_t launch(K kernel, const dhx_packed_quantisation& p, uint64_t group_stride, uint64_t per_row, hipStream_t s) {
     const int block_rows = (int)std::max<uint64_t>(256 / per_row, 1);
     const uint64_t blocks = std::min<uint64_t>((p.rows + block_rows - 1) / block_rows, kMostBlocks);
     return enqueue(kernel, dim3((unsigned)blocks), dim3(256), 0, s, p.x, p.codes, p.scales, (int)p.rows, (int)p.columns, p.x_stride,
-                   p.codes_stride, p.scales_stride, p.starts, (int)p.sequences, block_rows);
+                   p.codes_stride, p.scales_stride, group_stride, p.starts, (int)p.sequences, block_rows);
 }
 
 }  // namespace
 
-hipError_t launch_packed_quantise(const dhx_packed_quantisation& p, hipStream_t s) {
+hipError_t launch_packed_quantise(const dhx_packed_quantisation& p, hipStream_t s, uint64_t group_stride) {
     const uint64_t per_row = scale_bytes(p.columns) * 4;
-    return p.type == DHX_F16 ? launch(packed_quantise_kernel<half_t>, p, per_row, s) : launch(packed_quantise_kernel<bf16_t>, p, per_row, s);
+    return p.type == DHX_F16 ? launch(packed_quantise_kernel<half_t>, p, group_stride, per_row, s)
+                             : launch(packed_quantise_kernel<bf16_t>, p, group_stride, per_row, s);
 }
 
 hipError_t launch_packed_dequantise(const dhx_packed_quantisation& p, hipStream_t s) {
     const uint64_t per_row = p.columns / 8;
-    return p.type == DHX_F16 ? launch(packed_dequantise_kernel<half_t>, p, per_row, s) : launch(packed_dequantise_kernel<bf16_t>, p, per_row, s);
+    return p.type == DHX_F16 ? launch(packed_dequantise_kernel<half_t>, p, 32, per_row, s)
+                             : launch(packed_dequantise_kernel<bf16_t>, p, 32, per_row, s);
 }
 
 }  // namespace dhx

@@ -4,16 +4,9 @@
 #include "packed_product.hpp"
 
 namespace dhx {
-namespace {
 
-template <class T>
-hipError_t launch(const Product& p, hipStream_t s) {
-    return launch_tiles<T, true, false, 64, 64, 32, 32, 4, 2>(p, s);
-}
-
-}  // namespace
-
-uint64_t quantised_rows_bytes(uint64_t rows, uint64_t columns) { return rows * (code_bytes(columns) + scale_bytes(columns)); }
+// Scales as the product reads them, [32 blocks][row][32].
+uint64_t quantised_rows_bytes(uint64_t rows, uint64_t columns) { return rows * (code_bytes(columns) + (blocks_of(columns) + 31) / 32 * 32); }
 
 hipError_t quantise_rows(uint32_t type, const void* x, uint64_t x_stride, uint64_t rows, uint32_t columns, void* workspace, Product* product,
                          hipStream_t s) {
@@ -26,13 +19,13 @@ hipError_t quantise_rows(uint32_t type, const void* x, uint64_t x_stride, uint64
     q.codes = static_cast<uint8_t*>(workspace);
     q.codes_stride = code_bytes(columns);
     q.scales = q.codes + rows * q.codes_stride;
-    q.scales_stride = scale_bytes(columns);
+    q.scales_stride = 32;
     product->x = q.codes;
     product->x_stride = q.codes_stride;
     product->xs = q.scales;
-    product->xs_stride = q.scales_stride;
+    product->xs_stride = rows * 32;
     product->pieces = (uint32_t)blocks_of(columns);
-    return launch_packed_quantise(q, s);
+    return launch_packed_quantise(q, s, rows * 32);
 }
 
 uint64_t packed_quantised_linear_bytes(const dhx_packed_quantised_linear& p) { return quantised_rows_bytes(p.rows, p.inputs); }
@@ -53,7 +46,7 @@ hipError_t launch_packed_quantised_linear(const dhx_packed_quantised_linear& p, 
     a.out_stride = p.y_stride;
     const hipError_t err = quantise_rows(p.type, p.x, p.x_stride, p.rows, p.inputs, p.workspace, &a, s);
     if (err != hipSuccess) return err;
-    return p.type == DHX_F16 ? launch<half_t>(a, s) : launch<bf16_t>(a, s);
+    return p.type == DHX_F16 ? launch_product<half_t, true, false>(a, s) : launch_product<bf16_t, true, false>(a, s);
 }
 
 }  // namespace dhx

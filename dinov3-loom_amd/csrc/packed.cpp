@@ -255,7 +255,7 @@ void product_sizes(uint32_t type, uint64_t rows, uint32_t inputs, uint32_t outpu
     eights(outputs, "outputs");
     most(inputs, kMaxStride, "inputs");
     most(outputs, kMaxStride, "outputs");
-    most(((rows + 255) / 256) * ((outputs + 127) / 128), kMaxLinearTiles, "the number of tiles of 256 x 128 outputs");
+    most(((rows + 255) / 256) * ((outputs + 127) / 128), kMaxLinearTiles / 2, "the number of tiles of 256 x 128 outputs");
 }
 
 void quantised_linear_sizes(const dhx_packed_quantised_linear& p) { product_sizes(p.type, p.rows, p.inputs, p.outputs); }
@@ -417,7 +417,7 @@ int dhx_packed_quantise_run(dhx_engine* e, const dhx_packed_quantisation* p, voi
             quantisation_check(a);
             return a.rows > 0;
         },
-        dhx::launch_packed_quantise);
+        [](const dhx_packed_quantisation& a, hipStream_t s) { return dhx::launch_packed_quantise(a, s); });
 }
 
 int dhx_packed_dequantise_run(dhx_engine* e, const dhx_packed_quantisation* p, void* stream) {
