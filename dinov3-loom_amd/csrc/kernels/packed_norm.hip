@@ -16,7 +16,7 @@ namespace {
 
 // The sum of v over the G lanes (G <= 64: of a wave, else of the workgroup) that
 // hold a row, in all of them, by the same tree in each: inside rows of 16 lanes by
-// moves between lanes, then across them. part: a float per wave.
+// moves between lanes (G at least 8), then across them. part: a float per wave.
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* part) {
     auto move = [](float a, auto ctrl) {
@@ -25,11 +25,9 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
     v += move(v, std::integral_constant<int, 0xb1>{});   // quad_perm 1, 0, 3, 2
     v += move(v, std::integral_constant<int, 0x4e>{});   // quad_perm 2, 3, 0, 1
     v += move(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
-    v += move(v, std::integral_constant<int, 0x140>{});  // row_mirror
-    if constexpr (G >= 64) {
-        v += __shfl_xor(v, 16);
-        v = half_pair_sum(v);
-    }
+    if constexpr (G >= 16) v += move(v, std::integral_constant<int, 0x140>{});  // row_mirror
+    if constexpr (G >= 32) v += __shfl_xor(v, 16);
+    if constexpr (G >= 64) v = half_pair_sum(v);
     if constexpr (G > 64) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         if (lane == 0) part[wave] = v;
@@ -87,22 +85,21 @@ __device__ __forceinline__ void store8(S* p, const float (&v)[8]) {
     }
 }
 
-// v[p] times (product) or plus a channel vector's piece, where there is one.
-template <bool PRODUCT>
-__device__ __forceinline__ void with_vector(const float* vector, int c, float (&v)[8]) {
-    if (!vector) return;
-    float w[8];
-    load8(vector + c, w);
+// A channel vector's piece; ones or zeros where there is no vector.
+__device__ __forceinline__ void vector8(const float* vector, int c, float none, float (&v)[8]) {
+    if (vector) {
+        load8(vector + c, v);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = PRODUCT ? v[e] * w[e] : v[e] + w[e];
+        for (int e = 0; e < 8; ++e) v[e] = none;
+    }
 }
 
-// One norm of the row whose P pieces of 8 channels a lane holds (zeros where a
-// piece does not exist). The mean first, then the sum of squared deviations from
-// it, both from registers. part: 2 G / 64 floats, taken in turn.
+// One over the row's root of its mean square, of P pieces of 8 channels a lane
+// (zeros where a piece does not exist); for LayerNorm of the deviations from the
+// mean, which it leaves in v. Both sums are of registers. part: 2 G / 64 floats.
 template <int G, int P>
-__device__ __forceinline__ void normalise(float (&v)[P][8], const bool (&there)[P], const int (&at)[P], int kind, float eps, int channels,
-                                          const float* weight, const float* bias, float* part) {
+__device__ __forceinline__ float inverse(float (&v)[P][8], const bool (&there)[P], int kind, float eps, int channels, float* part) {
     const float each = 1.0f / (float)channels;
     if (kind == DHX_NORM_LAYER) {
         float sum = 0.f;
@@ -121,16 +118,7 @@ __device__ __forceinline__ void normalise(float (&v)[P][8], const bool (&there)[
     for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(v[p][e], v[p][e], sum);
-    const float scale = rsqrtf(fmaf(row_sum<G>(sum, part + (G > 64 ? G / 64 : 0)), each, eps));
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[p][e] *= scale;
-        if (there[p]) {
-            with_vector<true>(weight, at[p], v[p]);
-            with_vector<false>(bias, at[p], v[p]);
-        }
-    }
+    return rsqrtf(fmaf(row_sum<G>(sum, part + (G > 64 ? G / 64 : 0)), each, eps));
 }
 
 // T: y and h, S: x and x'. G lanes hold a row, P pieces of 8 channels each: piece p
@@ -171,23 +159,52 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void packed_norm_kernel(DHX_NORM
                 if (y) load8(y + row * y_stride + at[p], z[p]);
             }
         }
+        // x' = x + (y' r) by + plus
+        auto step_vectors = [&](int p, float (&by)[8], float (&plus)[8]) __attribute__((always_inline)) {
+            const int c = there[p] ? at[p] : 0;
+            float scale[8], gate[8];
+            vector8(post_weight_, c, 1.f, by);
+            vector8(post_bias_, c, 0.f, plus);
+            vector8(scale_, c, 1.f, scale);
+            vector8(gate_.a ? (const float*)gate_ + max(s, 0) * gate_stride : nullptr, c, 1.f, gate);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                scale[e] *= gate[e];
+                by[e] *= scale[e];
+                plus[e] *= scale[e];
+            }
+        };
+        auto pre_vectors = [&](int p, float (&by)[8], float (&plus)[8]) __attribute__((always_inline)) {
+            const int c = there[p] ? at[p] : 0;
+            vector8(pre_weight_, c, 1.f, by);
+            vector8(pre_bias_, c, 0.f, plus);
+        };
+        // With one piece per lane the vectors are loaded in front of the first sum, so that
+        // one latency is waited for; those of more pieces would not fit in registers.
+        float by[8], plus[8], pre_by[8], pre_plus[8];
+        if constexpr (P == 1) {
+            if (y) step_vectors(0, by, plus);
+            if (pre != DHX_NORM_NONE) pre_vectors(0, pre_by, pre_plus);
+        }
         if (y) {
-            if (post != DHX_NORM_NONE) normalise<G, P>(z, there, at, post, post_eps, channels, post_weight_, post_bias_, part);
+            const float r = post != DHX_NORM_NONE ? inverse<G, P>(z, there, post, post_eps, channels, part) : 1.f;
 #pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (in && there[p]) {
-                    with_vector<true>(scale_, at[p], z[p]);
-                    if (gate_.a) with_vector<true>((const float*)gate_ + s * gate_stride, at[p], z[p]);
+            for (int p = 0; p < P; ++p) {
+                if constexpr (P > 1) step_vectors(p, by, plus);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[p][e] += z[p][e];
-                    store8((S*)x_out_ + row * x_out_stride + at[p], v[p]);
-                }
+                for (int e = 0; e < 8; ++e) v[p][e] = there[p] ? v[p][e] + fmaf(z[p][e] * r, by[e], plus[e]) : 0.f;
+                if (in && there[p]) store8((S*)x_out_ + row * x_out_stride + at[p], v[p]);
+            }
         }
         if (pre != DHX_NORM_NONE) {
-            normalise<G, P>(v, there, at, pre, pre_eps, channels, pre_weight_, pre_bias_, part + (G > 64 ? 2 * G / 64 : 0));
+            const float r = inverse<G, P>(v, there, pre, pre_eps, channels, part + (G > 64 ? 2 * G / 64 : 0));
 #pragma unroll
-            for (int p = 0; p < P; ++p)
+            for (int p = 0; p < P; ++p) {
+                if constexpr (P > 1) pre_vectors(p, pre_by, pre_plus);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[p][e] = fmaf(v[p][e] * r, pre_by[e], pre_plus[e]);
                 if (in && there[p]) store8((T*)h_ + row * h_stride + at[p], v[p]);
+            }
         }
         if (G > 64) __syncthreads();  // part, for the next row
     }
@@ -208,10 +225,18 @@ hipError_t launch(const dhx_packed_norm& p, hipStream_t s) {
 template <class T, class S>
 hipError_t launch_pieces(const dhx_packed_norm& p, hipStream_t s) {
     const uint32_t pieces = p.channels / 8;
+    // A lane per piece, and as few lanes as that leaves idle: 39 MB of 384 channels, 64
+    // lanes 11.1 us, 32 lanes of two pieces 13.2, 128 lanes 18.4; of 2048, 256 lanes
+    // 11.3, 128 of two 11.5, 64 of four 19.5, 512 lanes 15.2.
+    if (pieces <= 8) return launch<T, S, 8, 1>(p, s);
     if (pieces <= 16) return launch<T, S, 16, 1>(p, s);
-    if (pieces <= 64) return launch<T, S, 16, 4>(p, s);
-    if (pieces <= 256) return launch<T, S, 64, 4>(p, s);
-    if (pieces <= 1024) return launch<T, S, 256, 4>(p, s);
+    if (pieces <= 32) return launch<T, S, 32, 1>(p, s);
+    if (pieces <= 64) return launch<T, S, 64, 1>(p, s);
+    if (pieces <= 128) return launch<T, S, 128, 1>(p, s);
+    if (pieces <= 256) return launch<T, S, 256, 1>(p, s);
+    if (pieces <= 512) return launch<T, S, 512, 1>(p, s);
+    if (pieces <= 1024) return launch<T, S, 1024, 1>(p, s);
+    if (pieces <= 2048) return launch<T, S, 1024, 2>(p, s);
     return launch<T, S, 1024, 4>(p, s);
 }
 
