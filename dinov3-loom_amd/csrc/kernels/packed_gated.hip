@@ -1,12 +1,15 @@
 // The gated projections of a feed-forward block on packed batches
 // (include/dinov3_packed.h): out = act(x Wg^T + bg) (x Wu^T + bu), one product
 // kernel whose tiles hold rows of both matrices (packed_product.hpp), with weights in
-// 16 bits, or in 4 behind the kernel that quantises x (packed_quantise.hip).
+// 16 bits, or in 4 behind the kernel that quantises x (packed_quantise.hip); few rows
+// against 4 bits have a kernel that does both.
 #include "packed_product.hpp"
 
 namespace dhx {
 
-uint64_t packed_gated_bytes(const dhx_packed_gated& p) { return p.gate_scales ? quantised_rows_bytes(p.rows, p.inputs) : 0; }
+uint64_t packed_gated_bytes(const dhx_packed_gated& p) {
+    return p.gate_scales && !few_product(p.rows, p.inputs, p.outputs) ? quantised_rows_bytes(p.rows, p.inputs) : 0;
+}
 
 hipError_t launch_packed_gated(const dhx_packed_gated& p, hipStream_t s) {
     Product a{};
@@ -27,6 +30,12 @@ hipError_t launch_packed_gated(const dhx_packed_gated& p, hipStream_t s) {
         a.us = p.up_scales;
         a.w_stride = p.w_stride;
         a.ws_stride = p.scales_stride;
+        if (few_product(p.rows, p.inputs, p.outputs)) {
+        a.x = p.x;
+        a.x_stride = p.x_stride * 2;
+        a.pieces = p.inputs;
+        return p.type == DHX_F16 ? launch_few_rows<half_t, true>(a, s) : launch_few_rows<bf16_t, true>(a, s);
+    }
         const hipError_t err = quantise_rows(p.type, p.x, p.x_stride, p.rows, p.inputs, p.workspace, &a, s);
         if (err != hipSuccess) return err;
         return p.type == DHX_F16 ? launch_product<half_t, true, true>(a, s) : launch_product<bf16_t, true, true>(a, s);

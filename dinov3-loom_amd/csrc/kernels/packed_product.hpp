@@ -7,8 +7,9 @@
 // lane of each side.
 #pragma once
 #include <type_traits>
+#include <algorithm>
 
-#include "packed.hpp"
+#include "packed_four.hpp"
 
 namespace dhx {
 
@@ -48,6 +49,12 @@ __device__ __forceinline__ float16_t product32(uint4_t a, uint4_t b, float16_t c
         typedef typename Num<T>::v8 v8;
         return Num<T>::mfma(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c);
     }
+}
+
+// The same with 16 x 16 outputs, of 4 bits; the scale is a word's lowest byte.
+__device__ __forceinline__ float4_t product16(uint4_t a, uint4_t b, float4_t c, uint32_t a_scale, uint32_t b_scale) {
+    const int8v_t wide_a = {(int)a[0], (int)a[1], (int)a[2], (int)a[3]}, wide_b = {(int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide_a, wide_b, c, 4, 4, 0, (int)a_scale, 0, (int)b_scale);
 }
 
 // The lane's number, from no register that would have to hold it.
@@ -380,6 +387,160 @@ hipError_t launch_tiles(const Product& p, hipStream_t s) {
     const uint64_t total = ((uint64_t)p.rows + BM - 1) / BM * ((p.outputs + BO - 1) / BO);
     return enqueue_product(packed_product_kernel<T, FOUR, GATED, BM, BN, WM, WN, NST, PER_SIMD>, dim3((unsigned)((total + 7) / 8 * 8)),
                            dim3(64 * (BM / WM) * (BN / WN)), s, p);
+}
+
+// Few rows against 4-bit weights, which are all there is to read: a workgroup takes
+// 16 outputs at a time (gated: and both of their sums) and all rows (16 XB of them), its
+// waves share the columns out in steps of QUADS * 4 blocks and join their sums in LDS.
+// Weights go straight into registers; a wave quantises its own columns of x into its
+// own LDS while they are on their way, so that one launch does it all. Where every wave
+// has no more than one step, a workgroup takes further outputs with the x it has.
+#define DHX_FEW_PARAMS Addr x_, Addr w_, Addr up_, int rows, int inputs, int outputs, uint32_t x_stride, uint32_t w_stride, Addr starts_, Addr ws_, Addr us_, Addr bias_, Addr up_bias_, Addr out_, uint64_t out_stride, int sequences, int activation, uint32_t ws_stride
+
+constexpr int kFewProductWaves = 8;
+template <class T, bool GATED, int XB, int QUADS>
+__global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kernel(DHX_FEW_PARAMS) {
+    typedef typename Num<T>::v8 v8;
+    constexpr int AB = GATED ? 2 : 1, ROWS = 16 * XB, WAVES = kFewProductWaves;
+    constexpr int LANES = 16 * QUADS, SIDE = 64 / LANES;      // of a row, rows side by side
+    constexpr int LOADS = ROWS / SIDE < 4 ? ROWS / SIDE : 4;  // of x on their way at a time
+    static_assert(ROWS % (LOADS * SIDE) == 0, "no row behind the last");
+    constexpr int PITCH = QUADS * 64 + 16, SCALES = QUADS * 4;  // bytes of a row's codes, and of its scales
+    __shared__ __attribute__((aligned(16))) char all_codes[WAVES * ROWS * PITCH], all_scales[WAVES * ROWS * SCALES];
+    __shared__ float sum[AB][WAVES][ROWS][20];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, part = lane >> 4;
+    char *const codes = all_codes + wave * ROWS * PITCH, *const scales = all_scales + wave * ROWS * SCALES;
+    const int pieces = (inputs + 31) >> 5, steps = (pieces + 4 * QUADS - 1) / (4 * QUADS), blocks = (outputs + 15) >> 4;
+    int first = 0, end = rows;  // the rows that count
+    if (starts_.a) {
+        first = start_at(starts_, 0, rows);
+        end = start_at(starts_, sequences, rows);
+    }
+    // A lane's blocks: 4 kk + part, kk = 0 .. QUADS-1, of a step's.
+    uint4_t fw[AB][QUADS];
+    uint32_t sw[AB][QUADS];
+    auto load_weights = [&](int block, int s) __attribute__((always_inline)) {
+        const int col = min(block * 16 + l16, outputs - 1), left = pieces - s * 4 * QUADS - part;
+#pragma unroll
+        for (int a = 0; a < AB; ++a) {
+            const char *w = (const char*)(a ? up_ : w_) + (uint64_t)col * w_stride + part * 16, *ws = (const char*)(a ? us_ : ws_) + (uint64_t)col * ws_stride;
+#pragma unroll
+            for (int kk = 0; kk < QUADS; ++kk) {
+                const bool in = 4 * kk < left;
+                fw[a][kk] = in ? *(const uint4_t*)(w + (s * QUADS + kk) * 64) : uint4_t{};
+                sw[a][kk] = in ? *(const uint32_t*)(ws + (s * QUADS + kk) * 4) >> (8 * part) : 0;
+            }
+        }
+    };
+    auto quantise = [&](int s) __attribute__((always_inline)) {
+        const int at = s * QUADS * 128 + lane % LANES * 8;  // the lane's first column of x
+        wave_lds_sync();  // the step before has been read
+#pragma unroll
+        for (int r0 = 0; r0 < ROWS; r0 += LOADS * SIDE) {
+            if (r0 >= rows) break;  // what stands in the other rows is multiplied, and not stored
+            v8 v[LOADS];
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = r0 + i * SIDE + lane / LANES;
+                v[i] = r < rows && at < inputs ? *(const v8*)((const char*)x_ + (uint64_t)r * x_stride + at * 2) : v8{};
+            }
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = r0 + i * SIDE + lane / LANES;
+                const FourBits got = four_bits<T>(v[i]);
+                *(uint32_t*)(codes + r * PITCH + lane % LANES * 4) = got.codes;
+                if ((lane & 3) == 0) scales[r * SCALES + lane % LANES / 4] = (char)got.scale;
+            }
+        }
+        wave_lds_sync();
+    };
+    if (wave < steps) {
+        load_weights(blockIdx.x, wave);
+        quantise(wave);
+    }
+    for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
+        float4_t acc[AB][XB] = {};
+        for (int s = wave; s < steps; s += WAVES) {
+            if (s != wave) {
+                load_weights(block, s);
+                quantise(s);
+            }
+#pragma unroll
+            for (int m = 0; m < XB; ++m)
+#pragma unroll
+                for (int kk = 0; kk < QUADS; ++kk) {
+                    const int r = m * 16 + l16;
+                    const uint4_t fx = *(const uint4_t*)(codes + r * PITCH + (kk * 4 + part) * 16);
+                    const uint32_t sx = *(const uint32_t*)(scales + r * SCALES + kk * 4) >> (8 * part);
+#pragma unroll
+                    for (int a = 0; a < AB; ++a) acc[a][m] = product16(fw[a][kk], fx, acc[a][m], sw[a][kk], sx);
+                }
+        }
+        if (wave < steps && block + (int)gridDim.x < blocks) load_weights(block + gridDim.x, wave);
+        // Lane: row 16 m + l16, columns 4 part .. +3.
+#pragma unroll
+        for (int a = 0; a < AB; ++a)
+#pragma unroll
+            for (int m = 0; m < XB; ++m) *(float4_t*)&sum[a][wave][m * 16 + l16][4 * part] = acc[a][m];
+        lds_barrier();
+        const int row = tid >> 2, c = (tid & 3) * 4, col = block * 16 + c;
+        if (row >= first && row < min(end, ROWS) && col < outputs) {
+            float4_t v[AB] = {};
+#pragma unroll
+            for (int a = 0; a < AB; ++a) {
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) v[a] += *(const float4_t*)&sum[a][i][row][c];
+                const float* bias = a ? up_bias_ : bias_;
+                if (bias) v[a] += *(const float4_t*)(bias + col);
+            }
+            typename Num<T>::v4 o;
+            if constexpr (GATED) {
+                with_activation(activation, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = (T)(v[1][e] * activated<decltype(act)::value>(v[0][e]));
+                });
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (T)v[0][e];
+            }
+            *(typename Num<T>::v4*)((T*)out_ + (uint64_t)row * out_stride + col) = o;
+        }
+        lds_barrier();  // the sums have been read
+    }
+}
+
+// Whether the few-rows kernel takes a call. Every workgroup quantises all of x, so
+// that rows x inputs is what it costs. us against tiles (with their launch that
+// quantises x), linear: 1024 -> 1024, 1 row 3.2 and 5.9, 32 rows 4.2 and 6.6; 4096 ->
+// 4096, 1 row 4.8 and 10.0, 24 rows 9.6 and 10.7, 32 rows 11.4 and 10.9; 16384 -> 4096, 16
+// rows 21.5 and 28.3, 24 rows 29.8 and 28.4; 4096 -> 16384 (1024 blocks of 16 outputs), 8
+// rows 12.5 and 13.0, 16 rows 14.2 and 13.3.
+inline bool few_product(uint64_t rows, uint64_t inputs, uint64_t outputs) {
+    const uint64_t blocks = (outputs + 15) / 16;
+    if (rows <= 8) return blocks <= 256 || inputs <= 4096;
+    return blocks <= 256 && (rows <= 16 || (rows <= 32 && rows * inputs <= 24 * 4096));
+}
+
+// p.x is the call's own here, in 16 bits, and p.pieces the columns of it. Two
+// workgroups of 16 rows run on a CU, one of 32.
+template <class T, bool GATED, int XB, int QUADS>
+hipError_t launch_few(const Product& p, hipStream_t s) {
+    uint32_t blocks = (p.outputs + 15) / 16;
+    if (p.pieces <= 128 * QUADS * kFewProductWaves) blocks = std::min(blocks, XB == 1 ? 512u : 256u);
+    return enqueue(packed_product_few_kernel<T, GATED, XB, QUADS>, dim3(blocks), dim3(64 * kFewProductWaves), 0, s, p.x, p.w, p.up,
+                   (int)p.rows, (int)p.pieces, (int)p.outputs, (uint32_t)p.x_stride, (uint32_t)p.w_stride, p.starts, p.ws, p.us, p.bias,
+                   p.up_bias, p.out, p.out_stride, (int)p.sequences, (int)p.activation, (uint32_t)p.ws_stride);
+}
+template <class T, bool GATED, int XB>
+hipError_t launch_few_columns(const Product& p, hipStream_t s) {
+    if (p.pieces <= 1024) return launch_few<T, GATED, XB, 1>(p, s);
+    if (p.pieces <= 2048) return launch_few<T, GATED, XB, 2>(p, s);
+    return launch_few<T, GATED, XB, 4>(p, s);
+}
+template <class T, bool GATED>
+hipError_t launch_few_rows(const Product& p, hipStream_t s) {
+    return p.rows <= 16 ? launch_few_columns<T, GATED, 1>(p, s) : launch_few_columns<T, GATED, 2>(p, s);
 }
 
 // The tile of a call, from the number of workgroups that each would make and the

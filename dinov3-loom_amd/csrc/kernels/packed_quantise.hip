@@ -4,26 +4,12 @@
 // memory. A lane takes 8 values (16 bytes), four lanes a block.
 #include <algorithm>
 
-#include "packed.hpp"
+#include "packed_four.hpp"
 
 namespace dhx {
 namespace {
 
 #define DHX_QUANTISE_PARAMS Addr x_, Addr codes_, Addr scales_, int rows, int columns, uint64_t x_stride, uint64_t codes_stride, uint64_t scales_stride, uint64_t group_stride, Addr starts_, int sequences, int block_rows
-
-// The float whose exponent is scale byte b's (what the conversions take).
-__device__ __forceinline__ float scale_of(uint32_t b) { return __builtin_bit_cast(float, b << 23); }
-
-// Codes of two values; which byte of `to` they go into is a constant.
-template <int BYTE>
-__device__ __forceinline__ uint32_t two_codes(uint32_t to, half2_t v, float scale) {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(to, v, scale, BYTE);
-}
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-template <int BYTE>
-__device__ __forceinline__ uint32_t two_codes(uint32_t to, bf16x2_t v, float scale) {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(to, v, scale, BYTE);
-}
 
 // Whether the rows of the call hold `row`.
 __device__ __forceinline__ bool counts(const int32_t* starts, int sequences, int rows, int64_t row) {
@@ -35,7 +21,6 @@ __device__ __forceinline__ bool counts(const int32_t* starts, int sequences, int
 template <class T>
 __global__ __launch_bounds__(256) void packed_quantise_kernel(DHX_QUANTISE_PARAMS) {
     typedef typename Num<T>::v8 v8;
-    typedef T v2 __attribute__((ext_vector_type(2)));
     const int blocks = (columns + 31) >> 5, per_row = ((blocks + 15) & ~15) * 4;
     for (int64_t row0 = (int64_t)blockIdx.x * block_rows; row0 < rows; row0 += (int64_t)gridDim.x * block_rows) {
         const int n = (int)min((int64_t)block_rows, rows - row0) * per_row;
@@ -45,31 +30,12 @@ __global__ __launch_bounds__(256) void packed_quantise_kernel(DHX_QUANTISE_PARAM
             v8 v = {};
             const bool in = counts(starts_, sequences, rows, row);
             if (in && piece * 8 < columns) v = *(const v8*)((const T*)x_ + row * x_stride + piece * 8);
-            // The largest magnitude of the block's 32 values, as the bits of a T: those of
-            // magnitudes are in order, and what is not finite lies above all others.
-            const uint4_t w = __builtin_bit_cast(uint4_t, v);
-            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-            u16x2 top = {};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
-            uint32_t m = max((uint32_t)top[0], (uint32_t)top[1]);
-            m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, false));  // quad_perm 1, 0, 3, 2
-            m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, false));  // quad_perm 2, 3, 0, 1
-            const float largest = (float)__builtin_bit_cast(T, (uint16_t)m);
-            const int exponent = (int)(__builtin_bit_cast(uint32_t, largest) >> 23);
-            const bool odd = exponent == 255;
-            const uint32_t byte = odd ? 255 : (uint32_t)max(exponent - 2, 0);
-            const float scale = scale_of(byte);
-            uint32_t c = 0;
-            c = two_codes<0>(c, v2{v[0], v[1]}, scale);
-            c = two_codes<1>(c, v2{v[2], v[3]}, scale);
-            c = two_codes<2>(c, v2{v[4], v[5]}, scale);
-            c = two_codes<3>(c, v2{v[6], v[7]}, scale);
+            const FourBits got = four_bits<T>(v);
             if (!in) continue;
-            if (piece < blocks * 4) *(uint32_t*)((char*)codes_ + row * codes_stride + piece * 4) = odd ? 0 : c;
+            if (piece < blocks * 4) *(uint32_t*)((char*)codes_ + row * codes_stride + piece * 4) = got.codes;
             if ((piece & 3) == 0) {
                 const int b = piece >> 2;
-                *((uint8_t*)scales_ + (b >> 5) * group_stride + row * scales_stride + (b & 31)) = b < blocks ? (uint8_t)byte : 0;
+                *((uint8_t*)scales_ + (b >> 5) * group_stride + row * scales_stride + (b & 31)) = b < blocks ? (uint8_t)got.scale : 0;
             }
         }
     }

@@ -1,6 +1,7 @@
 // A projection whose weights are held in 4 bits, on packed batches
 // (include/dinov3_packed.h). Two kernels: x is quantised into the workspace
-// (packed_quantise.hip), then the product of both sides' codes (packed_product.hpp).
+// (packed_quantise.hip), then the product of both sides' codes (packed_product.hpp);
+// few rows have a kernel that does both.
 #include "packed_product.hpp"
 
 namespace dhx {
@@ -28,7 +29,9 @@ hipError_t quantise_rows(uint32_t type, const void* x, uint64_t x_stride, uint64
     return launch_packed_quantise(q, s, rows * 32);
 }
 
-uint64_t packed_quantised_linear_bytes(const dhx_packed_quantised_linear& p) { return quantised_rows_bytes(p.rows, p.inputs); }
+uint64_t packed_quantised_linear_bytes(const dhx_packed_quantised_linear& p) {
+    return few_product(p.rows, p.inputs, p.outputs) ? 0 : quantised_rows_bytes(p.rows, p.inputs);
+}
 
 hipError_t launch_packed_quantised_linear(const dhx_packed_quantised_linear& p, hipStream_t s) {
     Product a{};
@@ -44,6 +47,12 @@ hipError_t launch_packed_quantised_linear(const dhx_packed_quantised_linear& p, 
     a.w_stride = p.w_stride;
     a.ws_stride = p.scales_stride;
     a.out_stride = p.y_stride;
+    if (few_product(p.rows, p.inputs, p.outputs)) {
+        a.x = p.x;
+        a.x_stride = p.x_stride * 2;
+        a.pieces = p.inputs;
+        return p.type == DHX_F16 ? launch_few_rows<half_t, false>(a, s) : launch_few_rows<bf16_t, false>(a, s);
+    }
     const hipError_t err = quantise_rows(p.type, p.x, p.x_stride, p.rows, p.inputs, p.workspace, &a, s);
     if (err != hipSuccess) return err;
     return p.type == DHX_F16 ? launch_product<half_t, true, false>(a, s) : launch_product<bf16_t, true, false>(a, s);

@@ -218,7 +218,7 @@ int dhx_packed_dequantise_run(dhx_engine *e, const dhx_packed_quantisation *p, v
  *   y[t] = w Q(x[t]) + bias,
  * Q(x) the row quantised as above within the call (so the products are of 4-bit
  * values, which the matrix units multiply at four times the rate of 16-bit ones;
- * products and sums are float32). A block of x or w that is not a number makes
+ * products and sums are float32; few rows need no workspace). A block of x or w that is not a number makes
  * its row's or column's outputs not a number. */
 typedef struct dhx_packed_quantised_linear {
     uint32_t type; /* DHX_F16 or DHX_BF16: x, y */
@@ -248,7 +248,7 @@ int dhx_packed_quantised_linear_run(dhx_engine *e, const dhx_packed_quantised_li
  * rounded once. Where a sum is infinite or not a number, so may be the output.
  * The weights are of the type of x, or, with gate_scales and up_scales, 4-bit
  * codes as above; then x is quantised alike within the call, and only then is
- * there a workspace. The matrices may be the halves of one. */
+ * there a workspace (of 0 bytes where rows are few). The matrices may be the halves of one. */
 enum { DHX_SILU = 0, DHX_GELU = 1, DHX_GELU_TANH = 2, DHX_RELU = 3, DHX_SIGMOID = 4 };
 
 typedef struct dhx_packed_gated {
