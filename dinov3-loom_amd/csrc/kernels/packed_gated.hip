@@ -8,7 +8,7 @@
 namespace dhx {
 
 uint64_t packed_gated_bytes(const dhx_packed_gated& p) {
-    return p.gate_scales && !few_product(p.rows, p.inputs, p.outputs) ? quantised_rows_bytes(p.rows, p.inputs) : 0;
+    return p.gate_scales && !few_product(p.rows, p.inputs, p.outputs, true) ? quantised_rows_bytes(p.rows, p.inputs) : 0;
 }
 
 hipError_t launch_packed_gated(const dhx_packed_gated& p, hipStream_t s) {
@@ -30,7 +30,7 @@ hipError_t launch_packed_gated(const dhx_packed_gated& p, hipStream_t s) {
         a.us = p.up_scales;
         a.w_stride = p.w_stride;
         a.ws_stride = p.scales_stride;
-        if (few_product(p.rows, p.inputs, p.outputs)) {
+        if (few_product(p.rows, p.inputs, p.outputs, true)) {
         a.x = p.x;
         a.x_stride = p.x_stride * 2;
         a.pieces = p.inputs;

@@ -14,9 +14,10 @@ namespace {
 
 #define DHX_NORM_PARAMS Addr x_, Addr y_, Addr x_out_, Addr h_, int rows, int channels, uint64_t x_stride, uint64_t y_stride, Addr starts_, Addr scale_, Addr gate_, Addr post_weight_, Addr post_bias_, Addr pre_weight_, Addr pre_bias_, uint64_t x_out_stride, uint64_t h_stride, uint64_t gate_stride, int sequences, int post, int pre, float post_eps, float pre_eps
 
-// The sum of v over the G lanes (G <= 64: of a wave, else of the workgroup) that
+// The sum of v over the G lanes (G <= 64: of a wave, else all of the workgroup) that
 // hold a row, in all of them, by the same tree in each: inside rows of 16 lanes by
-// moves between lanes (G at least 8), then across them. part: a float per wave.
+// moves between lanes (G at least 8), then across them. part: a float for each of 16
+// waves, zeros behind the last.
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* part) {
     auto move = [](float a, auto ctrl) {
@@ -34,7 +35,7 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
         __syncthreads();
         v = 0.f;
 #pragma unroll
-        for (int w = 0; w < G / 64; ++w) v += part[w];
+        for (int w = 0; w < 16; ++w) v += part[w];
     }
     return v;
 }
@@ -72,18 +73,26 @@ __device__ __forceinline__ void load8(const S* p, float (&v)[8]) {
         for (int e = 0; e < 8; ++e) v[e] = (float)a[e];
     }
 }
+// 8 values from element `at` of rows on: 16-bit ones through the L2 (12864 rows of 384
+// channels 11.0 us, 11.5 without), float32 ones, of which an instruction stores half a
+// line only, not (5,000,000 values 14.0 us, through it 17.5).
 template <class S>
-__device__ __forceinline__ void store8(S* p, const float (&v)[8]) {
-    if constexpr (std::is_same_v<S, float>) {
-        *(float4_t*)p = float4_t{v[0], v[1], v[2], v[3]};
-        *(float4_t*)(p + 4) = float4_t{v[4], v[5], v[6], v[7]};
-    } else {
-        typename Num<S>::v8 a;
+struct Rows {
+    S* first;
+    WtOut through;
+    __device__ __forceinline__ explicit Rows(S* p) : first(p), through(p, ~0u) {}
+    __device__ __forceinline__ void store8(uint32_t at, const float (&v)[8]) const {
+        if constexpr (std::is_same_v<S, float>) {
+            *(float4_t*)(first + at) = float4_t{v[0], v[1], v[2], v[3]};
+            *(float4_t*)(first + at + 4) = float4_t{v[4], v[5], v[6], v[7]};
+        } else {
+            typename Num<S>::v8 a;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = (S)v[e];
-        *(typename Num<S>::v8*)p = a;
+            for (int e = 0; e < 8; ++e) a[e] = (S)v[e];
+            through.store(at * 2, a);
+        }
     }
-}
+};
 
 // A channel vector's piece; ones or zeros where there is no vector.
 __device__ __forceinline__ void vector8(const float* vector, int c, float none, float (&v)[8]) {
@@ -97,7 +106,7 @@ __device__ __forceinline__ void vector8(const float* vector, int c, float none, 
 
 // One over the row's root of its mean square, of P pieces of 8 channels a lane
 // (zeros where a piece does not exist); for LayerNorm of the deviations from the
-// mean, which it leaves in v. Both sums are of registers. part: 2 G / 64 floats.
+// mean, which it leaves in v. Both sums are of registers. part: 32 floats.
 template <int G, int P>
 __device__ __forceinline__ float inverse(float (&v)[P][8], const bool (&there)[P], int kind, float eps, int channels, float* part) {
     const float each = 1.0f / (float)channels;
@@ -118,28 +127,32 @@ __device__ __forceinline__ float inverse(float (&v)[P][8], const bool (&there)[P
     for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(v[p][e], v[p][e], sum);
-    return rsqrtf(fmaf(row_sum<G>(sum, part + (G > 64 ? G / 64 : 0)), each, eps));
+    return rsqrtf(fmaf(row_sum<G>(sum, part + 16), each, eps));
 }
 
-// T: y and h, S: x and x'. G lanes hold a row, P pieces of 8 channels each: piece p
-// of lane l is G p + l of the row.
+// T: y and h, S: x and x'. G lanes (over 64: those of the workgroup, however many)
+// hold a row, P pieces of 8 channels each: piece p of lane l is G p + l of the row.
 template <class T, class S, int G, int P>
 __global__ __launch_bounds__(G <= 64 ? 256 : G) void packed_norm_kernel(DHX_NORM_PARAMS) {
-    constexpr int THREADS = G <= 64 ? 256 : G, ROWS = THREADS / G, WAVE_ROWS = G <= 64 ? 64 / G : 1;
-    __shared__ float part[G > 64 ? 4 * G / 64 : 1];
+    constexpr int ROWS = G <= 64 ? 256 / G : 1, WAVE_ROWS = G <= 64 ? 64 / G : 1;
+    __shared__ float part[G > 64 ? 64 : 1];  // 16 waves' sums, of four kinds
     const S* x = x_;
     const T* y = y_;
-    const int tid = threadIdx.x, lane = tid % G, in_wave = G <= 64 ? (tid & 63) / G : 0;
+    const int tid = threadIdx.x, lanes = G <= 64 ? G : blockDim.x, lane = G <= 64 ? tid % G : tid, in_wave = G <= 64 ? (tid & 63) / G : 0;
     const int pieces = channels >> 3;
     bool there[P];
     int at[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        there[p] = G * p + lane < pieces;
-        at[p] = (G * p + lane) * 8;
+        there[p] = lanes * p + lane < pieces;
+        at[p] = (lanes * p + lane) * 8;
     }
+    if (G > 64 && tid < 64 && tid % 16 >= lanes >> 6) part[tid] = 0.f;
     for (int64_t first = (int64_t)blockIdx.x * ROWS; first < rows; first += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = first + tid / G;
+        const int in_block = G <= 64 ? tid / G : 0;
+        const int64_t row = first + in_block;
+        const Rows<S> x_rows((S*)x_out_ + first * x_out_stride);
+        const Rows<T> h_rows((T*)h_ + first * h_stride);
         const int32_t* starts = starts_;
         bool in = row < rows;
         int s = 0;
@@ -193,17 +206,17 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void packed_norm_kernel(DHX_NORM
                 if constexpr (P > 1) step_vectors(p, by, plus);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[p][e] = there[p] ? v[p][e] + fmaf(z[p][e] * r, by[e], plus[e]) : 0.f;
-                if (in && there[p]) store8((S*)x_out_ + row * x_out_stride + at[p], v[p]);
+                if (in && there[p]) x_rows.store8(in_block * (uint32_t)x_out_stride + at[p], v[p]);
             }
         }
         if (pre != DHX_NORM_NONE) {
-            const float r = inverse<G, P>(v, there, pre, pre_eps, channels, part + (G > 64 ? 2 * G / 64 : 0));
+            const float r = inverse<G, P>(v, there, pre, pre_eps, channels, part + 32);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 if constexpr (P > 1) pre_vectors(p, pre_by, pre_plus);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[p][e] = fmaf(v[p][e] * r, pre_by[e], pre_plus[e]);
-                if (in && there[p]) store8((T*)h_ + row * h_stride + at[p], v[p]);
+                if (in && there[p]) h_rows.store8(in_block * (uint32_t)h_stride + at[p], v[p]);
             }
         }
         if (G > 64) __syncthreads();  // part, for the next row
@@ -214,9 +227,10 @@ constexpr uint64_t kMostBlocks = 1u << 21;  // a launch has fewer than 2^32 thre
 
 template <class T, class S, int G, int P>
 hipError_t launch(const dhx_packed_norm& p, hipStream_t s) {
-    constexpr int THREADS = G <= 64 ? 256 : G, ROWS = THREADS / G;
+    constexpr int ROWS = G <= 64 ? 256 / G : 1;
+    const uint32_t threads = G <= 64 ? 256 : (p.channels / 8 + 64 * P - 1) / (64 * P) * 64;
     const uint64_t blocks = std::min<uint64_t>((p.rows + ROWS - 1) / ROWS, kMostBlocks);
-    return enqueue(packed_norm_kernel<T, S, G, P>, dim3((unsigned)blocks), dim3(THREADS), 0, s, p.x, p.y, p.x_out, p.h, (int)p.rows,
+    return enqueue(packed_norm_kernel<T, S, G, P>, dim3((unsigned)blocks), dim3(threads), 0, s, p.x, p.y, p.x_out, p.h, (int)p.rows,
                    (int)p.channels, p.x_stride, p.y_stride, p.starts, p.scale, p.gate, p.post_weight, p.post_bias, p.pre_weight,
                    p.pre_bias, p.x_out_stride, p.h_stride, p.gate_stride, (int)p.sequences, (int)p.post, (int)p.pre, p.post_eps,
                    p.pre_eps);
@@ -232,9 +246,6 @@ hipError_t launch_pieces(const dhx_packed_norm& p, hipStream_t s) {
     if (pieces <= 16) return launch<T, S, 16, 1>(p, s);
     if (pieces <= 32) return launch<T, S, 32, 1>(p, s);
     if (pieces <= 64) return launch<T, S, 64, 1>(p, s);
-    if (pieces <= 128) return launch<T, S, 128, 1>(p, s);
-    if (pieces <= 256) return launch<T, S, 256, 1>(p, s);
-    if (pieces <= 512) return launch<T, S, 512, 1>(p, s);
     if (pieces <= 1024) return launch<T, S, 1024, 1>(p, s);
     if (pieces <= 2048) return launch<T, S, 1024, 2>(p, s);
     return launch<T, S, 1024, 4>(p, s);

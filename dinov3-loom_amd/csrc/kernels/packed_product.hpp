@@ -107,7 +107,6 @@ __device__ __forceinline__ void with_activation(int activation, F f) {
 // then, 190 so). Those of x lie [32 blocks][row][32], so that a load's rows are one piece.
 template <class T, bool FOUR, bool GATED, int BM, int BN, int WM, int WN, int NST, int PER_SIMD>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_product_kernel(DHX_PRODUCT_PARAMS) {
-    typedef typename Num<T>::v8 v8;
     typedef typename Num<T>::v4 v4;
     constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES;
     constexpr int XL = BM / 8 / WAVES, WL = BN / 8 / WAVES;  // loads of 8 rows per wave and stage
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
     // Buffers of the tile's rows: a load's address is one register per lane and one
     // of the wave, and a lane beyond the end fetches zeros. A wave loads rows of one
     // of the matrices.
-    static_assert(32 % (WL * 8) == 0, "of gate or of up");
+    static_assert(!GATED || 32 % (WL * 8) == 0, "of gate or of up");
     const int columns = min(BO, outputs - col0);
     auto rows_of = [&](Addr base, int row, int n, uint32_t stride) {
         return __builtin_amdgcn_make_buffer_rsrc((void*)(base.a + (uint64_t)row * stride), 0, (int)((uint32_t)(n - 1) * stride + pieces * 16),
@@ -332,15 +331,39 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
             step(std::integral_constant<int, 3>{}, NST > 2 ? s3 : s1, s0, s + 3);
         }
     }
-    wait_vm<0>();  // no load may come when the LDS is another workgroup's
+    wait_vm<0>();  // no load may come when the LDS holds outputs, or is another workgroup's
+    barrier();
 
     // Lane: row l32 of a block, columns 8 g + 4 hi .. +3 of its 32 in register group
-    // g; both halves exchange groups, so that each stores 8 columns at once.
+    // g; both halves exchange groups, so that each holds 8 columns at once. A wave's
+    // 32 rows go through its own part of the LDS, from where they are stored as whole
+    // lines, through the L2 as WtOut's (common.hpp). us, 32-byte pieces straight from
+    // registers, whole lines, and those through the L2: linear, 4 bits, 16384 rows, 4096 ->
+    // 4096, 192, 180, 178; gated, 12864 rows, 384 -> 1536, 46.6, 44.1, 41.7, 2299 rows, 1000
+    // -> 2728 with 4 bits 20.7, 20.6, 18.5. (Pieces through the L2 257, 52.6 and 19.5.)
+    constexpr int ROW = (GATED ? WN / 2 : WN) * 2, PITCH = ROW + 16, LANES = ROW / 16;  // bytes; lanes of a stored row
+    static_assert(WAVES * 32 * PITCH <= SS, "the first stage's buffer holds them");
+    char* const mine = s0 + wave * 32 * PITCH;
+    const uint32_t out_bytes = (uint32_t)out_stride * 2;
+    const __amdgpu_buffer_rsrc_t out_rows = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(out_.a + (uint64_t)row0 * out_bytes), 0, (int)((uint32_t)(min(BM, rows - row0) - 1) * out_bytes + outputs * 2), kBufferRsrcWord3);
     auto bias4 = [&](int k, int g) { return *(const float4_t*)(sBias + wn + k * 32 + 8 * g + 4 * hi); };
-    auto store = [&](int i, int col, v4 lo, v4 up) __attribute__((always_inline)) {
-        const int row = row0 + wm + i * 32 + l32;
-        const v8 piece = __builtin_bit_cast(v8, frag_swap(__builtin_bit_cast(half4_t, lo), __builtin_bit_cast(half4_t, up)));
-        if (row >= first && row < end && col + hi * 8 < outputs) *(v8*)((T*)out_ + (uint64_t)row * out_stride + col + hi * 8) = piece;
+    auto put = [&](int column, v4 lo, v4 up) __attribute__((always_inline)) {
+        *(half8_t*)(mine + l32 * PITCH + (column + hi * 8) * 2) = frag_swap(__builtin_bit_cast(half4_t, lo), __builtin_bit_cast(half4_t, up));
+    };
+    auto store = [&](int i) __attribute__((always_inline)) {
+        wave_lds_sync();
+#pragma unroll
+        for (int j = 0; j < 32 * LANES / 64; ++j) {
+            const int r = j * (64 / LANES) + lane / LANES, row = row0 + wm + i * 32 + r;
+            const int col = col0 + (GATED ? wn / 2 : wn) + lane % LANES * 8;
+            const bool there = row >= first && row < end && col < outputs;
+            const uint32_t at = there ? (uint32_t)(row - row0) * out_bytes + col * 2 : ~15u;  // past the end: not stored
+            const uint4_t piece = *(const uint4_t*)(mine + r * PITCH + lane % LANES * 16);
+            constexpr int kSc1 = 16;
+            __builtin_amdgcn_raw_buffer_store_b128(piece, out_rows, (int)at, 0, kSc1);
+        }
+        wave_lds_sync();
     };
     auto rounded = [](float4_t v) {
         v4 o;
@@ -352,7 +375,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
     if constexpr (GATED) {
         with_activation(activation, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
+            for (int i = 0; i < MB; ++i) {
 #pragma unroll
                 for (int k = 0; k < NB; k += 2)
 #pragma unroll
@@ -366,18 +389,21 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
                             for (int e = 0; e < 4; ++e) u[e] *= activated<decltype(act)::value>(a[e]);
                             o[q] = rounded(u);
                         }
-                        store(i, col0 + (wn + k * 32) / 2 + kk * 16, o[0], o[1]);
+                        put(k * 16 + kk * 16, o[0], o[1]);
                     }
+                store(i);
+            }
         });
     } else {
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+        for (int i = 0; i < MB; ++i) {
 #pragma unroll
             for (int k = 0; k < NB; ++k)
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
-                    store(i, col0 + wn + k * 32 + kk * 16, rounded(group(acc[i][k], 2 * kk) + bias4(k, 2 * kk)),
-                          rounded(group(acc[i][k], 2 * kk + 1) + bias4(k, 2 * kk + 1)));
+                    put(k * 32 + kk * 16, rounded(group(acc[i][k], 2 * kk) + bias4(k, 2 * kk)), rounded(group(acc[i][k], 2 * kk + 1) + bias4(k, 2 * kk + 1)));
+            store(i);
+        }
     }
 }
 
@@ -390,7 +416,7 @@ hipError_t launch_tiles(const Product& p, hipStream_t s) {
 }
 
 // Few rows against 4-bit weights, which are all there is to read: a workgroup takes
-// 16 outputs at a time (gated: and both of their sums) and all rows (16 XB of them), its
+// 16 outputs at a time (gated: and both of their sums) and 16 XB rows, its
 // waves share the columns out in steps of QUADS * 4 blocks and join their sums in LDS.
 // Weights go straight into registers; a wave quantises its own columns of x into its
 // own LDS while they are on their way, so that one launch does it all. Where every wave
@@ -411,6 +437,8 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, part = lane >> 4;
     char *const codes = all_codes + wave * ROWS * PITCH, *const scales = all_scales + wave * ROWS * SCALES;
+    const int row0 = blockIdx.y * ROWS, mine = min(rows - row0, ROWS);
+    const char* x0 = (const char*)x_ + (uint64_t)row0 * x_stride;
     const int pieces = (inputs + 31) >> 5, steps = (pieces + 4 * QUADS - 1) / (4 * QUADS), blocks = (outputs + 15) >> 4;
     int first = 0, end = rows;  // the rows that count
     if (starts_.a) {
@@ -438,12 +466,12 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
         wave_lds_sync();  // the step before has been read
 #pragma unroll
         for (int r0 = 0; r0 < ROWS; r0 += LOADS * SIDE) {
-            if (r0 >= rows) break;  // what stands in the other rows is multiplied, and not stored
+            if (r0 >= mine) break;  // what stands in the other rows is multiplied, and not stored
             v8 v[LOADS];
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int r = r0 + i * SIDE + lane / LANES;
-                v[i] = r < rows && at < inputs ? *(const v8*)((const char*)x_ + (uint64_t)r * x_stride + at * 2) : v8{};
+                v[i] = r < mine && at < inputs ? *(const v8*)(x0 + (uint64_t)r * x_stride + at * 2) : v8{};
             }
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
@@ -484,13 +512,13 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
 #pragma unroll
             for (int m = 0; m < XB; ++m) *(float4_t*)&sum[a][wave][m * 16 + l16][4 * part] = acc[a][m];
         lds_barrier();
-        const int row = tid >> 2, c = (tid & 3) * 4, col = block * 16 + c;
-        if (row >= first && row < min(end, ROWS) && col < outputs) {
+        const int r = tid >> 2, row = row0 + r, c = (tid & 3) * 4, col = block * 16 + c;
+        if (r < mine && row >= first && row < end && col < outputs) {
             float4_t v[AB] = {};
 #pragma unroll
             for (int a = 0; a < AB; ++a) {
 #pragma unroll
-                for (int i = 0; i < WAVES; ++i) v[a] += *(const float4_t*)&sum[a][i][row][c];
+                for (int i = 0; i < WAVES; ++i) v[a] += *(const float4_t*)&sum[a][i][r][c];
                 const float* bias = a ? up_bias_ : bias_;
                 if (bias) v[a] += *(const float4_t*)(bias + col);
             }
@@ -510,16 +538,20 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
     }
 }
 
-// Whether the few-rows kernel takes a call. Every workgroup quantises all of x, so
-// that rows x inputs is what it costs. us against tiles (with their launch that
-// quantises x), linear: 1024 -> 1024, 1 row 3.2 and 5.9, 32 rows 4.2 and 6.6; 4096 ->
+// Whether the few-rows kernel takes a call. Every workgroup quantises all of its rows
+// of x, so that rows x inputs is what it costs. us against tiles (with their launch
+// that quantises x), linear: 1024 -> 1024, 1 row 3.2 and 5.9, 32 rows 4.2 and 6.6; 4096 ->
 // 4096, 1 row 4.8 and 10.0, 24 rows 9.6 and 10.7, 32 rows 11.4 and 10.9; 16384 -> 4096, 16
 // rows 21.5 and 28.3, 24 rows 29.8 and 28.4; 4096 -> 16384 (1024 blocks of 16 outputs), 8
-// rows 12.5 and 13.0, 16 rows 14.2 and 13.3.
-inline bool few_product(uint64_t rows, uint64_t inputs, uint64_t outputs) {
-    const uint64_t blocks = (outputs + 15) / 16;
+// rows 12.5 and 13.0, 16 rows 14.2 and 13.3. In several blocks of 32 rows: 1024 -> 1024,
+// 256 rows (512 workgroups) 6.1 and 6.9, 512 rows 9.8 and 7.0; 2048 -> 2048, 64 rows (256)
+// 6.5 and 8.5, 128 rows 9.7 and 8.7; gated, 1024 -> 2728, 64 rows (342) 7.3 and 7.0, 384 ->
+// 1536, 128 rows (384) 4.9 and 6.2.
+inline bool few_product(uint64_t rows, uint64_t inputs, uint64_t outputs, bool gated) {
+    const uint64_t blocks = (outputs + 15) / 16, all = (rows + 31) / 32 * blocks;
     if (rows <= 8) return blocks <= 256 || inputs <= 4096;
-    return blocks <= 256 && (rows <= 16 || (rows <= 32 && rows * inputs <= 24 * 4096));
+    if (rows <= 32) return blocks <= 256 && (rows <= 16 || rows * inputs <= 24 * 4096);
+    return all <= 512 && inputs <= 2048 && all * inputs * (gated ? 2 : 1) <= 512 * 1024;
 }
 
 // p.x is the call's own here, in 16 bits, and p.pieces the columns of it. Two
@@ -528,7 +560,8 @@ template <class T, bool GATED, int XB, int QUADS>
 hipError_t launch_few(const Product& p, hipStream_t s) {
     uint32_t blocks = (p.outputs + 15) / 16;
     if (p.pieces <= 128 * QUADS * kFewProductWaves) blocks = std::min(blocks, XB == 1 ? 512u : 256u);
-    return enqueue(packed_product_few_kernel<T, GATED, XB, QUADS>, dim3(blocks), dim3(64 * kFewProductWaves), 0, s, p.x, p.w, p.up,
+    return enqueue(packed_product_few_kernel<T, GATED, XB, QUADS>, dim3(blocks, (p.rows + 16 * XB - 1) / (16 * XB)),
+                   dim3(64 * kFewProductWaves), 0, s, p.x, p.w, p.up,
                    (int)p.rows, (int)p.pieces, (int)p.outputs, (uint32_t)p.x_stride, (uint32_t)p.w_stride, p.starts, p.ws, p.us, p.bias,
                    p.up_bias, p.out, p.out_stride, (int)p.sequences, (int)p.activation, (uint32_t)p.ws_stride);
 }
@@ -550,8 +583,9 @@ hipError_t launch_few_rows(const Product& p, hipStream_t s) {
 // - 256 x 256 where they fill the CUs once or in rounds of which the last is not
 //   mostly empty: gated, 4096 -> 8192, 1024 rows (256 tiles) 116, 128 x 128 148; 512 rows
 //   (128 tiles) 98 and 77; 1024 -> 2728, 2048 rows (176) 27.4 and 30.5, 4096 rows (352)
-//   55.9 and 51.8; 384 -> 1536, 12864 rows (612) 46.7 and 45.8; four bits, two stages
-//   (384 -> 1536, 4096 rows) 17.4 and 15.1;
+//   55.9 and 51.8; 384 -> 1536, 12864 rows (612) 41.4 and 44.5; four bits, two stages
+//   (384 -> 1536, 4096 rows) 17.4 and 15.1; gated, waves of 64 x 128, which hold whole
+//   lines of outputs (128 x 64: 8192 rows, 4096 -> 8192, 860 and 844);
 // - long rows and a CU for every tile: four stages in flight, of the smallest such tile:
 //   gated, 4096 -> 8192, 48 rows, 64 x 64 34.1 (two stages 49.9), 128 rows, 128 x 64 38.9
 //   (55.6), 256 rows, 128 x 128 49.4 (60.8; four bits 20.8 and 19.2); short rows gain
@@ -565,8 +599,10 @@ hipError_t launch_product(const Product& p, hipStream_t s) {
     const uint64_t largest = (p.rows + 255ull) / 256 * ((p.outputs + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
     const uint32_t steps = (p.pieces + 7) / 8;
     constexpr int WM = GATED ? 32 : 64, WN = GATED ? 64 : 32;  // of a 128 x 64 tile: a wave of the gated one holds both sums
-    const bool fills = largest <= 256 ? largest >= 160 : largest * 20 >= (largest + 255) / 256 * 256 * 17;
-    if (fills && (!FOUR || steps > 2)) return launch_tiles<T, FOUR, GATED, 256, 256, 128, 64, 2, 2>(p, s);
+    const bool fills = largest <= 256 ? largest >= 160 : largest * 4 >= (largest + 255) / 256 * 256 * 3;
+    // (With 4 bits that tile takes stages by fours.)
+    if (fills && (!FOUR || (steps + 3) / 4 * 16 <= steps * 5))
+        return launch_tiles<T, FOUR, GATED, 256, 256, GATED ? 64 : 128, GATED ? 128 : 64, 2, 2>(p, s);
     if (steps >= 12) {
         if (count(64, 64) <= 256) return launch_tiles<T, FOUR, GATED, 64, 64, 32, GATED ? 64 : 32, 4, GATED ? 1 : 2>(p, s);
         if (count(128, 64) <= 256) return launch_tiles<T, FOUR, GATED, 128, 64, WM, WN, 4, 1>(p, s);

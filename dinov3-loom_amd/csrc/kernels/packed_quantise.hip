@@ -1,7 +1,9 @@
 // Rows of a packed batch to 4-bit codes with a scale per block of 32 values, and
 // back (include/dinov3_packed.h). Every value is read once and every code written
 // once, or the other way round; there is little arithmetic, so both are bound by
-// memory. A lane takes 8 values (16 bytes), four lanes a block.
+// memory. A lane takes 8 values (16 bytes), four lanes a block. Codes and values are
+// stored through the L2 (WtOut, common.hpp): 8192 rows of 4096 to codes and back 36.7
+// us without, 34.5 so (168 MB, 4.9 TB/s), 2299 of 1000 5.9 and 5.5.
 #include <algorithm>
 
 #include "packed_four.hpp"
@@ -23,6 +25,7 @@ __global__ __launch_bounds__(256) void packed_quantise_kernel(DHX_QUANTISE_PARAM
     typedef typename Num<T>::v8 v8;
     const int blocks = (columns + 31) >> 5, per_row = ((blocks + 15) & ~15) * 4;
     for (int64_t row0 = (int64_t)blockIdx.x * block_rows; row0 < rows; row0 += (int64_t)gridDim.x * block_rows) {
+        const __amdgpu_buffer_rsrc_t code_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(codes_.a + row0 * codes_stride), 0, -1, kBufferRsrcWord3);
         const int n = (int)min((int64_t)block_rows, rows - row0) * per_row;
         for (int i = threadIdx.x; i < n; i += 256) {  // n is a multiple of 64: whole waves
             const int r = i / per_row, piece = i - r * per_row;
@@ -32,7 +35,10 @@ __global__ __launch_bounds__(256) void packed_quantise_kernel(DHX_QUANTISE_PARAM
             if (in && piece * 8 < columns) v = *(const v8*)((const T*)x_ + row * x_stride + piece * 8);
             const FourBits got = four_bits<T>(v);
             if (!in) continue;
-            if (piece < blocks * 4) *(uint32_t*)((char*)codes_ + row * codes_stride + piece * 4) = got.codes;
+            if (piece < blocks * 4) {
+                constexpr int kSc1 = 16;
+                __builtin_amdgcn_raw_buffer_store_b32(got.codes, code_rows, (int)((uint32_t)r * (uint32_t)codes_stride + piece * 4), 0, kSc1);
+            }
             if ((piece & 3) == 0) {
                 const int b = piece >> 2;
                 *((uint8_t*)scales_ + (b >> 5) * group_stride + row * scales_stride + (b & 31)) = b < blocks ? (uint8_t)got.scale : 0;
@@ -46,6 +52,7 @@ __global__ __launch_bounds__(256) void packed_dequantise_kernel(DHX_QUANTISE_PAR
     typedef typename Num<T>::v8 v8;
     const int per_row = columns >> 3;
     for (int64_t row0 = (int64_t)blockIdx.x * block_rows; row0 < rows; row0 += (int64_t)gridDim.x * block_rows) {
+        const WtOut x_rows((const T*)x_ + row0 * x_stride, ~0u);
         const int n = (int)min((int64_t)block_rows, rows - row0) * per_row;
         for (int i = threadIdx.x; i < n; i += 256) {
             const int r = i / per_row, piece = i - r * per_row;
@@ -60,7 +67,7 @@ __global__ __launch_bounds__(256) void packed_dequantise_kernel(DHX_QUANTISE_PAR
                 v[2 * e] = (T)two[0];
                 v[2 * e + 1] = (T)two[1];
             }
-            *(v8*)((T*)x_ + row * x_stride + piece * 8) = v;
+            x_rows.store((uint32_t)r * (uint32_t)x_stride * 2 + piece * 16, v);
         }
     }
 }

@@ -30,7 +30,7 @@ hipError_t quantise_rows(uint32_t type, const void* x, uint64_t x_stride, uint64
 }
 
 uint64_t packed_quantised_linear_bytes(const dhx_packed_quantised_linear& p) {
-    return few_product(p.rows, p.inputs, p.outputs) ? 0 : quantised_rows_bytes(p.rows, p.inputs);
+    return few_product(p.rows, p.inputs, p.outputs, false) ? 0 : quantised_rows_bytes(p.rows, p.inputs);
 }
 
 hipError_t launch_packed_quantised_linear(const dhx_packed_quantised_linear& p, hipStream_t s) {
@@ -47,7 +47,7 @@ hipError_t launch_packed_quantised_linear(const dhx_packed_quantised_linear& p, 
     a.w_stride = p.w_stride;
     a.ws_stride = p.scales_stride;
     a.out_stride = p.y_stride;
-    if (few_product(p.rows, p.inputs, p.outputs)) {
+    if (few_product(p.rows, p.inputs, p.outputs, false)) {
         a.x = p.x;
         a.x_stride = p.x_stride * 2;
         a.pieces = p.inputs;
