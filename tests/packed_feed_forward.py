@@ -224,7 +224,9 @@ def values(codes, scales, columns):
     table = torch.tensor(GRID + [-v for v in GRID], dtype=torch.float64, device=codes.device)
     v = torch.stack([table[(codes & 15).long()], table[(codes >> 4).long()]], 2).flatten(1)
     n = v.shape[1] // 32
-    by = torch.where(scales[:, :n] == 255, math.nan, torch.ldexp(torch.ones(1, dtype=torch.float64, device=codes.device), scales[:, :n].int() - 127))
+    # Powers of two from the host: on the GPU ldexp is a product with a rounded pow.
+    steps = torch.tensor([2.0 ** (b - 127) for b in range(255)] + [math.nan], dtype=torch.float64).to(codes.device)
+    by = steps[scales[:, :n].long()]
     return (v.view(-1, n, 32) * by[:, :, None]).flatten(1)[:, :columns]
 
 
