@@ -212,24 +212,33 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
     static_assert(XL % 2 == 0 || XL == 1, "rows 16 apart have their pieces at the same slots");
     auto chunk = [&](int j) { return (lane & 7) ^ slot_of<64>((j & 1) * 8 + (lane >> 3)); };
     const int chunk_x = chunk(wave * XL), chunk_w = chunk(wave * WL);  // of a wave's even loads; bit 1 differs in odd ones
-    auto move = [&](char* to, int s, int turn) __attribute__((always_inline)) {
+    // Load n of a wave's XL + WL of a stage, the scales with the first.
+    auto move_one = [&](char* to, int s, int turn, int n) __attribute__((always_inline)) {
         const int left = pieces - s * 8;
-        if (turn == 0) move_scales(s);
+        if (n == 0 && turn == 0) move_scales(s);
+        if (n < XL) buffer_load(x_rows, to + (wave * XL + n) * 1024, (chunk_x ^ (n & 1) * 2) < left ? xo[n < XL ? n : 0] : ~15u, s * 128);
+        const int j = n - XL;
+        if (j >= 0)
+            buffer_load(w_rows, to + WS + (wave * WL + j) * 1024, (chunk_w ^ (j & 1) * 2) < left ? wo[j >= 0 ? j : 0] : ~15u, s * 128);
+    };
+    auto move = [&](char* to, int s, int turn) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < XL; ++j) buffer_load(x_rows, to + (wave * XL + j) * 1024, (chunk_x ^ (j & 1) * 2) < left ? xo[j] : ~15u, s * 128);
-#pragma unroll
-        for (int j = 0; j < WL; ++j) buffer_load(w_rows, to + WS + (wave * WL + j) * 1024, (chunk_w ^ (j & 1) * 2) < left ? wo[j] : ~15u, s * 128);
+        for (int n = 0; n < XL + WL; ++n) move_one(to, s, turn, n);
     };
 
     const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
     const int frag = l32 * 128 + (((hi * 4) ^ slot_of<64>(l32)) << 4);
     float16_t acc[MB][NB] = {};
     uint4_t fx[2][MB], fw[2][NB];
+    // Fragment n of MB + NB.
+    auto load_one = [&](const char* from, int kk, int set, int n) __attribute__((always_inline)) {
+        const int at = frag ^ (kk << 4);
+        if (n < MB) fx[set][n < MB ? n : 0] = *(const uint4_t*)(from + (wm + n * 32) * 128 + at);
+        else fw[set][n < MB ? 0 : n - MB] = *(const uint4_t*)(from + WS + (wn + (n - MB) * 32) * 128 + at);
+    };
     auto load = [&](const char* from, int kk, int set) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) fx[set][i] = *(const uint4_t*)(from + (wm + i * 32) * 128 + (frag ^ (kk << 4)));
-#pragma unroll
-        for (int i = 0; i < NB; ++i) fw[set][i] = *(const uint4_t*)(from + WS + (wn + i * 32) * 128 + (frag ^ (kk << 4)));
+        for (int n = 0; n < MB + NB; ++n) load_one(from, kk, set, n);
     };
     // The scales of stage s: two stages in a ring take them from LDS stage by stage,
     // four take those of four stages at once, since their place is filled anew before
@@ -272,12 +281,28 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
                 }
         }
     };
-    auto multiply = [&](auto kk, int set, int scales) __attribute__((always_inline)) {
+    // The products of step kk; between them the reads of the next step's fragments, in
+    // the first half, and loads d0 .. d1-1 of a stage. (With all reads and loads in front
+    // of the products the matrix units wait while they are issued: gated, 12864 rows, 384
+    // -> 1536, 44.8 us, so 38.1; linear, 4 bits, 16384 rows, 4096 -> 4096, 186 and 172;
+    // loads only between the products 42.0 and 178.)
+    auto multiply = [&](auto kk, int scales, auto read, auto fetch, int d0, int d1) __attribute__((always_inline)) {
+        constexpr int STEP = decltype(kk)::value, N = MB * NB, HALF = (N + 1) / 2;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int k = 0; k < NB; ++k)
-                acc[i][k] = product32<T, FOUR, decltype(kk)::value>(fw[set][k], fx[set][i], acc[i][k], FOUR ? scale_w[scales][k] : 0, FOUR ? scale_x[scales][i] : 0);
+            for (int k = 0; k < NB; ++k) {
+                const int m = i * NB + k;
+                acc[i][k] = product32<T, FOUR, STEP>(fw[STEP & 1][k], fx[STEP & 1][i], acc[i][k], FOUR ? scale_w[scales][k] : 0, FOUR ? scale_x[scales][i] : 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (m < HALF) {
+#pragma unroll
+                    for (int r = m * (MB + NB) / HALF; r < (m + 1) * (MB + NB) / HALF; ++r) read(r);
+                }
+#pragma unroll
+                for (int n = d0 + m * (d1 - d0) / N; n < d0 + (m + 1) * (d1 - d0) / N; ++n) fetch(n);
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
     move(s0, 0, 0);
     if (tid < BN) {
@@ -291,44 +316,43 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void packed_p
     // Opens stage s: it has landed (the NST - 2 stages behind it may be on their way,
     // with their scales), and every wave has read the one before, whose place stage
     // s + NST - 1 takes. turn: s % 4, a constant.
-    auto open = [&](auto turn, char* free, int s) __attribute__((always_inline)) {
+    auto open = [&](auto turn) __attribute__((always_inline)) {
         constexpr int TURN = decltype(turn)::value;
         wait_vm<(NST - 2) * (XL + WL) + (NST == 4 && TURN >= 2 ? SL : 0)>();
         wait_lgkm();
         barrier();
-        move(free, s + NST - 1, (TURN + NST - 1) & 3);
     };
-    // Multiplies a stage; the next one's first fragments are on their way under the
-    // last products.
-    auto step = [&](auto turn, char* now, const char* next, int s) __attribute__((always_inline)) {
+    // Multiplies a stage; the next one's first fragments are read between its last
+    // products, and the loads of the stage that takes its place begin there too, in
+    // large tiles the half of them (in small ones that gained nothing).
+    constexpr int ALL = XL + WL, FIRST = MB * NB >= 4 ? ALL / 2 : ALL;
+    auto step = [&](auto turn, char* before, char* now, const char* next, int s) __attribute__((always_inline)) {
         constexpr int TURN = decltype(turn)::value, SET = NST == 2 ? TURN & 1 : TURN, NEXT = (TURN + 1) & 3;
-        auto inner = [&](auto kk) __attribute__((always_inline)) {
-            load(now, kk + 1, (kk + 1) & 1);
-            if (NST == 2 && kk == 0 && (TURN & 1) == 0) load_scales(s + 1, TURN + 1);
-            __builtin_amdgcn_sched_barrier(0);  // the reads go ahead of the products they pass under
-            multiply(kk, kk & 1, SET);
-            __builtin_amdgcn_sched_barrier(0);
+        auto read = [&](const char* from, int kk) { return [&, from, kk](int r) __attribute__((always_inline)) { load_one(from, kk, kk & 1, r); }; };
+        auto fetch = [&](char* to, int ahead) {
+            return [&, to, ahead](int n) __attribute__((always_inline)) { move_one(to, s + ahead, (TURN + ahead) & 3, n); };
         };
-        inner(std::integral_constant<int, 0>{});
-        inner(std::integral_constant<int, 1>{});
-        inner(std::integral_constant<int, 2>{});
-        open(std::integral_constant<int, NEXT>{}, now, s + 1);
-        load(next, 0, 0);
+        if (NST == 2 && (TURN & 1) == 0) load_scales(s + 1, TURN + 1);
+        multiply(std::integral_constant<int, 0>{}, SET, read(now, 1), fetch(before, NST - 1), FIRST, ALL);
+        multiply(std::integral_constant<int, 1>{}, SET, read(now, 2), [](int) {}, 0, 0);
+        multiply(std::integral_constant<int, 2>{}, SET, read(now, 3), [](int) {}, 0, 0);
+        open(std::integral_constant<int, NEXT>{});
         if (NST == 2 && (TURN & 1) == 1) load_scales(s + 1, NEXT);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 3>{}, 1, SET);
+        multiply(std::integral_constant<int, 3>{}, SET, read(next, 0), fetch(now, NST), 0, FIRST);
         if (NST == 4 && TURN == 3) load_scales(s + 1, 0);
     };
-    open(std::integral_constant<int, 0>{}, NST == 2 ? s1 : s3, 0);
+    open(std::integral_constant<int, 0>{});
+#pragma unroll
+    for (int n = 0; n < FIRST; ++n) move_one(NST == 2 ? s1 : s3, NST - 1, NST - 1, n);
     load(s0, 0, 0);
     load_scales(0, 0);
     for (int s = 0; s < steps; s += TURNS) {  // an odd number of stages: one of zeros behind them
-        step(std::integral_constant<int, 0>{}, s0, s1, s);
-        step(std::integral_constant<int, 1>{}, s1, NST > 2 ? s2 : s0, s + 1);
+        step(std::integral_constant<int, 0>{}, NST > 2 ? s3 : s1, s0, s1, s);
+        step(std::integral_constant<int, 1>{}, s0, s1, NST > 2 ? s2 : s0, s + 1);
         if constexpr (TURNS > 2) {
             if (BREAK && s + 2 >= steps) break;
-            step(std::integral_constant<int, 2>{}, NST > 2 ? s2 : s0, NST > 2 ? s3 : s1, s + 2);
-            step(std::integral_constant<int, 3>{}, NST > 2 ? s3 : s1, s0, s + 3);
+            step(std::integral_constant<int, 2>{}, s1, NST > 2 ? s2 : s0, NST > 2 ? s3 : s1, s + 2);
+            step(std::integral_constant<int, 3>{}, NST > 2 ? s2 : s0, NST > 2 ? s3 : s1, s0, s + 3);
         }
     }
     wait_vm<0>();  // no load may come when the LDS holds outputs, or is another workgroup's

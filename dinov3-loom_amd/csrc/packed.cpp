@@ -210,6 +210,7 @@ void norm_check(const dhx_packed_norm& p) {
         pointer(p.h, 16, "h", work);
         stride(p.h_stride, p.channels, "h_stride");
         if (p.h && p.h == p.y && p.h_stride != p.y_stride) throw Error("in place, h_stride must be y_stride");
+        if (work && p.h == p.x_out) throw Error("h and x_out must not be the same");
     } else if (p.h) {
         throw Error("h needs a norm in pre");
     }

@@ -162,7 +162,8 @@ int dhx_packed_attention_run(dhx_engine *e, const dhx_packed_attention *p, void 
  * gate, zeros for bias. Statistics, sums and the x_out that pre takes are float32:
  * h does not see x_out's rounding to its type. A row with a value that is not
  * finite has outputs that are not, others are not touched by it; a row whose
- * squares pass the range of float32 gives zeros (v / infinity) or NaN.
+ * squares pass the range of float32 gives zeros (v / infinity) or NaN, and one whose
+ * mean square (LayerNorm: variance) and eps are both 0 gives NaN.
  * x_out may be x and h may be y, with the same stride (in place). */
 enum { DHX_NORM_NONE = 0, DHX_NORM_RMS = 1, DHX_NORM_LAYER = 2 };
 

@@ -186,8 +186,25 @@ def test_norm_of_large_means(eng):
     run_norm(eng, x, None, None, h, "none", "layer")
     torch.cuda.synchronize()
     want = torch.nn.functional.layer_norm(x.double(), (384,), eps=1e-6)
-    # the mean is off by at most 9 roundings of 1000 (8 + 1 + the tree's 6 and the product, each under F 1000)
+    # the mean of 1000 passes at most 8 sums in a lane, 6 across lanes and two roundings
+    # (of 1 / 384 and the product), each under F 1001
     within(h, want, 17 * F * 1001 * 1.2 + 17 * F * want.abs(), torch.float16)
+
+
+def test_norm_of_rows_past_the_range_and_of_zeros(eng):
+    # As the header says: squares past float32's range, and 0 / 0 with eps 0; their
+    # neighbours are untouched.
+    for channels in (64, 384, 4096):
+        x = torch.ones(4, channels, dtype=torch.bfloat16, device="cuda")
+        x[1] = 1e30
+        x[2] = 0.0
+        h = torch.empty_like(x)
+        run_norm(eng, x, None, None, h, "none", "rms", eps=(0.0, 0.0))
+        torch.cuda.synchronize()
+        assert (h[0] == 1).all() and (h[3] == 1).all() and (h[1] == 0).all() and h[2].isnan().all()
+        run_norm(eng, x, None, None, h, "none", "layer", eps=(0.0, 1e-5))
+        torch.cuda.synchronize()
+        assert (h[[0, 2, 3]] == 0).all()
 
 
 # --- 4 bits ------------------------------------------------------------------

@@ -71,6 +71,7 @@ REFUSED = [
     ("norm", dict(h_stride=0), "h_stride must be at least 384"),
     ("norm", dict(x_out=A, x_out_stride=392), "in place, x_out_stride must be x_stride"),
     ("norm", dict(h=2 * A, h_stride=392), "in place, h_stride must be y_stride"),
+    ("norm", dict(h=3 * A), "h and x_out must not be the same"),
     ("norm", dict(scale=A + 4), "scale must be 16-byte aligned"),
     ("norm", dict(gate=A + 8), "gate must be 16-byte aligned"),
     ("norm", dict(gate_stride=100), "gate_stride must be a multiple of 8"),
