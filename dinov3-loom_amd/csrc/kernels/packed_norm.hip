@@ -116,7 +116,7 @@ __device__ __forceinline__ float inverse(float (&v)[P][8], const bool (&there)[P
         for (int p = 0; p < P; ++p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum += v[p][e];
-        const float mean = row_sum<G>(sum, part) * each;
+        const float mean = row_sum<G>(sum, part) / (float)channels;  // a row of one value has no deviations
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll

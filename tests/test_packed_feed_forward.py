@@ -19,10 +19,10 @@ NORM = dict(type=packed.F16, stream_type=packed.F16, post=packed.RMS, pre=packed
             pre_eps=0.0, x=A, y=2 * A, x_out=3 * A, h=4 * A, post_weight=A, pre_weight=A, pre_bias=A, scale=A, gate=A, x_stride=384,
             y_stride=384, x_out_stride=384, h_stride=384, gate_stride=384, starts=A)
 QUANTISATION = dict(type=packed.BF16, rows=10, columns=1000, x=A, codes=A, scales=A, x_stride=1000, codes_stride=512, scales_stride=32)
-QUANTISED_LINEAR = dict(type=packed.BF16, sequences=3, rows=100, inputs=1000, outputs=128, x=A, w=A, w_scales=A, bias=A, y=A, x_stride=1000,
-                        y_stride=128, w_stride=512, scales_stride=32, starts=A, workspace=A, workspace_bytes=1 << 30)
-GATED = dict(type=packed.F16, activation=packed.SILU, rows=100, inputs=64, outputs=128, x=A, gate=A, up=A, out=A, x_stride=64,
-             out_stride=128, w_stride=64)
+QUANTISED_LINEAR = dict(type=packed.BF16, sequences=3, rows=1000, inputs=1000, outputs=1280, x=A, w=A, w_scales=A, bias=A, y=A, x_stride=1000,
+                        y_stride=1280, w_stride=512, scales_stride=32, starts=A, workspace=A, workspace_bytes=1 << 30)
+GATED = dict(type=packed.F16, activation=packed.SILU, rows=1000, inputs=64, outputs=1280, x=A, gate=A, up=A, out=A, x_stride=64,
+             out_stride=1280, w_stride=64)
 GATED_FOUR = dict(GATED, gate_scales=A, up_scales=A, w_stride=32, scales_stride=16, workspace=A, workspace_bytes=1 << 20)
 CALLS = {"norm": ("norm", packed.Norm, NORM), "quantise": ("quantise", packed.Quantisation, QUANTISATION),
          "dequantise": ("dequantise", packed.Quantisation, QUANTISATION),
@@ -112,7 +112,7 @@ REFUSED = [
     ("quantised_linear", dict(y=0), "y is a null device pointer"),
     ("quantised_linear", dict(w_stride=496), "w_stride must be at least 512"),
     ("quantised_linear", dict(scales_stride=24), "scales_stride must be a multiple of 16"),
-    ("quantised_linear", dict(y_stride=120), "y_stride must be at least 128"),
+    ("quantised_linear", dict(y_stride=1272), "y_stride must be at least 1280"),
     ("quantised_linear", dict(starts=0), "starts is a null device pointer"),
     ("quantised_linear", dict(workspace_bytes=100), "the workspace has 100 bytes"),
     ("quantised_linear", dict(workspace=A + 8), "workspace must be 16-byte aligned"),
@@ -126,7 +126,7 @@ REFUSED = [
     ("gated", dict(up_bias=A + 8), "up_bias must be 16-byte aligned"),
     ("gated", dict(out=0), "out is a null device pointer"),
     ("gated", dict(w_stride=56), "w_stride must be at least 64"),
-    ("gated", dict(out_stride=120), "out_stride must be at least 128"),
+    ("gated", dict(out_stride=1272), "out_stride must be at least 1280"),
     ("gated_four", dict(w_stride=16), "w_stride must be at least 32"),
     ("gated_four", dict(scales_stride=0), "scales_stride must be at least 16"),
     ("gated_four", dict(up_scales=A + 1), "up_scales must be 16-byte aligned"),
@@ -150,7 +150,7 @@ def test_what_may_be_missing():
 
 
 def test_workspaces():
-    for name, least in (("quantised_linear", 100 * (512 + 32)), ("gated_four", 100 * (32 + 16))):
+    for name, least in (("quantised_linear", 1000 * (512 + 32)), ("gated_four", 1000 * (32 + 16))):
         function, kind, fields = CALLS[name]
         need = d.packed_workspace(function, kind(**fields))
         assert need >= least
@@ -160,6 +160,10 @@ def test_workspaces():
         with pytest.raises(d.DINOv3Error, match="inputs must be"):
             d.packed_workspace(function, kind(**{**fields, "inputs": 12}))
     assert d.packed_workspace("gated", packed.Gated(**GATED)) == 0
+    # Few rows are quantised by the product itself.
+    assert d.packed_workspace("gated", packed.Gated(**{**GATED_FOUR, "rows": 24})) == 0
+    assert message("gated_four", rows=24, workspace=0, workspace_bytes=0) == "null engine"
+    assert d.packed_workspace("quantised_linear", packed.QuantisedLinear(**{**QUANTISED_LINEAR, "rows": 1})) == 0
     assert d._lib.dhx_packed_gated_workspace(None, None) == 1
 
 
