@@ -1,8 +1,9 @@
 """The operators on packed batches (include/dinov3_packed.h): a projection with
 low-rank adapters, the position rotation, attention, and the feed-forward half of a
 block (norms with the residual step between them, the gated projection, rows and
-weights in 4 bits), over the rows of many sequences that lie back to back. A call is described once, with device
-addresses as integers, and run by an Engine any number of times:
+weights in 4 bits), over the rows of many sequences that lie back to back. A call is
+described once, with device addresses as integers, and run by an Engine any number
+of times:
 
     from dinov3_hrx import Engine, packed
     call = packed.Attention(type=packed.BF16, causal=1, sequences=n, heads=32, kv_heads=8, head_dim=128, ...)
