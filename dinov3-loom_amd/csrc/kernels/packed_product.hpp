@@ -568,24 +568,32 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
 // that quantises x), linear: 1024 -> 1024, 1 row 3.2 and 5.9, 32 rows 4.2 and 6.6; 4096 ->
 // 4096, 1 row 4.8 and 10.0, 24 rows 9.6 and 10.7, 32 rows 11.4 and 10.9; 16384 -> 4096, 16
 // rows 21.5 and 28.3, 24 rows 29.8 and 28.4; 4096 -> 16384 (1024 blocks of 16 outputs), 8
-// rows 12.5 and 13.0, 16 rows 14.2 and 13.3. In several blocks of 32 rows: 1024 -> 1024,
-// 256 rows (512 workgroups) 6.1 and 6.9, 512 rows 9.8 and 7.0; 2048 -> 2048, 64 rows (256)
-// 6.5 and 8.5, 128 rows 9.7 and 8.7; gated, 1024 -> 2728, 64 rows (342) 7.3 and 7.0, 384 ->
-// 1536, 128 rows (384) 4.9 and 6.2.
+// rows 12.5 and 13.0, 16 rows 14.2 and 13.3. In several blocks of 32 rows: 384 -> 384,
+// 1024 rows (768 pairs of a row block and 16 outputs) 5.0 and 5.9, 2048 rows (1536) 7.1 and
+// 6.0; 136 -> 1848, 256 rows (928) 5.2 and 6.1; 1024 -> 1024, 256 rows (512) 5.1 and 7.1,
+// 512 rows (1024) 7.2 and 7.1; 2048 -> 2048, 128 rows (512) 7.5 and 9.0, 256 rows (1024)
+// 11.5 and 9.3; gated, 384 -> 1536, 256 rows (768) 6.3 and 6.4; 1024 -> 2728, 64 rows (342)
+// 6.6 and 7.3, 128 rows (684) 8.5 and 7.4.
 inline bool few_product(uint64_t rows, uint64_t inputs, uint64_t outputs, bool gated) {
     const uint64_t blocks = (outputs + 15) / 16, all = (rows + 31) / 32 * blocks;
     if (rows <= 8) return blocks <= 256 || inputs <= 4096;
     if (rows <= 32) return blocks <= 256 && (rows <= 16 || rows * inputs <= 24 * 4096);
-    return all <= 512 && inputs <= 2048 && all * inputs * (gated ? 2 : 1) <= 512 * 1024;
+    return all < 1024 && inputs <= 2048 && all * inputs * (gated ? 2 : 1) <= 1024 * 1024;
 }
 
 // p.x is the call's own here, in 16 bits, and p.pieces the columns of it. Two
-// workgroups of 16 rows run on a CU, one of 32.
+// workgroups of 16 rows run on a CU, one of 32. A workgroup that takes several blocks of
+// 16 outputs quantises its rows once for all of them. Several blocks of rows are best in
+// one round of workgroups from 1024 inputs on, where that costs most (us of one round, of
+// two, of a workgroup for every 16 outputs: 1024 -> 1024, 256 rows 5.1, 6.1, 6.0; 2048 ->
+// 2048, 128 rows 7.5, 9.7, 9.7), and in two below (384 -> 1152, 512 rows 6.3, 5.8, 8.6; 552
+// -> 3320, 128 rows 6.3, 5.8, 8.2; gated, 384 -> 1536, 128 rows 5.4, 4.8, 4.8).
 template <class T, bool GATED, int XB, int QUADS>
 hipError_t launch_few(const Product& p, hipStream_t s) {
     uint32_t blocks = (p.outputs + 15) / 16;
-    if (p.pieces <= 128 * QUADS * kFewProductWaves) blocks = std::min(blocks, XB == 1 ? 512u : 256u);
-    return enqueue(packed_product_few_kernel<T, GATED, XB, QUADS>, dim3(blocks, (p.rows + 16 * XB - 1) / (16 * XB)),
+    const uint32_t row_blocks = (p.rows + 16 * XB - 1) / (16 * XB), at_once = XB == 1 || (row_blocks > 1 && p.pieces < 1024) ? 512 : 256;
+    if (p.pieces <= 128 * QUADS * kFewProductWaves) blocks = std::min(blocks, std::max(1u, at_once / row_blocks));
+    return enqueue(packed_product_few_kernel<T, GATED, XB, QUADS>, dim3(blocks, row_blocks),
                    dim3(64 * kFewProductWaves), 0, s, p.x, p.w, p.up,
                    (int)p.rows, (int)p.pieces, (int)p.outputs, (uint32_t)p.x_stride, (uint32_t)p.w_stride, p.starts, p.ws, p.us, p.bias,
                    p.up_bias, p.out, p.out_stride, (int)p.sequences, (int)p.activation, (uint32_t)p.ws_stride);
