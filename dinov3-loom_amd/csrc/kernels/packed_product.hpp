@@ -563,35 +563,33 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
     }
 }
 
-// Whether the few-rows kernel takes a call. Every workgroup quantises all of its rows
-// of x, so that rows x inputs is what it costs. us against tiles (with their launch
-// that quantises x), linear: 1024 -> 1024, 1 row 3.2 and 5.9, 32 rows 4.2 and 6.6; 4096 ->
-// 4096, 1 row 4.8 and 10.0, 24 rows 9.6 and 10.7, 32 rows 11.4 and 10.9; 16384 -> 4096, 16
-// rows 21.5 and 28.3, 24 rows 29.8 and 28.4; 4096 -> 16384 (1024 blocks of 16 outputs), 8
-// rows 12.5 and 13.0, 16 rows 14.2 and 13.3. In several blocks of 32 rows: 384 -> 384,
-// 1024 rows (768 pairs of a row block and 16 outputs) 5.0 and 5.9, 2048 rows (1536) 7.1 and
-// 6.0; 136 -> 1848, 256 rows (928) 5.2 and 6.1; 1024 -> 1024, 256 rows (512) 5.1 and 7.1,
-// 512 rows (1024) 7.2 and 7.1; 2048 -> 2048, 128 rows (512) 7.5 and 9.0, 256 rows (1024)
-// 11.5 and 9.3; gated, 384 -> 1536, 256 rows (768) 6.3 and 6.4; 1024 -> 2728, 64 rows (342)
-// 6.6 and 7.3, 128 rows (684) 8.5 and 7.4.
+// Whether the few-rows kernel takes a call, by its pairs of 16 rows and 16 outputs, of
+// which a gated one has two products. us against tiles (with their launch that quantises
+// x), linear: 1024 -> 1024, 1 row 3.2 and 5.9, 64 rows (256 pairs) 3.5 and 6.9; 4096 ->
+// 4096, 1 row 4.8 and 10.0, 32 rows (512) 10.7 and 11.4, 48 rows (768) 13.6 and 11.8; 4096
+// -> 16384 (1024), 8 rows 12.5 and 13.0, 16 rows 14.2 and 13.3; 16384 -> 128, 512 rows (256)
+// 25.0 and 29.6, 1000 rows (504) 45.2 and 31.2; short rows: 384 -> 384, 1024 rows (1536)
+// 4.7 and 5.9, 2048 rows 6.9 and 6.1; 1024 -> 1024, 256 rows (1024) 5.1 and 7.0, 512 rows
+// 7.2 and 7.1; 2048 -> 2048, 128 rows (1024) 7.6 and 9.0, 256 rows 11.5 and 9.3. Gated:
+// 4096 -> 512, 128 rows (256) 9.5 and 12.6, 256 rows 15.0 and 12.8; 1024 -> 2728, 64 rows
+// (684) 6.6 and 7.3, 128 rows 8.5 and 7.4; 384 -> 1536, 128 rows (768) 5.0 and 6.3, 256
+// rows 6.3 and 6.4.
 inline bool few_product(uint64_t rows, uint64_t inputs, uint64_t outputs, bool gated) {
-    const uint64_t blocks = (outputs + 15) / 16, all = (rows + 31) / 32 * blocks;
+    const uint64_t blocks = (outputs + 15) / 16, all = (rows + 15) / 16 * blocks * (gated ? 2 : 1);
     if (rows <= 8) return blocks <= 256 || inputs <= 4096;
-    if (rows <= 32) return blocks <= 256 && (rows <= 16 || rows * inputs <= 24 * 4096);
-    return all < 1024 && inputs <= 2048 && all * inputs * (gated ? 2 : 1) <= 1024 * 1024;
+    if (all <= 256 || (all <= 512 && (gated || inputs <= 4096))) return true;
+    return all <= 2048 && inputs <= 2048 && all * inputs <= 2048 * 1024;
 }
 
 // p.x is the call's own here, in 16 bits, and p.pieces the columns of it. Two
 // workgroups of 16 rows run on a CU, one of 32. A workgroup that takes several blocks of
-// 16 outputs quantises its rows once for all of them. Several blocks of rows are best in
-// one round of workgroups from 1024 inputs on, where that costs most (us of one round, of
-// two, of a workgroup for every 16 outputs: 1024 -> 1024, 256 rows 5.1, 6.1, 6.0; 2048 ->
-// 2048, 128 rows 7.5, 9.7, 9.7), and in two below (384 -> 1152, 512 rows 6.3, 5.8, 8.6; 552
-// -> 3320, 128 rows 6.3, 5.8, 8.2; gated, 384 -> 1536, 128 rows 5.4, 4.8, 4.8).
+// 16 outputs quantises its rows once for all of them, so that one round of workgroups is
+// better than one for every block (32 rows: 1024 -> 1024, 256 rows 5.1 us and 6.0; 384 ->
+// 1152, 512 rows 6.3 and 8.6).
 template <class T, bool GATED, int XB, int QUADS>
 hipError_t launch_few(const Product& p, hipStream_t s) {
     uint32_t blocks = (p.outputs + 15) / 16;
-    const uint32_t row_blocks = (p.rows + 16 * XB - 1) / (16 * XB), at_once = XB == 1 || (row_blocks > 1 && p.pieces < 1024) ? 512 : 256;
+    const uint32_t row_blocks = (p.rows + 16 * XB - 1) / (16 * XB), at_once = XB == 1 ? 512 : 256;
     if (p.pieces <= 128 * QUADS * kFewProductWaves) blocks = std::min(blocks, std::max(1u, at_once / row_blocks));
     return enqueue(packed_product_few_kernel<T, GATED, XB, QUADS>, dim3(blocks, row_blocks),
                    dim3(64 * kFewProductWaves), 0, s, p.x, p.w, p.up,
@@ -601,12 +599,21 @@ hipError_t launch_few(const Product& p, hipStream_t s) {
 template <class T, bool GATED, int XB>
 hipError_t launch_few_columns(const Product& p, hipStream_t s) {
     if (p.pieces <= 1024) return launch_few<T, GATED, XB, 1>(p, s);
-    if (p.pieces <= 2048) return launch_few<T, GATED, XB, 2>(p, s);
-    return launch_few<T, GATED, XB, 4>(p, s);
+    if constexpr (XB == 1) {
+        if (p.pieces > 2048) return launch_few<T, GATED, 1, 4>(p, s);
+    }
+    return launch_few<T, GATED, XB, 2>(p, s);
 }
+// Blocks of 16 rows take half as long as those of 32 to be quantised, and read the weights
+// twice as often. us of 16 and 32 rows: 1024 -> 1024, 64 rows (256 pairs of 16 rows and 16
+// outputs) 3.5 and 4.3, 128 rows 4.6 and 4.3; gated, 128 rows 5.8 and 5.3; short rows: 640
+// -> 640, 256 rows (640) 4.4 and 4.7, 896 -> 2048, 128 rows (1024) 5.0 and 4.9; long ones:
+// 4096 -> 512, 256 rows (512) 11.1 and 11.6, 2048 -> 2048, 64 rows (512) 6.7 and 6.5.
 template <class T, bool GATED>
 hipError_t launch_few_rows(const Product& p, hipStream_t s) {
-    return p.rows <= 16 ? launch_few_columns<T, GATED, 1>(p, s) : launch_few_columns<T, GATED, 2>(p, s);
+    const uint64_t all = (p.rows + 15) / 16 * ((p.outputs + 15) / 16);
+    if (p.rows <= 16 || all <= 256 || p.pieces <= 768 || p.pieces > 2048) return launch_few_columns<T, GATED, 1>(p, s);
+    return launch_few_columns<T, GATED, 2>(p, s);
 }
 
 // The tile of a call, from the number of workgroups that each would make and the

@@ -283,9 +283,10 @@ def test_on_engine_regions_and_the_engines_stream(eng):
 # 4, 8 and 16 blocks, more steps than waves, more outputs than workgroups take at
 # once, several blocks of rows).
 GATED = [(2300, 200, 2304), (300, 776, 5000), (3000, 136, 1504), (200, 776, 4000), (1000, 136, 1200), (50, 800, 264), (300, 136, 1000)]
-GATED4 = [(2300, 1000, 2304), (3000, 136, 1504), (200, 2888, 4000), (1000, 136, 1200), (50, 2888, 264), (600, 136, 1000)]
-LINEAR4 = [(3400, 1000, 3304), (3000, 136, 2600), (300, 2888, 4104), (2000, 136, 2000), (50, 2888, 520), (700, 136, 1400)]
-FEW = [(3, 1000, 9000), (5, 8200, 304), (20, 1504, 504), (30, 2400, 104), (100, 304, 200), (24, 1000, 1000), (1, 16, 8)]
+GATED4 = [(2300, 1000, 2304), (3000, 136, 1504), (200, 2888, 4000), (1000, 136, 1200), (50, 2888, 264), (600, 136, 1000), (100, 2888, 1000)]
+LINEAR4 = [(3400, 1000, 3304), (3000, 136, 2600), (300, 2888, 4104), (2000, 136, 2000), (50, 2888, 520), (700, 136, 1400), (100, 2888, 2000)]
+FEW = [(3, 1000, 9000), (5, 8200, 304), (20, 1504, 504), (30, 2400, 104), (100, 304, 200), (24, 1000, 1000), (1, 16, 8),
+       (100, 1000, 1000), (150, 1504, 1000), (100, 304, 2000), (100, 5000, 200), (40, 2400, 1000)]
 CASES = [("gated", *c) for c in GATED] + [("gated4", *c) for c in GATED4 + FEW] + [("linear4", *c) for c in LINEAR4 + FEW]
 
 
@@ -441,15 +442,22 @@ def test_refusals_change_nothing_and_failures_poison(gpu):
     run = lambda pre: run_norm(e, x, None, None, out, "none", pre)  # noqa: E731
     with pytest.raises(d.DINOv3Error, match="pre is needed"):
         e.packed_norm(packed.Norm(type=packed.F16, rows=4, channels=64, x=at(x), x_stride=64))
-    many, y = torch.ones(64, 2056, device="cuda").half(), torch.full((64, 64), 7.0, device="cuda").half()
-    codes, scales = quantised(e, many)
-    call = packed.QuantisedLinear(type=packed.F16, rows=64, inputs=2056, outputs=64, x=at(many), w=at(codes), w_scales=at(scales), y=at(y),
-                                  x_stride=2056, y_stride=64, w_stride=codes.shape[1], scales_stride=scales.shape[1])
-    assert e.packed_quantised_linear_workspace(call) > 0
-    with pytest.raises(d.DINOv3Error, match="the call needs"):
-        e.packed_quantised_linear(call)
-    torch.cuda.synchronize()
-    assert (out == 7.0).all() and (y == 7.0).all()
+    for rows, outputs in ((64, 64), (400, 1000)):
+        many, y = torch.ones(rows, 2056, device="cuda").half(), torch.full((rows, outputs), 7.0, device="cuda").half()
+        codes, scales = quantised(e, torch.ones(outputs, 2056, device="cuda").half())
+        call = packed.QuantisedLinear(type=packed.F16, rows=rows, inputs=2056, outputs=outputs, x=at(many), w=at(codes), w_scales=at(scales),
+                                      y=at(y), x_stride=2056, y_stride=outputs, w_stride=codes.shape[1], scales_stride=scales.shape[1])
+        if rows == 64:  # few rows need no workspace, and run without one
+            assert e.packed_quantised_linear_workspace(call) == 0
+            e.packed_quantised_linear(call)
+            torch.cuda.synchronize()
+            assert (y == 2056.0).all()
+            continue
+        assert e.packed_quantised_linear_workspace(call) > 0
+        with pytest.raises(d.DINOv3Error, match="the call needs"):
+            e.packed_quantised_linear(call)
+        torch.cuda.synchronize()
+        assert (out == 7.0).all() and (y == 7.0).all()
     run("rms")
     torch.cuda.synchronize()
     assert (out == 1.0).all()
