@@ -440,6 +440,44 @@ hipError_t launch_tiles(const Product& p, hipStream_t s) {
                            dim3(64 * (BM / WM) * (BN / WN)), s, p);
 }
 
+// The end of a workgroup of few rows: its waves' parts of 16 outputs of 16 XB rows from
+// row0 on are joined in LDS, and the rows in first .. end-1 are stored. A lane's part:
+// row 16 m + lane % 16, columns 4 (lane / 16) .. +3.
+constexpr int kFewProductWaves = 8;
+template <class T, bool GATED, int XB>
+__device__ __forceinline__ void store_few(float (*sum)[kFewProductWaves][16 * XB][20], const float4_t (*acc)[XB], int col0, int row0, int first,
+                                          int end, int outputs, int activation, Addr bias_, Addr up_bias_, Addr out_, uint64_t out_stride) {
+    constexpr int AB = GATED ? 2 : 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+    for (int a = 0; a < AB; ++a)
+#pragma unroll
+        for (int m = 0; m < XB; ++m) *(float4_t*)&sum[a][wave][m * 16 + (lane & 15)][4 * (lane >> 4)] = acc[a][m];
+    lds_barrier();
+    const int r = tid >> 2, row = row0 + r, c = (tid & 3) * 4, col = col0 + c;
+    if (r < 16 * XB && row >= first && row < end && col < outputs) {
+        float4_t v[AB] = {};
+#pragma unroll
+        for (int a = 0; a < AB; ++a) {
+#pragma unroll
+            for (int i = 0; i < kFewProductWaves; ++i) v[a] += *(const float4_t*)&sum[a][i][r][c];
+            const float* bias = a ? up_bias_ : bias_;
+            if (bias) v[a] += *(const float4_t*)(bias + col);
+        }
+        typename Num<T>::v4 o;
+        if constexpr (GATED) {
+            with_activation(activation, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (T)(v[1][e] * activated<decltype(act)::value>(v[0][e]));
+            });
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (T)v[0][e];
+        }
+        *(typename Num<T>::v4*)((T*)out_ + (uint64_t)row * out_stride + col) = o;
+    }
+}
+
 // Few rows against 4-bit weights, which are all there is to read: a workgroup takes
 // 16 outputs at a time (gated: and both of their sums) and 16 XB rows, its
 // waves share the columns out in steps of QUADS * 4 blocks and join their sums in LDS.
@@ -448,7 +486,6 @@ hipError_t launch_tiles(const Product& p, hipStream_t s) {
 // has no more than one step, a workgroup takes further outputs with the x it has.
 #define DHX_FEW_PARAMS Addr x_, Addr w_, Addr up_, int rows, int inputs, int outputs, uint32_t x_stride, uint32_t w_stride, Addr starts_, Addr ws_, Addr us_, Addr bias_, Addr up_bias_, Addr out_, uint64_t out_stride, int sequences, int activation, uint32_t ws_stride
 
-constexpr int kFewProductWaves = 8;
 template <class T, bool GATED, int XB, int QUADS>
 __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kernel(DHX_FEW_PARAMS) {
     typedef typename Num<T>::v8 v8;
@@ -531,34 +568,7 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
                 }
         }
         if (wave < steps && block + (int)gridDim.x < blocks) load_weights(block + gridDim.x, wave);
-        // Lane: row 16 m + l16, columns 4 part .. +3.
-#pragma unroll
-        for (int a = 0; a < AB; ++a)
-#pragma unroll
-            for (int m = 0; m < XB; ++m) *(float4_t*)&sum[a][wave][m * 16 + l16][4 * part] = acc[a][m];
-        lds_barrier();
-        const int r = tid >> 2, row = row0 + r, c = (tid & 3) * 4, col = block * 16 + c;
-        if (r < mine && row >= first && row < end && col < outputs) {
-            float4_t v[AB] = {};
-#pragma unroll
-            for (int a = 0; a < AB; ++a) {
-#pragma unroll
-                for (int i = 0; i < WAVES; ++i) v[a] += *(const float4_t*)&sum[a][i][r][c];
-                const float* bias = a ? up_bias_ : bias_;
-                if (bias) v[a] += *(const float4_t*)(bias + col);
-            }
-            typename Num<T>::v4 o;
-            if constexpr (GATED) {
-                with_activation(activation, [&](auto act) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = (T)(v[1][e] * activated<decltype(act)::value>(v[0][e]));
-                });
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (T)v[0][e];
-            }
-            *(typename Num<T>::v4*)((T*)out_ + (uint64_t)row * out_stride + col) = o;
-        }
+        store_few<T, GATED, XB>(sum, acc, block * 16, row0, first, min(end, rows), outputs, activation, bias_, up_bias_, out_, out_stride);
         lds_barrier();  // the sums have been read
     }
 }

@@ -24,7 +24,7 @@ def loads_from_buffers_too(monkeypatch):
 
 
 @pytest.mark.parametrize("src,kernels,with_dma", [
-    ("packed_gated.hip", ("packed_product_kernel", "packed_product_few_kernel"), ("packed_product_kernel",)),
+    ("packed_gated.hip", ("packed_product_kernel", "packed_product_few_kernel", "packed_gated_few_kernel"), ("packed_product_kernel",)),
     ("packed_quantised.hip", ("packed_product_kernel", "packed_product_few_kernel"), ("packed_product_kernel",)),
     ("packed_norm.hip", ("packed_norm_kernel",), ()),
     ("packed_quantise.hip", ("packed_quantise_kernel", "packed_dequantise_kernel"), ()),
