@@ -283,7 +283,8 @@ def test_on_engine_regions_and_the_engines_stream(eng):
 # 4, 8 and 16 blocks, more steps than waves, more outputs than workgroups take at
 # once, several blocks of rows).
 GATED = [(2300, 200, 2304), (300, 776, 5000), (3000, 136, 1504), (200, 776, 4000), (1000, 136, 1200), (50, 800, 264), (300, 136, 1000), (100, 800, 1000)]
-FEW_GATED = [(16, 2056, 8200), (100, 1032, 520), (130, 1032, 520), (70, 1504, 1000), (40, 8200, 200), (3, 136, 1000), (1, 16, 8), (20, 1504, 8)]
+FEW_GATED = [(16, 2056, 8200), (100, 1032, 520), (130, 1032, 520), (70, 1504, 1000), (40, 8200, 200), (3, 136, 1000), (1, 16, 8), (20, 1504, 8),
+             (20, 1032, 8200), (100, 2056, 2000), (300, 800, 1000), (5, 136, 9000)]
 GATED4 = [(2300, 1000, 2304), (3000, 136, 1504), (200, 2888, 4000), (1000, 136, 1200), (50, 2888, 264), (600, 136, 1000), (100, 2888, 1000)]
 LINEAR4 = [(3400, 1000, 3304), (3000, 136, 2600), (300, 2888, 4104), (2000, 136, 2000), (50, 2888, 520), (700, 136, 1400), (100, 2888, 2000)]
 FEW = [(3, 1000, 9000), (5, 8200, 304), (20, 1504, 504), (30, 2400, 104), (100, 304, 200), (24, 1000, 1000), (1, 16, 8),
