@@ -40,6 +40,23 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
     return v;
 }
 
+// The value of a row's first lane (of those of row_sum), in all of them.
+template <int G>
+__device__ __forceinline__ float row_first(float v, float* part) {
+    if constexpr (G < 64) {
+        int first = __builtin_bit_cast(int, v);
+        first = __builtin_amdgcn_update_dpp(first, first, 0x000, 0xf, 0xf, false);  // quad_perm 0, 0, 0, 0
+        first = __builtin_amdgcn_update_dpp(first, first, 0x114, 0xf, 0xa, false);  // row_shr:4 into lanes 4-7 and 12-15
+        if constexpr (G >= 16) first = __builtin_amdgcn_update_dpp(first, first, 0x118, 0xf, 0xc, false);  // row_shr:8 into lanes 8-15
+        if constexpr (G >= 32) first = __builtin_amdgcn_update_dpp(first, first, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+        return __builtin_bit_cast(float, first);
+    }
+    if constexpr (G == 64) return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+    if (threadIdx.x == 0) *part = v;
+    __syncthreads();
+    return *part;
+}
+
 // The last sequence that does not begin behind row0 + mine, one of the ROWS rows
 // from row0 on that a wave holds; -1: none.
 template <int ROWS>
@@ -106,28 +123,57 @@ __device__ __forceinline__ void vector8(const float* vector, int c, float none, 
 
 // One over the row's root of its mean square, of P pieces of 8 channels a lane
 // (zeros where a piece does not exist); for LayerNorm of the deviations from the
-// mean, which it leaves in v. Both sums are of registers. part: 32 floats.
+// mean, which it leaves in v. Both sums are of registers.
+// A mean is off by some 30 roundings of itself (8 values of a lane, 6 steps across lanes, 16
+// waves), which deviations far smaller than the mean would show: a float32 row of one
+// value would have some, and its norm nothing else. Where the mean is more than 128 times
+// the deviations, which are exact so near to it, these are therefore taken from the first
+// of them, so that nothing is left of a row of one value, and then from their own mean.
+// Other rows pay a comparison (12864 rows of 384 channels 10.84 us without it and with;
+// held between every row's least and largest value, the mean would cost 0.5 us of it).
+// part: 48 floats, of which the last 16 are any.
 template <int G, int P>
 __device__ __forceinline__ float inverse(float (&v)[P][8], const bool (&there)[P], int kind, float eps, int channels, float* part) {
     const float each = 1.0f / (float)channels;
-    if (kind == DHX_NORM_LAYER) {
+    auto less = [&](float mean) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[p][e] = there[p] ? v[p][e] - mean : 0.f;
+    };
+    auto mean_of = [&]() __attribute__((always_inline)) {
         float sum = 0.f;
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum += v[p][e];
-        const float mean = row_sum<G>(sum, part) / (float)channels;  // a row of one value has no deviations
+        return row_sum<G>(sum, part) / (float)channels;
+    };
+    auto square = [&]() __attribute__((always_inline)) {
+        float sum = 0.f;
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[p][e] = there[p] ? v[p][e] - mean : 0.f;
+            for (int e = 0; e < 8; ++e) sum = fmaf(v[p][e], v[p][e], sum);
+        return row_sum<G>(sum, part + 16);
+    };
+    float mean = 0.f;
+    if (kind == DHX_NORM_LAYER) {
+        mean = mean_of();
+        less(mean);
     }
-    float sum = 0.f;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(v[p][e], v[p][e], sum);
-    return rsqrtf(fmaf(row_sum<G>(sum, part + 16), each, eps));
+    float all = square();
+    if (kind == DHX_NORM_LAYER) {
+        const bool near = mean != 0.f && all * each <= mean * mean * 0x1p-14f;
+        if (__any(near)) {
+            const float first = row_first<G>(v[0][0], part + 32);
+            less(near ? first : 0.f);
+            const float more = mean_of();
+            less(near ? more : 0.f);
+            all = square();
+        }
+    }
+    return rsqrtf(fmaf(all, each, eps));
 }
 
 // T: y and h, S: x and x'. G lanes (over 64: those of the workgroup, however many)
@@ -135,7 +181,7 @@ __device__ __forceinline__ float inverse(float (&v)[P][8], const bool (&there)[P
 template <class T, class S, int G, int P>
 __global__ __launch_bounds__(G <= 64 ? 256 : G) void packed_norm_kernel(DHX_NORM_PARAMS) {
     constexpr int ROWS = G <= 64 ? 256 / G : 1, WAVE_ROWS = G <= 64 ? 64 / G : 1;
-    __shared__ float part[G > 64 ? 64 : 1];  // 16 waves' sums, of four kinds
+    __shared__ float part[G > 64 ? 96 : 1];  // for each norm 16 waves' sums, of two kinds, and a value
     const S* x = x_;
     const T* y = y_;
     const int tid = threadIdx.x, lanes = G <= 64 ? G : blockDim.x, lane = G <= 64 ? tid % G : tid, in_wave = G <= 64 ? (tid & 63) / G : 0;
@@ -147,7 +193,7 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void packed_norm_kernel(DHX_NORM
         there[p] = lanes * p + lane < pieces;
         at[p] = (lanes * p + lane) * 8;
     }
-    if (G > 64 && tid < 64 && tid % 16 >= lanes >> 6) part[tid] = 0.f;
+    if (G > 64 && tid < 96 && tid % 16 >= lanes >> 6) part[tid] = 0.f;
     for (int64_t first = (int64_t)blockIdx.x * ROWS; first < rows; first += (int64_t)gridDim.x * ROWS) {
         const int in_block = G <= 64 ? tid / G : 0;
         const int64_t row = first + in_block;
@@ -210,7 +256,7 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void packed_norm_kernel(DHX_NORM
             }
         }
         if (pre != DHX_NORM_NONE) {
-            const float r = inverse<G, P>(v, there, pre, pre_eps, channels, part + 32);
+            const float r = inverse<G, P>(v, there, pre, pre_eps, channels, part + (G > 64 ? 48 : 0));
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 if constexpr (P > 1) pre_vectors(p, pre_by, pre_plus);
