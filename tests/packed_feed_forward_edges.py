@@ -1,13 +1,15 @@
 """The operators of the feed-forward half of a packed block at edges of their
-definitions: float32 rows of one value. Tolerances as in packed_feed_forward.py."""
+definitions: float32 rows of one value, activations far from zero. Tolerances as in packed_feed_forward.py."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import dinov3_hrx as d  # noqa: E402
 
-from packed_feed_forward import norm_want, run_norm  # noqa: E402
-from packed_operators import F, TYPES, gen, within  # noqa: E402
+from packed_feed_forward import ACTIVATIONS, activation_want, norm_want, run_gated, run_norm  # noqa: E402
+from packed_operators import F, TYPES, gen, normal, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +72,53 @@ def test_layer_norm_of_a_row_of_nearly_one_value(eng, t, channels):
     v = x.double() - x.double().mean(1, keepdim=True)
     want, e = norm_want(v, 2 * F * (v.abs() + v[:, :1].abs()), "rms", 0.0, w, b)
     within(h, want, e, dt)
+
+
+# --- activations -------------------------------------------------------------
+
+# Down to where the factor of g still has float32's whole precision (2^-126).
+LOWEST = {"silu": -86.0, "gelu": -12.5, "gelu_tanh": -9.9, "relu": -40.0, "sigmoid": -86.0}
+
+
+def far_activation_want(name, g):
+    """(act(g), its error) for exact g, relative to act(g) where g is negative."""
+    if name == "gelu_tanh":  # without the cancellation of 1 + tanh
+        inner = 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+        want = g * torch.sigmoid(inner)
+        return want, 1.1 * want.abs() * (6 * inner.abs() + 9) * F
+    if name != "gelu":
+        return activation_want(name, g, torch.zeros_like(g))
+    # Half of erfc: the polynomial's 2.6 F near 0, up to 300 times as much (780 F) where erfc
+    # is small; its argument 1 / (1 + c |g|) to 3 F, which the polynomial and its factor
+    # pass on up to 2.3 times; five steps with their coefficients 5 F; e^(-g^2 / 2) to 2 F
+    # and, of the three roundings of its argument, 1.5 g^2 F; two products. Then the last sum.
+    less = g.abs() * 0.5 * torch.special.erfc(g.abs() / math.sqrt(2))
+    want = g.clamp_min(0) - less
+    return want, 1.1 * less * (2.6 * (1 / torch.special.erfc(g.abs() / math.sqrt(2))).clamp_max(300) + 16 + 1.5 * g * g) * F + F * want.abs()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("rows", [3, 300])
+def test_activations_far_from_zero(eng, t, activation, bits, rows):
+    # Sums of nothing but the bias, with an up projection that brings what is left of
+    # a negative g back into the type's range.
+    dt = TYPES[t][1]
+    outputs, inputs = 1000, 64
+    gate_bias = torch.cat([torch.linspace(LOWEST[activation], -0.01, 800, device="cuda"), torch.linspace(0.01, 30, 200, device="cuda")])
+    want, e = far_activation_want(activation, gate_bias.double())
+    up_bias = (1 / want.clamp_min(1e-30) if activation == "relu" else 1 / want).clamp(-1e37, 1e37).float()
+    up_bias[want == 0] = 1.0
+    x = normal(gen(rows), dt, rows, inputs)
+    out = torch.empty(rows, outputs, dtype=dt, device="cuda")
+    if bits == 4:
+        codes, scales = (torch.zeros(outputs, n, dtype=torch.uint8, device="cuda") for n in (32, 16))
+        run_gated(eng, x, codes, codes, gate_bias, up_bias, out, activation, (scales, scales))
+    else:
+        none = torch.zeros(outputs, inputs, dtype=dt, device="cuda")
+        run_gated(eng, x, none, none, gate_bias, up_bias, out, activation)
+    torch.cuda.synchronize()
+    e = e * up_bias.double().abs()
+    want = want * up_bias.double()
+    within(out, want.expand(rows, outputs), (e + F * want.abs()).expand(rows, outputs), dt)
