@@ -203,6 +203,8 @@ void norm_check(const dhx_packed_norm& p) {
         stride(p.y_stride, p.channels, "y_stride");
         stride(p.x_out_stride, p.channels, "x_out_stride");
         if (work && p.x == p.x_out && p.x_stride != p.x_out_stride) throw Error("in place, x_out_stride must be x_stride");
+        if (work && p.y == p.x_out && (p.type != p.stream_type || p.y_stride != p.x_out_stride))
+            throw Error("x_out in the place of y must have its type, and x_out_stride be y_stride");
     } else if (work && (p.post != DHX_NORM_NONE || p.pre == DHX_NORM_NONE || p.scale || p.gate || p.x_out)) {
         throw Error("without y there are no post, scale, gate and x_out, and pre is needed");
     }
@@ -210,6 +212,8 @@ void norm_check(const dhx_packed_norm& p) {
         pointer(p.h, 16, "h", work);
         stride(p.h_stride, p.channels, "h_stride");
         if (p.h && p.h == p.y && p.h_stride != p.y_stride) throw Error("in place, h_stride must be y_stride");
+        if (work && p.h == p.x && (p.type != p.stream_type || p.h_stride != p.x_stride))
+            throw Error("h in the place of x must have its type, and h_stride be x_stride");
         if (work && p.h == p.x_out) throw Error("h and x_out must not be the same");
     } else if (p.h) {
         throw Error("h needs a norm in pre");

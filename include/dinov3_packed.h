@@ -164,7 +164,8 @@ int dhx_packed_attention_run(dhx_engine *e, const dhx_packed_attention *p, void 
  * finite has outputs that are not, others are not touched by it; a row whose
  * squares pass the range of float32 gives zeros (v / infinity) or NaN, and one whose
  * mean square (LayerNorm: variance) and eps are both 0 gives NaN.
- * x_out may be x and h may be y, with the same stride (in place). */
+ * x_out and h may each be x or y of the same type with the same stride (in place),
+ * but not both the same. */
 enum { DHX_NORM_NONE = 0, DHX_NORM_RMS = 1, DHX_NORM_LAYER = 2 };
 
 typedef struct dhx_packed_norm {

@@ -1,5 +1,6 @@
 """The operators of the feed-forward half of a packed block at edges of their
-definitions: float32 rows of one value, activations far from zero. Tolerances as in packed_feed_forward.py."""
+definitions: float32 rows of one value, outputs in the place
+of inputs, activations far from zero. Tolerances as in packed_feed_forward.py."""
 import math
 
 import pytest
@@ -72,6 +73,26 @@ def test_layer_norm_of_a_row_of_nearly_one_value(eng, t, channels):
     v = x.double() - x.double().mean(1, keepdim=True)
     want, e = norm_want(v, 2 * F * (v.abs() + v[:, :1].abs()), "rms", 0.0, w, b)
     within(h, want, e, dt)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("channels", [64, 384, 4096, 12288])
+def test_norm_in_place_the_other_way_round(eng, dt, channels):
+    # h where x was, x_out where y was.
+    g = gen(channels)
+    x, y = normal(g, dt, 33, channels), normal(g, dt, 33, channels)
+    for post, pre in (("none", "layer"), ("rms", "rms")):
+        out, h = torch.empty_like(x), torch.empty_like(x)
+        run_norm(eng, x, y, out, h, post, pre)
+        a, b = x.clone(), y.clone()
+        run_norm(eng, a, b, b, a, post, pre)
+        torch.cuda.synchronize()
+        assert torch.equal(a, h) and torch.equal(b, out)
+    a = x.clone()
+    run_norm(eng, x, None, None, h, "none", "rms")
+    run_norm(eng, a, None, None, a, "none", "rms")
+    torch.cuda.synchronize()
+    assert torch.equal(a, h)
 
 
 # --- activations -------------------------------------------------------------

@@ -1,0 +1,30 @@
+"""Calls of the feed-forward half of a packed block that lie at the edge of what is
+taken (CPU only: a null engine shows which check answers)."""
+import pytest
+
+import test_packed_feed_forward as calls
+from dinov3_hrx import packed
+from test_packed_feed_forward import PLAIN, A, message
+
+X, Y = calls.NORM["x"], calls.NORM["y"]
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(h=X, h_stride=392), "h in the place of x must have its type, and h_stride be x_stride"),
+    (dict(h=X, stream_type=packed.F32), "h in the place of x must have its type"),
+    (dict(PLAIN, h=X, h_stride=768), "h in the place of x must have its type"),
+    (dict(PLAIN, h=X, stream_type=packed.F32), "h in the place of x must have its type"),
+    (dict(x_out=Y, x_out_stride=392), "x_out in the place of y must have its type, and x_out_stride be y_stride"),
+    (dict(x_out=Y, stream_type=packed.F32), "x_out in the place of y must have its type"),
+    (dict(x_out=Y, h=Y), "h and x_out must not be the same"),
+    (dict(x_out=X, h=X), "h and x_out must not be the same"),
+])
+def test_outputs_in_the_place_of_inputs_refused(change, text):
+    # Rows of another size or distance would be written over rows that are not yet read.
+    assert text in message("norm", **change)
+
+
+def test_outputs_in_the_place_of_inputs_taken():
+    for change in (dict(h=X), dict(x_out=Y), dict(h=X, x_out=Y), dict(PLAIN, h=X), dict(x_out=X, h=Y), dict(x_out=X, h=Y, stream_type=packed.F32),
+                   dict(rows=0, x=0, y=A, x_out=A, h=0, stream_type=packed.F32)):
+        assert message("norm", **change) == "null engine", change
