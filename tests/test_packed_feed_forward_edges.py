@@ -1,5 +1,11 @@
 """Calls of the feed-forward half of a packed block that lie at the edge of what is
-taken (CPU only: a null engine shows which check answers)."""
+taken (CPU only: a null engine shows which check answers), and the documents'
+examples of them."""
+import ast
+import glob
+import os
+import re
+
 import pytest
 
 import test_packed_feed_forward as calls
@@ -28,3 +34,19 @@ def test_outputs_in_the_place_of_inputs_taken():
     for change in (dict(h=X), dict(x_out=Y), dict(h=X, x_out=Y), dict(PLAIN, h=X), dict(x_out=X, h=Y), dict(x_out=X, h=Y, stream_type=packed.F32),
                    dict(rows=0, x=0, y=A, x_out=A, h=0, stream_type=packed.F32)):
         assert message("norm", **change) == "null engine", change
+
+
+def test_the_documents_examples_name_their_stream():
+    # The null stream, which a call without one means, does not wait for PyTorch's other
+    # streams, nor they for it: an example on the current stream passes it in every call.
+    found = 0
+    for path in glob.glob(os.path.join(calls.ROOT, "*.md")):
+        with open(path) as f:
+            blocks = re.findall(r"```python\n(.*?)```", f.read(), re.S)
+        for block in blocks:
+            for node in ast.walk(ast.parse(block)):
+                name = getattr(getattr(node, "func", None), "attr", "")
+                if name.startswith("packed_") and not name.endswith("_workspace"):
+                    found += 1
+                    assert len(node.args) == 2, f"{os.path.basename(path)}: {name} without a stream"
+    assert found >= 3
