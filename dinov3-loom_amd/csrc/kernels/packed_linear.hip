@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * WAVES) void packed_shrink_kernel(DHX_SHRINK_PA
     constexpr int COLS = 16 * RB, XB = 2, TILE = 16 * XB;
     typedef Stream<T, RB, XB, WAVES, 4> S;
     __shared__ __attribute__((aligned(16))) T s0[WAVES * S::STAGE], s1[WAVES * S::STAGE], s2[WAVES * S::STAGE], s3[WAVES * S::STAGE];
-    __shared__ float sum[WAVES][TILE][COLS + 4];
+    __shared__ __attribute__((aligned(16))) float sum[WAVES][TILE][COLS + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int at = lane % TILE, l16 = lane & 15, part = lane >> 4;
     const int row0 = blockIdx.x * TILE;
@@ -621,7 +621,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void packed_linear_few_kernel(DHX_L
     typedef Stream<T, 1, MB, kFewWaves, NST> S;
     constexpr int LDS = kFewWaves * S::STAGE;
     __shared__ __attribute__((aligned(16))) T s0[LDS], s1[LDS], s2[LDS], s3[NST > 3 ? LDS : 8];
-    __shared__ float sum[kFewWaves][ROWS][20];
+    __shared__ __attribute__((aligned(16))) float sum[kFewWaves][ROWS][20];
     __shared__ int sRun[ROWS], sList[ROWS], sCount[kFewWaves], sOdd;  // sOdd: some value of B is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, part = lane >> 4;

@@ -499,7 +499,7 @@ __global__ __launch_bounds__(64 * kFewProductWaves) void packed_product_few_kern
     static_assert(ROWS % (LOADS * SIDE) == 0, "no row behind the last");
     constexpr int PITCH = QUADS * 64 + 16, SCALES = QUADS * 4;  // bytes of a row's codes, and of its scales
     __shared__ __attribute__((aligned(16))) char all_codes[WAVES * ROWS * PITCH], all_scales[WAVES * ROWS * SCALES];
-    __shared__ float sum[AB][WAVES][ROWS][20];
+    __shared__ __attribute__((aligned(16))) float sum[AB][WAVES][ROWS][20];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, part = lane >> 4;
     char *const codes = all_codes + wave * ROWS * PITCH, *const scales = all_scales + wave * ROWS * SCALES;
