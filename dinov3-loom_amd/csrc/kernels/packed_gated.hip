@@ -137,7 +137,6 @@ uint64_t packed_gated_bytes(const dhx_packed_gated& p) {
 
 hipError_t launch_packed_gated(const dhx_packed_gated& p, hipStream_t s) {
     Product a{};
-    a.type = p.type;
     a.activation = p.activation;
     a.rows = (uint32_t)p.rows;
     a.outputs = p.outputs;

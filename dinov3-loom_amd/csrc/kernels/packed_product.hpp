@@ -16,7 +16,7 @@ namespace dhx {
 // What a launcher hands on; strides are in bytes but that of out. xs_stride: from 32
 // blocks' scales of all rows to the next 32's.
 struct Product {
-    uint32_t type, activation, rows, pieces, outputs, sequences;
+    uint32_t activation, rows, pieces, outputs, sequences;
     const void *x, *w, *up;             // up: gated only
     const void *xs, *ws, *us;           // scales: 4-bit only
     const float *bias, *up_bias;

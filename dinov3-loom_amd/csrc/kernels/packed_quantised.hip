@@ -35,7 +35,6 @@ uint64_t packed_quantised_linear_bytes(const dhx_packed_quantised_linear& p) {
 
 hipError_t launch_packed_quantised_linear(const dhx_packed_quantised_linear& p, hipStream_t s) {
     Product a{};
-    a.type = p.type;
     a.rows = (uint32_t)p.rows;
     a.outputs = p.outputs;
     a.sequences = p.sequences;

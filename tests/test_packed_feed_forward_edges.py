@@ -9,6 +9,7 @@ import re
 import pytest
 
 import test_packed_feed_forward as calls
+from test_dma_wait_order import KERNELS
 from dinov3_hrx import packed
 from test_packed_feed_forward import PLAIN, A, message
 
@@ -50,3 +51,14 @@ def test_the_documents_examples_name_their_stream():
                     found += 1
                     assert len(node.args) == 2, f"{os.path.basename(path)}: {name} without a stream"
     assert found >= 3
+
+
+def test_launchers_hand_on_nothing_unread():
+    # Each field of what a product's launcher hands on is read by the launches.
+    with open(os.path.join(KERNELS, "packed_product.hpp")) as f:
+        source = f.read()
+    fields = re.search(r"struct Product \{(.*?)\n\};", source, re.S).group(1)
+    names = re.findall(r"[ *](\w+)[,;]", re.sub(r"//.*", "", fields))
+    assert len(names) > 15
+    for name in names:
+        assert re.search(rf"\bp\.{name}\b", source), name
