@@ -1,6 +1,7 @@
 """The operators of the feed-forward half of a packed block at edges of their
-definitions: float32 rows of one value, outputs in the place
-of inputs, activations far from zero. Tolerances as in packed_feed_forward.py."""
+definitions: float32 rows of one value, outputs in the place of inputs, activations
+far from zero, forms of the kernels that few sizes take. Tolerances as in
+packed_feed_forward.py."""
 import math
 
 import pytest
@@ -9,6 +10,8 @@ torch = pytest.importorskip("torch")
 
 import dinov3_hrx as d  # noqa: E402
 
+import packed_block  # noqa: E402
+import packed_feed_forward  # noqa: E402
 from packed_feed_forward import ACTIVATIONS, activation_want, norm_want, run_gated, run_norm  # noqa: E402
 from packed_operators import F, TYPES, gen, normal, within  # noqa: E402
 
@@ -143,3 +146,24 @@ def test_activations_far_from_zero(eng, t, activation, bits, rows):
     e = e * up_bias.double().abs()
     want = want * up_bias.double()
     within(out, want.expand(rows, outputs), (e + F * want.abs()).expand(rows, outputs), dt)
+
+
+# --- routes ------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("post,pre", [("none", "layer"), ("rms", "rms"), ("layer", "layer"), ("rms", "none")])
+@pytest.mark.parametrize("lengths,channels,which", [([5, 0, 2], 8200, 31), ([3], 12288, 5), ([1, 4], 16384, 26), ([3], 16392, 31),
+                                                    ([2, 2], 20000, 31), ([3], 32760, 21)])
+def test_norm_of_several_pieces_per_lane(eng, t, wide, post, pre, lengths, channels, which):
+    # Two and four pieces, the last of which some lanes lack.
+    packed_feed_forward.test_norm(eng, t, wide, post, pre, lengths, channels, which)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("kind", ["gated4", "linear4"])
+@pytest.mark.parametrize("rows,inputs,outputs", [(100, 1000, 1200), (40, 1504, 3000), (5, 2000, 9000), (3, 4096, 9000)])
+def test_few_rows_walk_several_outputs(eng, t, kind, rows, inputs, outputs):
+    # Each form of the few-rows kernel whose workgroups take a further block of outputs:
+    # 32 rows in steps of 4 and 8 blocks, 16 rows in steps of 8 and 16.
+    packed_block.test_routes(eng, t, kind, rows, inputs, outputs)
