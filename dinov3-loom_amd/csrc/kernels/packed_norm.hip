@@ -1,8 +1,9 @@
 // The residual step behind a block of a packed batch, with the norms before and
 // behind it (include/dinov3_packed.h): x' = x + gate[s] scale post(y), h =
 // pre(x'). Each row of x and y is read once and held in registers through both
-// norms, x' and h are written once, and there is little arithmetic, so the kernel
-// is bound by memory (few rows: by one row's chain of loads, sums and stores).
+// norms (over 16384 channels partly in scratch), x' and h are written once, and there is
+// little arithmetic, so the kernel is bound by memory (few rows: by one row's chain of
+// loads, sums and stores).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -123,14 +124,16 @@ __device__ __forceinline__ void vector8(const float* vector, int c, float none, 
 
 // One over the row's root of its mean square, of P pieces of 8 channels a lane
 // (zeros where a piece does not exist); for LayerNorm of the deviations from the
-// mean, which it leaves in v. Both sums are of registers.
+// mean, which it leaves in v.
 // A mean is off by some 30 roundings of itself (8 values of a lane, 6 steps across lanes, 16
 // waves), which deviations far smaller than the mean would show: a float32 row of one
 // value would have some, and its norm nothing else. Where the mean is more than 128 times
 // the deviations, which are exact so near to it, these are therefore taken from the first
 // of them, so that nothing is left of a row of one value, and then from their own mean.
 // Other rows pay a comparison (12864 rows of 384 channels 10.84 us without it and with;
-// held between every row's least and largest value, the mean would cost 0.5 us of it).
+// most where both norms wait for several waves: 4882 rows of 1024 12.5 and 13.0, 24 rows of
+// 8192 4.23 and 4.45; holding the mean between every row's least and largest value took
+// 11.4, 14.5 and 4.69).
 // part: 48 floats, of which the last 16 are any.
 template <int G, int P>
 __device__ __forceinline__ float inverse(float (&v)[P][8], const bool (&there)[P], int kind, float eps, int channels, float* part) {
@@ -287,7 +290,11 @@ hipError_t launch_pieces(const dhx_packed_norm& p, hipStream_t s) {
     const uint32_t pieces = p.channels / 8;
     // A lane per piece, and as few lanes as that leaves idle: 39 MB of 384 channels, 64
     // lanes 11.1 us, 32 lanes of two pieces 13.2, 128 lanes 18.4; of 2048, 256 lanes
-    // 11.3, 128 of two 11.5, 64 of four 19.5, 512 lanes 15.2.
+    // 11.3, 128 of two 11.5, 64 of four 19.5, 512 lanes 15.2. A workgroup has at most 1024
+    // lanes, so that longer rows are two and four pieces a lane, and four do not fit in a
+    // lane's 128 registers: 31 to 35 of them are kept in scratch (128 to 144 bytes a lane),
+    // and 39 MB of 32768 channels take 20.2 us where as many bytes of 4096 take 11.2, one
+    // row 17 us and 3.1.
     if (pieces <= 8) return launch<T, S, 8, 1>(p, s);
     if (pieces <= 16) return launch<T, S, 16, 1>(p, s);
     if (pieces <= 32) return launch<T, S, 32, 1>(p, s);

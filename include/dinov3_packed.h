@@ -163,7 +163,8 @@ int dhx_packed_attention_run(dhx_engine *e, const dhx_packed_attention *p, void 
  * h does not see x_out's rounding to its type. A row with a value that is not
  * finite has outputs that are not, others are not touched by it; a row whose
  * squares pass the range of float32 gives zeros (v / infinity) or NaN, and one whose
- * mean square (LayerNorm: variance) and eps are both 0 gives NaN.
+ * mean square (LayerNorm: variance) and eps are both 0 gives NaN (or infinities, where only
+ * the squares are 0 in float32).
  * x_out and h may each be x or y of the same type with the same stride (in place),
  * but not both the same. */
 enum { DHX_NORM_NONE = 0, DHX_NORM_RMS = 1, DHX_NORM_LAYER = 2 };
@@ -247,9 +248,10 @@ int dhx_packed_quantised_linear_run(dhx_engine *e, const dhx_packed_quantised_li
  * act(g) = g / (1 + e^-g) (SILU), g (1 + erf(g / sqrt 2)) / 2 (GELU), its form
  * g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 (GELU_TANH), max(g, 0) (RELU) or
  * 1 / (1 + e^-g) (SIGMOID). Both sums stay float32 up to the product, which is
- * rounded once. act(g) is float32's to a few roundings of itself, of its exponential's
- * argument (to 3e-5), and GELU's erf for negative g to 5e-5; where the factor beside g is
- * below 2^-126, act(g) may be 0. Where a sum is infinite or not a number, so may be the output.
+ * rounded once. act(g) itself is within 7e-5 of its value for any g (most far from 0:
+ * the argument of the exponential is rounded, and GELU's erfc fitted), and may be 0 where
+ * the factor beside g is below 2^-126. Where a sum is infinite or not a number, so may be
+ * the output.
  * The weights are of the type of x, or, with gate_scales and up_scales, 4-bit
  * codes as above; then x is quantised alike within the call, and only then is
  * there a workspace (of 0 bytes where rows are few). The matrices may be the halves of one. */
