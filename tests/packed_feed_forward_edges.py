@@ -78,6 +78,25 @@ def test_layer_norm_of_a_row_of_nearly_one_value(eng, t, channels):
     within(h, want, e, dt)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("channels", [8, 72, 136, 384, 1000, 12288])
+def test_rows_of_one_value_beside_others(eng, t, channels):
+    # Rows that share a wave with them have the same bits as without them.
+    dt = TYPES[t][1]
+    g = gen(channels)
+    x = normal(g, torch.float32, 67, channels, scale=2.0)
+    x[5, 0], x[9, channels - 1] = math.inf, math.nan
+    with_them, odd = x.clone(), torch.arange(67, device="cuda") % 3 == 1
+    with_them[odd] = torch.randn(67, 1, generator=g, device="cuda")[odd].expand(-1, channels)
+    alone, h = torch.empty(67, channels, dtype=dt, device="cuda"), torch.empty(67, channels, dtype=dt, device="cuda")
+    run_norm(eng, x, None, None, alone, "none", "layer", eps=(0.0, 1e-6))
+    run_norm(eng, with_them, None, None, h, "none", "layer", eps=(0.0, 1e-6))
+    torch.cuda.synchronize()
+    bits = lambda v: v[~odd].view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(h), bits(alone)) and (h[odd] == 0).all()
+    assert h[5].isnan().all() and h[9].isnan().all()
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("channels", [64, 384, 4096, 12288])
 def test_norm_in_place_the_other_way_round(eng, dt, channels):
